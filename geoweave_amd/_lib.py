@@ -155,6 +155,23 @@ _SIGNATURES = {
          _p, _p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64,
          ctypes.c_float, _p, _p, _sz, _p],
     ),
+    "gw_rotary_axes": (
+        ctypes.c_int,
+        [ctypes.c_int, _p, _i64p, _p, _i64p, _i64, _p, _i64p, _p, _i64p, _i64, ctypes.c_int, _p, _i64p,
+         _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_double),
+         ctypes.c_int, _p],
+    ),
+    "gw_packed_attn_fwd": (
+        ctypes.c_int,
+        [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _p, _i64p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+         ctypes.c_int, ctypes.c_float, _p],
+    ),
+    "gw_packed_attn_bwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "gw_packed_attn_bwd": (
+        ctypes.c_int,
+        [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _p, _i64p, _p, _i64p, _p, _p, _i64p, _p, _i64p,
+         _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_float, _p, _sz, _p],
+    ),
 }
 
 _lock = threading.Lock()
@@ -209,8 +226,18 @@ def strides3(*vals: int):
     return (ctypes.c_int64 * 3)(*[int(x) for x in vals])
 
 
+def strides2(*vals: int):
+    return (ctypes.c_int64 * 2)(*[int(x) for x in vals])
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (a launch goes to the current device, and
+    a caller's tensors may lie on another)."""
+    return torch.cuda.device(device)
 
 
 def stream_handle(device: torch.device) -> int:

@@ -1,0 +1,206 @@
+// Pieces shared by the packed and paged attention passes: where a workgroup's tile lies among
+// sequences of different lengths, LDS tiles that are read by rows and by columns, and loads that end at a
+// sequence's last row.
+#pragma once
+
+#include "gw_common.h"
+#include "gw_mma.h"
+
+namespace gw {
+namespace {
+
+typedef __fp16 pk_fp16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) pk_fp16x4 lds_pk_h4;
+
+// ---------------------------------------------------------------------------------------
+// Host checks that the packed entry points share.
+// ---------------------------------------------------------------------------------------
+struct PackedArgs {
+  int dtype;
+  int64_t n, Tq, Tk, Hq, Hk, D;
+  float scale;
+};
+
+inline int pk_check_args(const PackedArgs& a) {
+  GW_CHECK_ARG(a.dtype == GW_DTYPE_BF16 || a.dtype == GW_DTYPE_FP16, "unknown dtype %d", a.dtype);
+  if (a.D != 64 && a.D != 128) return set_error(GW_ERR_UNSUPPORTED, "head dim %lld is not 64 or 128", (long long)a.D);
+  GW_CHECK_ARG(a.n >= 0 && a.Tq >= 0 && a.Tk >= 0, "negative size");
+  GW_CHECK_ARG(a.Hk >= 1 && a.Hq >= a.Hk && a.Hq % a.Hk == 0, "%lld query heads are no multiple of %lld key heads",
+               (long long)a.Hq, (long long)a.Hk);
+  GW_CHECK_ARG(a.scale > 0.f && a.scale <= 3.0e38f, "the softmax scale must be positive and finite");
+  if (a.n >= (1ll << 30) || a.Tq > 0x7FFFFFFFll / a.Hq || a.Tk > 0x7FFFFFFFll / a.Hq)
+    return set_error(GW_ERR_UNSUPPORTED, "tokens x heads must stay below 2^31, sequences below 2^30");
+  return GW_OK;
+}
+
+// Strides {token, head} of a [T, H, D] tensor whose rows are read 16 bytes at a time; 64 rows lie
+// within a load's 32-bit offset.
+inline bool pk_rows_ok(const void* p, const int64_t* s) {
+  return aligned16(p) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[0] >= 0 && s[0] < (1ll << 24);
+}
+
+// ---------------------------------------------------------------------------------------
+// Sequences. cu[0..n] bounds the n sequences of T packed tokens. Tokens before cu[0] and behind
+// cu[n] belong to none: they are treated as sequences 0 and n + 1 without keys (or queries), so that
+// their outputs are written (as zeros) like all others. Bounds are clamped to [0, T], so whatever the
+// device array holds, no access leaves the tensors.
+//
+// Tiles without a list: sequence i, whose rows are tokens x g heads, may use the slots from
+// floor(start_i g / BM) + i on; the next sequence's first slot is at least ceil(rows_i / BM) later, and
+// there are floor(T g / BM) + n + 2 slots in all, a number that the host knows without the lengths. A
+// workgroup finds the sequence of its slot by a search with 64 probes at a time (a wave's lanes),
+// two rounds for up to 4,094 sequences; slots without a tile end at once.
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ int pk_bound(const int32_t* cu, int n, int T, int i) {
+  if (i <= 0) return 0;
+  if (i > n + 1) return T;
+  return min(max(cu[i - 1], 0), T);
+}
+
+struct PackedTile {
+  int seq;       // 0..n+1 (0 and n + 1: tokens of no sequence)
+  int start;     // first token
+  int len;       // tokens
+  int tile;      // tile of the sequence
+};
+
+__device__ __forceinline__ PackedTile pk_find_tile(const int32_t* cu, int n, int T, int g, int bm, int slot) {
+  const int lane = threadIdx.x & 63;
+  auto first_slot = [&](int i) { return (int)((uint64_t)((uint32_t)pk_bound(cu, n, T, i) * (uint64_t)g) / (uint32_t)bm) + i; };
+  int lo = 0, cnt = n + 2;
+  while (cnt > 1) {
+    const int step = (cnt + 63) >> 6;
+    const int i = lo + lane * step;
+    const bool below = lane * step < cnt && first_slot(i) <= slot;
+    const uint64_t bal = __builtin_amdgcn_ballot_w64(below);
+    const int top = bal ? 63 - __builtin_clzll(bal) : 0;
+    lo += top * step;
+    cnt = min(step, cnt - top * step);
+  }
+  PackedTile r;
+  r.seq = __builtin_amdgcn_readfirstlane(lo);
+  r.start = __builtin_amdgcn_readfirstlane(pk_bound(cu, n, T, r.seq));
+  r.len = max(0, __builtin_amdgcn_readfirstlane(pk_bound(cu, n, T, r.seq + 1)) - r.start);
+  r.tile = slot - __builtin_amdgcn_readfirstlane(first_slot(r.seq));
+  return r;
+}
+
+// The other side's tokens of sequence seq (none for 0 and n + 1).
+__device__ __forceinline__ void pk_other(const int32_t* cu, int n, int T, int seq, int& start, int& len) {
+  start = len = 0;
+  if (seq >= 1 && seq <= n) {
+    start = __builtin_amdgcn_readfirstlane(pk_bound(cu, n, T, seq));
+    len = max(0, __builtin_amdgcn_readfirstlane(pk_bound(cu, n, T, seq + 1)) - start);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// LDS tiles of rows of 2 D bytes: the 16-byte chunk c of row R sits at c ^ pk_swz(R). Sixteen
+// consecutive rows at one chunk (row operands) touch all banks evenly, and so do four rows,
+// starting at a multiple of four, at four consecutive chunks (column operands).
+// ---------------------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ int pk_swz(int R) {
+  if constexpr (D == 64)
+    return (((R >> 1) & 1) << 2) | (((R >> 2) & 1) << 1) | ((R & 1) ^ ((R >> 3) & 1));
+  else
+    return ((R & 3) << 2) | ((R >> 2) & 3);
+}
+
+// A descriptor of `bytes` bytes at a wave-uniform base: loads past them give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t pk_rsrc(const char* base, int64_t bytes) {
+  const uint32_t n = (uint32_t)min(max(bytes, (int64_t)0), (int64_t)0xFFFFFFFF);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(uniform_ptr(base)), (short)0,
+                                           (int)__builtin_amdgcn_readfirstlane(n), 0x00020000);
+}
+
+// Row tiles of one head of one sequence: 64 rows at a time from memory straight to LDS. Lane i of a
+// wave writes 16 bytes at the wave's segment + 16 i, so it reads the chunk that the swizzle keeps there.
+// Rows past the sequence's end arrive as zeros.
+template <int D, int THREADS>
+struct PkRows {
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kChunks = D / 8;                       // 16-byte chunks of a row
+  static constexpr int kRowsPerPass = THREADS / kChunks;      // rows of one 16-byte load per thread
+  static constexpr int kPasses = 64 / kRowsPerPass;
+  const char* base;
+  int64_t bytes;       // from base to the end of the last row
+  uint32_t stride;     // bytes
+  uint32_t off;        // this lane's offset in pass 0
+  uint32_t seg;        // this wave's segment of the tile in pass 0
+
+  __device__ __forceinline__ void init(const void* p, int64_t stride_elems, int rows, int tid) {
+    base = uniform_ptr(static_cast<const char*>(p));
+    stride = (uint32_t)stride_elems * 2u;
+    bytes = rows > 0 ? (int64_t)(rows - 1) * stride + kRowBytes : 0;
+    const int row = tid / kChunks, c = tid % kChunks;
+    static_assert(kRowsPerPass % 16 == 0, "the swizzle repeats every 16 rows");
+    off = (uint32_t)row * stride + (uint32_t)((c ^ pk_swz<D>(row)) * 16);
+    seg = (uint32_t)(tid >> 6) * 1024u;
+  }
+  // Rows [64 n, 64 n + 64) to lds.
+  __device__ __forceinline__ void load(int n, uint8_t* lds) const {
+    const int64_t at = (int64_t)n * 64 * stride;
+    const __amdgpu_buffer_rsrc_t rs = pk_rsrc(base + at, bytes - at);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(lds + seg + i * kRowsPerPass * kRowBytes), 16,
+          (int)(off + (uint32_t)(i * kRowsPerPass) * stride), 0, 0, 0);
+  }
+};
+
+// Operand quads of a tile in LDS for the 32x32x16 products.
+// Rows: lane l supplies row 32 st + l % 32, elements 16 ks + 8 (l / 32) + 0..7.
+template <int D>
+__device__ __forceinline__ uint4 pk_row_quad(const uint8_t* tile, int st, int ks, int lane) {
+  const int col = lane & 31, half = lane >> 5;
+  return *reinterpret_cast<const uint4*>(tile + st * 32 * 2 * D + col * 2 * D + (((2 * ks + half) ^ pk_swz<D>(col)) << 4));
+}
+// Columns: lane l supplies column 32 db + l % 32 of rows 32 st + 16 ks + 4 (l / 32) + {0..3, 8..11}: the
+// rows that the accumulator entries 8 ks + 0..7 of lane l stand for, so that those, packed to 16
+// bits, are the other operand as they are. Two transposing reads (16 lanes read 4 rows of 32 bytes
+// and receive a column each).
+template <int D>
+__device__ __forceinline__ uint4 pk_col_quad(const uint8_t* tile, int st, int ks, int db, int lane) {
+  const int i = lane & 15, dh = (lane >> 4) & 1, half = lane >> 5;
+  uint2 q[2];
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {
+    const int r = 8 * jj + 4 * half + (i >> 2);  // within 16 rows
+    const int c = 4 * db + 2 * dh + ((i & 3) >> 1);
+    const uint8_t* a = tile + (32 * st + 16 * ks + r) * 2 * D + ((c ^ pk_swz<D>(r)) << 4) + 8 * (i & 1);
+    q[jj] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_pk_h4*)(a)));
+  }
+  return make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
+}
+
+// Stores a lane's column of a transposed accumulator (32 dims of one row) scaled by f: lanes l and
+// l ^ 32 exchange quads so that each stores eight consecutive dims.
+template <typename E>
+__device__ __forceinline__ void pk_store_col(uint16_t* row, const f32x16& acc, float f, int half, bool on) {
+#pragma unroll
+  for (int gp = 0; gp < 2; ++gp) {
+    uint32_t w[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = 4 * (2 * gp + u);
+      w[u][0] = pack_pair(E{}, acc[r] * f, acc[r + 1] * f);
+      w[u][1] = pack_pair(E{}, acc[r + 2] * f, acc[r + 3] * f);
+    }
+    const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+    if (on) *reinterpret_cast<uint4*>(row + 8 * (2 * gp + half)) = make_uint4(x[0], y[0], x[1], y[1]);
+  }
+}
+
+// Waits for this wave's loads and LDS accesses, then for the other waves.
+__device__ __forceinline__ void pk_tile_barrier() {
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+}  // namespace
+}  // namespace gw

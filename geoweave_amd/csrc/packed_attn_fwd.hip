@@ -1,0 +1,272 @@
+// Attention over packed sequences of different lengths, forward (gfx950): bidirectional or causal,
+// grouped heads, D = 64 or 128.
+//
+// For query token i of a sequence of Lq queries and Lk keys and head h (key head h / G):
+//   p_j = softmax_j(scale q_i . k_j) over j < Lk (causal: j <= i + Lk - Lq),  o_i = sum_j p_j v_j.
+// One pass over the keys with a running reference maximum m and sum l (held in fp32, in the exp2
+// domain): o = (sum_j 2^(s_j - m) v_j) / l. m is raised only when a lane's weights of 32 keys sum past
+// 2^15, so P fits fp16 and no maximum is taken per tile otherwise; the result does not depend on which m
+// was used. P is rounded to the inputs' 16-bit type for the second product (half a step, 2^-9 or 2^-12
+// of a weight, with errors that average out over the keys); sums add the fp32 weights.
+//
+// The rows of a key head are (token, head of the group), token-major, so a group's heads share the
+// K and V tiles. 4 waves per workgroup, each QPW blocks of 32 rows; tiles of 64 keys go from memory
+// straight to LDS, a tile ahead. Products are transposed (S^T = K Q^T, O^T += V^T P^T,
+// v_mfma_f32_32x32x16): a lane holds 16 keys of one row, the softmax stays in its registers and the
+// packed weights are the second product's operand as they are; V is read from its row-major tile by
+// transposing LDS reads. The next 32 keys' scores are issued before the current weights are formed.
+//
+// Rows of K and V behind a sequence's end arrive as zeros (the loads' descriptor ends there), so
+// what lies in memory behind it, inf and NaN included, cannot reach a result.
+#include <math.h>
+
+#include "gw_packed.h"
+
+namespace gw {
+namespace {
+
+constexpr float kPkSumCap = 32768.f;
+
+struct PackedFwdParams {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* o;
+  float* lse;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int n, Tq, Tk, H, Hk, G, causal;
+  int64_t qst, qsh, kst, ksh, vst, vsh, ost, osh;
+  float scale_log2;
+};
+
+template <typename E, int D, int QPW>
+__global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwdParams p) {
+  constexpr int KS = D / 16, DB = D / 32, BM = 128 * QPW;
+  constexpr int kTileBytes = 64 * 2 * D;
+  // Two buffers of each tile as arrays of their own, indexed at compile time: the compiler then
+  // knows which LDS reads a load in flight can overlap, and waits for none of them in the loop.
+  __shared__ __align__(16) uint8_t kt0[kTileBytes], kt1[kTileBytes], vt0[kTileBytes], vt1[kTileBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int hk = blockIdx.x % p.Hk;  // consecutive workgroups (different XCDs) take different heads
+  const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, p.G, BM, blockIdx.x / p.Hk);
+  const int rows = pt.len * p.G;  // fits: the host bounds Tq * H
+  const int ntile = (rows + BM - 1) / BM;
+  if (pt.tile >= ntile) return;
+  // Causal: the tiles with the most keys first.
+  const int row0 = (p.causal ? ntile - 1 - pt.tile : pt.tile) * BM;
+  int k0, lk;
+  pk_other(p.cu_k, p.n, p.Tk, pt.seq, k0, lk);
+  const int shift = lk - pt.len;  // causal: token i sees keys up to i + shift
+  const float sl2 = p.scale_log2;
+
+  // This lane's row of each block: its token and head, and its last key.
+  int lim[QPW], lim_lo[QPW];
+  int tok[QPW], head[QPW];
+  bool on[QPW];
+  uint4 qa[QPW][KS];
+#pragma unroll
+  for (int a = 0; a < QPW; ++a) {
+    const int base = row0 + (wave * QPW + a) * 32;
+    const int r = min(base + col, rows - 1);
+    on[a] = base + col < rows;
+    tok[a] = r / p.G;
+    head[a] = hk * p.G + (r - tok[a] * p.G);
+    lim[a] = p.causal ? min(tok[a] + shift, lk - 1) : lk - 1;
+    lim_lo[a] = __builtin_amdgcn_readfirstlane(lim[a]);  // rows are token-major: the block's first is its least
+    const uint16_t* qr = p.q + (int64_t)(pt.start + tok[a]) * p.qst + (int64_t)head[a] * p.qsh + half * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qa[a][ks] = *reinterpret_cast<const uint4*>(qr + ks * 16);
+  }
+  // The last keys of the wave's and of the workgroup's last row.
+  auto last_key = [&](int r) { return p.causal ? min(min(r, rows - 1) / p.G + shift, lk - 1) : lk - 1; };
+  const int lim_wave = row0 + wave * QPW * 32 < rows ? last_key(row0 + (wave + 1) * QPW * 32 - 1) : -1;
+  const int keys = last_key(row0 + BM - 1) + 1;
+  const int ntk = keys > 0 ? (keys + 63) >> 6 : 0;
+
+  f32x16 acc[QPW][DB];
+  float m[QPW], l[QPW];  // m: the same in lanes l and l ^ 32; l: this lane's keys only
+#pragma unroll
+  for (int a = 0; a < QPW; ++a) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][db][r] = 0.f;
+    m[a] = -3.4028234663852886e38f;  // finite: s - m stays -inf at masked entries
+    l[a] = 0.f;
+  }
+
+  PkRows<D, 256> krows, vrows;
+  krows.init(p.k + (int64_t)k0 * p.kst + (int64_t)hk * p.ksh, p.kst, lk, tid);
+  vrows.init(p.v + (int64_t)k0 * p.vst + (int64_t)hk * p.vsh, p.vst, lk, tid);
+
+  auto sub_qk = [&](const uint8_t* kt, int st, int j0, f32x16 (&s)[QPW]) __attribute__((always_inline)) {
+    uint4 ka[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ka[ks] = pk_row_quad<D>(kt, st, ks, lane);
+#pragma unroll
+    for (int a = 0; a < QPW; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[a][r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int a = 0; a < QPW; ++a) s[a] = mma(E{}, ka[ks], qa[a][ks], s[a]);
+#pragma unroll
+    for (int a = 0; a < QPW; ++a) {
+      if (j0 + 31 > lim_lo[a]) {
+        const int room = lim[a] - j0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[a][r] = 8 * (r / 4) + r % 4 <= room ? s[a][r] : -INFINITY;
+      }
+    }
+  };
+  auto sub_pv = [&](const uint8_t* vt, int st, f32x16 (&s)[QPW]) __attribute__((always_inline)) {
+    uint4 va[DB][2];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) va[db][ks] = pk_col_quad<D>(vt, st, ks, db, lane);
+#pragma unroll
+    for (int a = 0; a < QPW; ++a) {
+      uint4 pb[2];
+      auto weights = [&](float nm) __attribute__((always_inline)) {
+        float w[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] = fexp2(fmaf(s[a][r], sl2, nm));
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) pb[ks] = pack_quad<E>(w + 8 * ks);
+        float t[2] = {w[0], w[8]};
+#pragma unroll
+        for (int r = 1; r < 8; ++r) {
+          t[0] += w[r];
+          t[1] += w[8 + r];
+        }
+        return t[0] + t[1];
+      };
+      float ls = weights(-m[a]);
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= kPkSumCap)) != 0ull, 0)) {
+        // A row's weights have grown past the cap (or these are its first keys): every row of the
+        // block moves its reference to its largest score here if that is higher.
+        float mx = s[a][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[a][r]);
+        const float mn = fmaxf(m[a], pair_max(mx) * sl2);
+        const float alpha = fexp2(m[a] - mn);
+        m[a] = mn;
+        l[a] *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[a][db][r] *= alpha;
+        ls = weights(-mn);
+      }
+      l[a] += ls;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[a][db] = mma(E{}, va[db][ks], pb[ks], acc[a][db]);
+    }
+  };
+
+  if (ntk > 0) {
+    krows.load(0, kt0);
+    vrows.load(0, vt0);
+    pk_tile_barrier();
+    auto tile = [&](int n, const uint8_t* kc, const uint8_t* vc, uint8_t* kn, uint8_t* vn) __attribute__((always_inline)) {
+      // Past the end the last tile again, into the buffer that no wave reads any more.
+      krows.load(min(n + 1, ntk - 1), kn);
+      vrows.load(min(n + 1, ntk - 1), vn);
+      if (64 * n <= lim_wave) {
+        f32x16 s0[QPW], s1[QPW];
+        sub_qk(kc, 0, 64 * n, s0);
+        sub_qk(kc, 1, 64 * n + 32, s1);
+        sub_pv(vc, 0, s0);
+        sub_pv(vc, 1, s1);
+      }
+      pk_tile_barrier();
+    };
+    int n = 0;
+#pragma unroll 1
+    for (; n + 1 < ntk; n += 2) {
+      tile(n, kt0, vt0, kt1, vt1);
+      tile(n + 1, kt1, vt1, kt0, vt0);
+    }
+    if (n < ntk) tile(n, kt0, vt0, kt1, vt1);
+  }
+
+  // o = O / l, lse = (m + log2 l) ln 2.
+#pragma unroll
+  for (int a = 0; a < QPW; ++a) {
+    const float lt = pair_sum(l[a]);
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;  // no keys: o = 0; NaN stays NaN
+    uint16_t* orow = p.o + (int64_t)(pt.start + tok[a]) * p.ost + (int64_t)head[a] * p.osh;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) pk_store_col<E>(orow + 32 * db, acc[a][db], inv, half, on[a]);
+    if (on[a] && half == 0 && p.lse)
+      p.lse[(int64_t)(pt.start + tok[a]) * p.H + head[a]] = lt == 0.f ? -INFINITY : (m[a] + flog2(lt)) * kDLn2;
+  }
+}
+
+template <typename E, int D, int QPW>
+int packed_fwd_launch(const PackedFwdParams& p, hipStream_t stream) {
+  const int64_t slots = (int64_t)p.Tq * p.G / (128 * QPW) + p.n + 2;
+  GW_CHECK_ARG(slots * p.Hk < (1ll << 31), "grid of %lld workgroups is too large", (long long)(slots * p.Hk));
+  hipLaunchKernelGGL((packed_attn_fwd_kernel<E, D, QPW>), dim3((uint32_t)(slots * p.Hk)), dim3(256), 0, stream, p);
+  GW_HIP_LAUNCH_CHECK("gw_packed_attn_fwd");
+  return GW_OK;
+}
+
+template <typename E>
+int packed_fwd_dim(const PackedFwdParams& p, int64_t D, hipStream_t stream) {
+  return D == 64 ? packed_fwd_launch<E, 64, 2>(p, stream) : packed_fwd_launch<E, 128, 1>(p, stream);
+}
+
+}  // namespace
+}  // namespace gw
+
+extern "C" int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
+                                  const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                  const int32_t* cu_q, const int32_t* cu_k, void* o, const int64_t* o_strides,
+                                  float* lse, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                                  int causal, float softmax_scale, void* stream) {
+  using namespace gw;
+  clear_error();
+  PackedArgs a = {dtype, n, Tq, Tk, Hq, Hk, D, softmax_scale};
+  const int rc = pk_check_args(a);
+  if (rc != GW_OK) return rc;
+  if (Tq == 0) return GW_OK;
+  GW_CHECK_ARG(q && o && cu_q && cu_k && q_strides && k_strides && v_strides && o_strides && (Tk == 0 || (k && v)),
+               "a tensor is missing");
+  GW_CHECK_ARG(pk_rows_ok(q, q_strides) && pk_rows_ok(k, k_strides) && pk_rows_ok(v, v_strides) && pk_rows_ok(o, o_strides),
+               "q, k, v and o need 16-byte aligned rows, with token strides in [0, 2^24)");
+  PackedFwdParams p = {};
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.o = static_cast<uint16_t*>(o);
+  p.lse = lse;
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.n = (int)n;
+  p.Tq = (int)Tq;
+  p.Tk = (int)Tk;
+  p.H = (int)Hq;
+  p.Hk = (int)Hk;
+  p.G = (int)(Hq / Hk);
+  p.causal = causal != 0;
+  p.qst = q_strides[0];
+  p.qsh = q_strides[1];
+  p.kst = k_strides[0];
+  p.ksh = k_strides[1];
+  p.vst = v_strides[0];
+  p.vsh = v_strides[1];
+  p.ost = o_strides[0];
+  p.osh = o_strides[1];
+  p.scale_log2 = softmax_scale * kDLog2e;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == GW_DTYPE_BF16 ? packed_fwd_dim<BF16>(p, D, s) : packed_fwd_dim<FP16>(p, D, s);
+}

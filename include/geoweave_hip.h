@@ -634,6 +634,61 @@ int gw_sparse_attn_bwd_dense(int dtype,
                              void* workspace, size_t workspace_bytes,
                              void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Rotary positions with several axes (view, row, column, ...), on up to two tensors (q and
+ * k) in one pass.
+ *
+ * x0 [B, T, H0, D] and x1 [B, T, H1, D] through {stride_b, stride_t, stride_h}; y0, y1 the
+ * outputs of the same shapes (the same memory as the input is allowed where the strides are the
+ * same too). H1 = 0: one tensor. pos: element (b, t, a) of axis a through {stride_b, stride_t,
+ * stride_a}, of type pos_type. axis_dims (host): dims of each axis's block, even, one block
+ * behind the other from dim 0; an even number of dims may remain behind them and is copied.
+ * bases (host): positive. Dims i and i + d/2 of an axis's block of d turn by
+ * pos * base^(-2 i / d), by the negative of it with inverse != 0 (the gradient).
+ * dtype bf16, fp16 or fp32; D <= 256, up to 8 axes; B <= 65535. Angles are formed in 64 bits.
+ * ------------------------------------------------------------------------------------ */
+#define GW_POS_INT32 0
+#define GW_POS_INT64 1
+#define GW_POS_FP32 2
+int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strides, void* y0, const int64_t* y0_strides,
+                   int64_t H0, const void* x1, const int64_t* x1_strides, void* y1, const int64_t* y1_strides,
+                   int64_t H1, int pos_type, const void* pos, const int64_t* pos_strides,
+                   int64_t B, int64_t T, int64_t D, int n_axes, const int32_t* axis_dims, const double* bases,
+                   int inverse, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Attention over packed sequences of different lengths, forward.
+ *
+ * q [Tq, Hq, D], k and v [Tk, Hk, D] through {stride_t, stride_h}, Hq a multiple of Hk (query head
+ * h reads key head h / (Hq / Hk)). cu_q, cu_k: int32 [n + 1] on the device, non-decreasing:
+ * sequence i has the query tokens [cu_q[i], cu_q[i + 1]) and the keys [cu_k[i], cu_k[i + 1]). A
+ * query attends to its sequence's keys, causal != 0: key j <= i + Lk - Lq (i, j within the sequence).
+ * A row with no key, and a token in no sequence, gets o = 0, lse = -inf. lse (nullable): fp32
+ * [Tq, Hq], natural log. Bounds outside [0, Tq] or [0, Tk] are clamped.
+ * D in {64, 128}, bf16 or fp16, softmax_scale > 0; 16-byte aligned rows, token strides in [0, 2^24)
+ * elements; tokens x Hq below 2^31. Nothing is read from the device by the host: a captured graph may
+ * be replayed with other bounds of the same n.
+ * ------------------------------------------------------------------------------------ */
+int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, const int32_t* cu_q, const int32_t* cu_k,
+                       void* o, const int64_t* o_strides, float* lse, int64_t n, int64_t Tq, int64_t Tk,
+                       int64_t Hq, int64_t Hk, int64_t D, int causal, float softmax_scale, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Backward of gw_packed_attn_fwd: dq [Tq, Hq, D], dk and dv [Tk, Hk, D] (each element written once;
+ * tokens of no sequence, and rows without keys, get zeros) from the forward's o and lse and the
+ * gradient dout of o. No float atomics: the same inputs give the same bits. Arguments and limits as
+ * there. workspace: gw_packed_attn_bwd_workspace_size(...) bytes, 16-byte aligned.
+ * ------------------------------------------------------------------------------------ */
+size_t gw_packed_attn_bwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
+int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, const int32_t* cu_q, const int32_t* cu_k,
+                       const void* o, const int64_t* o_strides, const void* dout, const int64_t* do_strides,
+                       const float* lse, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides,
+                       void* dv, const int64_t* dv_strides, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq,
+                       int64_t Hk, int64_t D, int causal, float softmax_scale, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
