@@ -28,8 +28,8 @@ inline int pk_check_args(const PackedArgs& a) {
   GW_CHECK_ARG(a.Hk >= 1 && a.Hq >= a.Hk && a.Hq % a.Hk == 0, "%lld query heads are no multiple of %lld key heads",
                (long long)a.Hq, (long long)a.Hk);
   GW_CHECK_ARG(a.scale > 0.f && a.scale <= 3.0e38f, "the softmax scale must be positive and finite");
-  if (a.n >= (1ll << 30) || a.Tq > 0x7FFFFFFFll / a.Hq || a.Tk > 0x7FFFFFFFll / a.Hq)
-    return set_error(GW_ERR_UNSUPPORTED, "tokens x heads must stay below 2^31, sequences below 2^30");
+  if (a.n >= (1ll << 30) || a.Tq > 0x7FFFF000ll / a.Hq || a.Tk > 0x7FFFF000ll / a.Hq)
+    return set_error(GW_ERR_UNSUPPORTED, "tokens x heads must stay below 2^31 - 2^12, sequences below 2^30");
   return GW_OK;
 }
 

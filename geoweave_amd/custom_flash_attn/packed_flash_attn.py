@@ -33,6 +33,7 @@ __all__ = ["packed_flash_attn_func", "packed_flash_attn_inference_func", "Packed
 
 # The kernels' 32-bit load offsets bound a token stride (64 rows of a tile).
 MAX_ROW_STRIDE = 1 << 24
+MAX_TOKEN_HEADS = 0x7FFFF000
 
 
 def _check_heads(q, k, v):
@@ -74,8 +75,8 @@ def _check_inputs(q, k, v, cu_q, cu_k, softmax_scale):
             raise ValueError(f"cu_seqlens must be [sequences + 1], got {tuple(cu.shape)}")
     if cu_q.numel() != cu_k.numel():
         raise ValueError(f"cu_seqlens of {cu_q.numel() - 1} and {cu_k.numel() - 1} sequences")
-    if max(q.shape[0], k.shape[0]) * q.shape[1] >= 1 << 31:
-        raise ValueError("tokens x query heads must stay below 2^31")
+    if max(q.shape[0], k.shape[0]) * q.shape[1] > MAX_TOKEN_HEADS:
+        raise ValueError(f"tokens x query heads must not exceed {MAX_TOKEN_HEADS}")
     if not (q.is_cuda and all(t.device == q.device for t in (k, v, cu_q, cu_k))):
         raise ValueError("q, k, v and cu_seqlens must be tensors of one GPU")
     return cu_q.contiguous(), cu_k.contiguous(), _check_scale(softmax_scale, q.shape[-1])

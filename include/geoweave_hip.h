@@ -689,6 +689,28 @@ int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const
                        int64_t Hk, int64_t D, int causal, float softmax_scale, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Attention of a few new tokens per sequence over a paged key-value cache, split over the cache's
+ * length and joined.
+ *
+ * q and o [B, N, Hq, D] through {stride_b, stride_t, stride_h}; k and v [pages, page_size, Hk, D]
+ * through {stride_page, stride_slot, stride_h}; block_table int32 [B, table_width] (row stride
+ * table_stride, unit column stride): sequence b's key j is slot j % page_size of page
+ * block_table[b][j / page_size]; lens int32 [B]: its keys, the new tokens' own included (values
+ * outside [0, table_width * page_size] are clamped). Key of a page outside [0, pages): seen by nobody.
+ * causal != 0: new token i of N sees the keys below lens - N + 1 + i, else all. A row with no key gets
+ * o = 0, lse = -inf. lse (nullable): fp32 [B, N, Hq], natural log.
+ * D in {64, 128}, bf16 or fp16, softmax_scale > 0, 16-byte aligned rows, table_width * page_size and
+ * B * N * Hq below 2^31 - 2^12. workspace: gw_paged_attn_fwd_workspace_size(...) bytes, 16-byte
+ * aligned. Nothing is read from the device by the host: a captured graph follows the table and lengths.
+ * ------------------------------------------------------------------------------------ */
+size_t gw_paged_attn_fwd_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D);
+int gw_paged_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                      const void* v, const int64_t* v_strides, const int32_t* block_table, int64_t table_stride,
+                      const int32_t* lens, void* o, const int64_t* o_strides, float* lse, int64_t B, int64_t N,
+                      int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size, int64_t table_width,
+                      int causal, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
