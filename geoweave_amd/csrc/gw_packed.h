@@ -85,6 +85,24 @@ __device__ __forceinline__ PackedTile pk_find_tile(const int32_t* cu, int n, int
   return r;
 }
 
+// The sequence of token t (a search per lane).
+__device__ __forceinline__ PackedTile pk_token(const int32_t* cu, int n, int T, int t) {
+  int lo = 0, hi = n + 2;  // the sequence lies in [lo, hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pk_bound(cu, n, T, mid) <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  PackedTile r;
+  r.seq = lo;
+  r.start = pk_bound(cu, n, T, lo);
+  r.len = max(0, pk_bound(cu, n, T, lo + 1) - r.start);
+  r.tile = 0;
+  return r;
+}
+
 // The other side's tokens of sequence seq (none for 0 and n + 1).
 __device__ __forceinline__ void pk_other(const int32_t* cu, int n, int T, int seq, int& start, int& len) {
   start = len = 0;

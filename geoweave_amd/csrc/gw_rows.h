@@ -12,8 +12,8 @@ struct RowsParams {
   const uint16_t* v;
   uint16_t* o;
   float* lse;           // nullable
-  float* part;          // parts: [slot][Hk][16][D] normalised outputs, then [slot][Hk][16] log2 sums
-  float* part_lse;
+  float* part;          // parts of cut row tiles: [slot][Hk][16][D] normalised outputs,
+  float* part_lse;      // [slot][Hk][16] log2 sums
   // Paged: table [B][table_width] page numbers (row stride table_stride), lens [B].
   const int32_t* table;
   const int32_t* lens;
@@ -25,19 +25,22 @@ struct RowsParams {
   int n;                // sequences (paged: B)
   int Tq, Tk;           // packed: tokens; paged: Tq = new tokens of a sequence
   int H, Hk, G, causal;
-  int split;            // 0: one workgroup takes all keys of its rows
-  int want;             // workgroups per key head to aim at (split)
+  int split;            // 0: one workgroup takes all keys of its rows (paged only)
+  int want;             // parts per key head to aim at (split)
   int64_t qsb, qst, qsh, osb, ost, osh;   // packed: qsb = osb = 0
   int64_t ksp, kst, ksh, vsp, vst, vsh;   // per page (packed: 0), token, head
   float scale_log2;
 };
 
-// Row tiles (16 rows of a key head) of all sequences at most.
-int64_t rows_tiles(bool paged, int64_t n, int64_t Tq, int64_t G);
-// Slots per key head at most, and the workspace that the parts take.
-int64_t rows_slots(const RowsParams& p, bool paged);
-size_t rows_workspace(int64_t slots, int64_t Hk, int64_t D);
-// Launches on checked arguments (dtype bf16 or fp16, D 64 or 128).
+// Packed: sequences of at most this many rows (tokens x heads of a group) are this kernel's.
+constexpr int kRowsMax = 32;
+
+// Parts per key head to aim at: about four workgroups per CU over all heads.
+inline int rows_want(int64_t Hk) { return (int)(1024 / Hk > 0 ? 1024 / Hk : 1); }
+// Workspace of the parts of a split call. A tile is cut where its keys exceed the part length, so it
+// has fewer than two parts per part length of keys, and all cut tiles fewer than 2 want.
+inline size_t rows_workspace(int64_t Hk, int64_t D) { return (size_t)2 * rows_want(Hk) * Hk * 16 * (D + 1) * sizeof(float); }
+// Launches on checked arguments (dtype bf16 or fp16, D 64 or 128); p.split and p.want are set.
 int rows_attn(int dtype, int D, bool paged, RowsParams p, void* workspace, hipStream_t stream);
 
 }  // namespace gw

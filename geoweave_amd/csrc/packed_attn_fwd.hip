@@ -21,6 +21,7 @@
 #include <math.h>
 
 #include "gw_packed.h"
+#include "gw_rows.h"
 
 namespace gw {
 namespace {
@@ -36,6 +37,10 @@ struct PackedFwdParams {
   const int32_t* cu_q;
   const int32_t* cu_k;
   int n, Tq, Tk, H, Hk, G, causal;
+  int skip_rows;      // sequences of at most this many rows are another kernel's
+  int split;          // parts that a tile's keys are cut into
+  float* part;        // split > 1: [part][Tq][H][D] outputs, [part][Tq][H] log2 sums
+  float* part_lse;
   int64_t qst, qsh, kst, ksh, vst, vsh, ost, osh;
   float scale_log2;
 };
@@ -55,7 +60,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
   const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, p.G, BM, blockIdx.x / p.Hk);
   const int rows = pt.len * p.G;  // fits: the host bounds Tq * H
   const int ntile = (rows + BM - 1) / BM;
-  if (pt.tile >= ntile) return;
+  if (pt.tile >= ntile || rows <= p.skip_rows) return;
   // Causal: the tiles with the most keys first.
   const int row0 = (p.causal ? ntile - 1 - pt.tile : pt.tile) * BM;
   int k0, lk;
@@ -85,7 +90,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
   auto last_key = [&](int r) { return p.causal ? min(min(r, rows - 1) / p.G + shift, lk - 1) : lk - 1; };
   const int lim_wave = row0 + wave * QPW * 32 < rows ? last_key(row0 + (wave + 1) * QPW * 32 - 1) : -1;
   const int keys = last_key(row0 + BM - 1) + 1;
-  const int ntk = keys > 0 ? (keys + 63) >> 6 : 0;
+  // This part's tiles of 64 keys.
+  const int all = keys > 0 ? (keys + 63) >> 6 : 0;
+  const int per = p.split > 1 ? (all + p.split - 1) / p.split : all;
+  const int tk0 = min((int)blockIdx.y * per, all), ntk = min(per, all - tk0);
 
   f32x16 acc[QPW][DB];
   float m[QPW], l[QPW];  // m: the same in lanes l and l ^ 32; l: this lane's keys only
@@ -173,17 +181,18 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
   };
 
   if (ntk > 0) {
-    krows.load(0, kt0);
-    vrows.load(0, vt0);
+    krows.load(tk0, kt0);
+    vrows.load(tk0, vt0);
     pk_tile_barrier();
     auto tile = [&](int n, const uint8_t* kc, const uint8_t* vc, uint8_t* kn, uint8_t* vn) __attribute__((always_inline)) {
       // Past the end the last tile again, into the buffer that no wave reads any more.
-      krows.load(min(n + 1, ntk - 1), kn);
-      vrows.load(min(n + 1, ntk - 1), vn);
-      if (64 * n <= lim_wave) {
+      krows.load(tk0 + min(n + 1, ntk - 1), kn);
+      vrows.load(tk0 + min(n + 1, ntk - 1), vn);
+      const int j0 = 64 * (tk0 + n);
+      if (j0 <= lim_wave) {
         f32x16 s0[QPW], s1[QPW];
-        sub_qk(kc, 0, 64 * n, s0);
-        sub_qk(kc, 1, 64 * n + 32, s1);
+        sub_qk(kc, 0, j0, s0);
+        sub_qk(kc, 1, j0 + 32, s1);
         sub_pv(vc, 0, s0);
         sub_pv(vc, 1, s1);
       }
@@ -198,41 +207,140 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
     if (n < ntk) tile(n, kt0, vt0, kt1, vt1);
   }
 
-  // o = O / l, lse = (m + log2 l) ln 2.
+  // o = O / l, lse = (m + log2 l) ln 2; a part keeps its o in fp32 and its log2 sum.
 #pragma unroll
   for (int a = 0; a < QPW; ++a) {
     const float lt = pair_sum(l[a]);
     const float inv = lt == 0.f ? 0.f : 1.f / lt;  // no keys: o = 0; NaN stays NaN
-    uint16_t* orow = p.o + (int64_t)(pt.start + tok[a]) * p.ost + (int64_t)head[a] * p.osh;
+    const int64_t t = pt.start + tok[a];
+    if (p.split > 1) {
+      if (!on[a]) continue;
+      const int64_t at = ((int64_t)blockIdx.y * p.Tq + t) * p.H + head[a];
+      if (half == 0) p.part_lse[at] = lt == 0.f ? -INFINITY : m[a] + flog2(lt);
+      if (lt == 0.f) continue;  // a part without weight is not read
+      float* dst = p.part + at * D + 4 * half;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(dst + 32 * db + 8 * g) =
+              make_float4(acc[a][db][4 * g] * inv, acc[a][db][4 * g + 1] * inv, acc[a][db][4 * g + 2] * inv,
+                          acc[a][db][4 * g + 3] * inv);
+      continue;
+    }
+    uint16_t* orow = p.o + t * p.ost + (int64_t)head[a] * p.osh;
 #pragma unroll
     for (int db = 0; db < DB; ++db) pk_store_col<E>(orow + 32 * db, acc[a][db], inv, half, on[a]);
-    if (on[a] && half == 0 && p.lse)
-      p.lse[(int64_t)(pt.start + tok[a]) * p.H + head[a]] = lt == 0.f ? -INFINITY : (m[a] + flog2(lt)) * kDLn2;
+    if (on[a] && half == 0 && p.lse) p.lse[t * p.H + head[a]] = lt == 0.f ? -INFINITY : (m[a] + flog2(lt)) * kDLn2;
   }
+}
+
+// Joins the parts of each row (token, head): D / 4 threads of four dims, parts in order.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void packed_join_kernel(const PackedFwdParams p) {
+  constexpr int LPR = D / 4;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int c = threadIdx.x % LPR;
+  const int64_t total = (int64_t)p.Tq * p.H;
+  if (row >= total) return;
+  const int64_t t = row / p.H;
+  const int head = (int)(row - t * p.H);
+  if (p.skip_rows > 0) {
+    const PackedTile pt = pk_token(p.cu_q, p.n, p.Tq, (int)t);
+    if (pt.len * p.G <= p.skip_rows) return;
+  }
+  float mx = -INFINITY, lt = 0.f;
+  bool nan = false;
+  for (int i = 0; i < p.split; ++i) {
+    const float x = p.part_lse[i * total + row];
+    nan |= x != x;
+    mx = fmaxf(mx, x);
+  }
+  if (nan) mx = NAN;
+  float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < p.split; ++i) {
+    const float x = p.part_lse[i * total + row];
+    if (x == -INFINITY) continue;
+    const float f = fexp2(x - mx);
+    const float4 y = reinterpret_cast<const float4*>(p.part + (i * total + row) * D)[c];
+    lt += f;
+    out.x = fmaf(y.x, f, out.x);
+    out.y = fmaf(y.y, f, out.y);
+    out.z = fmaf(y.z, f, out.z);
+    out.w = fmaf(y.w, f, out.w);
+  }
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  *reinterpret_cast<uint2*>(p.o + t * p.ost + (int64_t)head * p.osh + 4 * c) =
+      make_uint2(pack_pair(E{}, out.x * inv, out.y * inv), pack_pair(E{}, out.z * inv, out.w * inv));
+  if (c == 0 && p.lse) p.lse[row] = lt == 0.f ? -INFINITY : (mx + flog2(lt)) * kDLn2;
+}
+
+// What a call launches, from the sizes that the host knows.
+// - Few-rows kernel (rows_attn_fwd.hip): where a sequence's rows are few on average and its keys many, the
+//   sequences of at most kRowsMax rows are split over all workgroups there; the tile kernel skips them.
+// - Tile kernel: rows in blocks of 128 (D = 64: or 256), and the keys of each tile cut into `split` parts
+//   where the tiles alone leave workgroup slots (two per CU) empty.
+struct FwdPlan {
+  bool rows, tiles;
+  int qpw, split;
+  size_t rows_bytes, split_bytes;
+};
+
+FwdPlan packed_fwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
+  FwdPlan f = {};
+  const int64_t G = Hq / Hk, rows = Tq * G, seqs = n > 0 ? n : 1, keys = Tk / seqs;
+  f.rows = n <= 1024 && rows / seqs <= 128 && keys >= 512;
+  f.tiles = !f.rows || rows > kRowsMax;
+  const int64_t big = (rows / 256 + n) * Hk;
+  f.qpw = D == 64 && big >= 1024 ? 2 : 1;
+  const int64_t wgs = (rows / (128 * f.qpw) + (rows / seqs < 128 ? n : n / 2) + 1) * Hk;
+  int64_t split = 512 / (wgs > 0 ? wgs : 1);
+  if (split > keys / 512) split = keys / 512;
+  if (split > 16) split = 16;
+  f.split = split > 1 ? (int)split : 1;
+  f.rows_bytes = f.rows ? (rows_workspace(Hk, D) + 255) / 256 * 256 : 0;
+  f.split_bytes = f.tiles && f.split > 1 ? (size_t)f.split * Tq * Hq * (D + 1) * sizeof(float) : 0;
+  return f;
 }
 
 template <typename E, int D, int QPW>
 int packed_fwd_launch(const PackedFwdParams& p, hipStream_t stream) {
   const int64_t slots = (int64_t)p.Tq * p.G / (128 * QPW) + p.n + 2;
   GW_CHECK_ARG(slots * p.Hk < (1ll << 31), "grid of %lld workgroups is too large", (long long)(slots * p.Hk));
-  hipLaunchKernelGGL((packed_attn_fwd_kernel<E, D, QPW>), dim3((uint32_t)(slots * p.Hk)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((packed_attn_fwd_kernel<E, D, QPW>), dim3((uint32_t)(slots * p.Hk), (uint32_t)p.split), dim3(256), 0,
+                     stream, p);
   GW_HIP_LAUNCH_CHECK("gw_packed_attn_fwd");
+  if (p.split > 1) {
+    constexpr int kRowsPerWg = 256 / (D / 4);
+    const int64_t wgs = ((int64_t)p.Tq * p.H + kRowsPerWg - 1) / kRowsPerWg;
+    hipLaunchKernelGGL((packed_join_kernel<E, D>), dim3((uint32_t)wgs), dim3(256), 0, stream, p);
+    GW_HIP_LAUNCH_CHECK("gw_packed_attn_fwd (join)");
+  }
   return GW_OK;
 }
 
 template <typename E>
-int packed_fwd_dim(const PackedFwdParams& p, int64_t D, hipStream_t stream) {
-  return D == 64 ? packed_fwd_launch<E, 64, 2>(p, stream) : packed_fwd_launch<E, 128, 1>(p, stream);
+int packed_fwd_dim(const PackedFwdParams& p, int64_t D, int qpw, hipStream_t stream) {
+  if (D == 128) return packed_fwd_launch<E, 128, 1>(p, stream);
+  return qpw == 2 ? packed_fwd_launch<E, 64, 2>(p, stream) : packed_fwd_launch<E, 64, 1>(p, stream);
 }
 
 }  // namespace
 }  // namespace gw
 
+extern "C" size_t gw_packed_attn_fwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
+  if (n < 0 || Tq < 1 || Tk < 0 || Hk < 1 || Hq < Hk || D < 1) return 0;
+  const gw::FwdPlan f = gw::packed_fwd_plan(n, Tq, Tk, Hq, Hk, D);
+  return f.rows_bytes + f.split_bytes;
+}
+
 extern "C" int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
                                   const int64_t* k_strides, const void* v, const int64_t* v_strides,
                                   const int32_t* cu_q, const int32_t* cu_k, void* o, const int64_t* o_strides,
                                   float* lse, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
-                                  int causal, float softmax_scale, void* stream) {
+                                  int causal, float softmax_scale, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   using namespace gw;
   clear_error();
   PackedArgs a = {dtype, n, Tq, Tk, Hq, Hk, D, softmax_scale};
@@ -267,6 +375,46 @@ extern "C" int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_str
   p.ost = o_strides[0];
   p.osh = o_strides[1];
   p.scale_log2 = softmax_scale * kDLog2e;
+  const FwdPlan f = packed_fwd_plan(n, Tq, Tk, Hq, Hk, D);
+  GW_CHECK_ARG(f.rows_bytes + f.split_bytes == 0 ||
+                   (workspace && aligned16(workspace) && workspace_bytes >= f.rows_bytes + f.split_bytes),
+               "workspace of %zu bytes, %zu are needed", workspace_bytes, f.rows_bytes + f.split_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == GW_DTYPE_BF16 ? packed_fwd_dim<BF16>(p, D, s) : packed_fwd_dim<FP16>(p, D, s);
+  if (f.rows) {
+    RowsParams r = {};
+    r.q = p.q;
+    r.k = p.k;
+    r.v = p.v;
+    r.o = p.o;
+    r.lse = lse;
+    r.cu_q = cu_q;
+    r.cu_k = cu_k;
+    r.n = p.n;
+    r.Tq = p.Tq;
+    r.Tk = p.Tk;
+    r.H = p.H;
+    r.Hk = p.Hk;
+    r.G = p.G;
+    r.causal = p.causal;
+    r.split = 1;
+    r.want = rows_want(Hk);
+    r.qst = p.qst;
+    r.qsh = p.qsh;
+    r.ost = p.ost;
+    r.osh = p.osh;
+    r.kst = p.kst;
+    r.ksh = p.ksh;
+    r.vst = p.vst;
+    r.vsh = p.vsh;
+    r.scale_log2 = p.scale_log2;
+    const int rr = rows_attn(dtype, (int)D, false, r, workspace, s);
+    if (rr != GW_OK || !f.tiles) return rr;
+    p.skip_rows = kRowsMax;
+  }
+  p.split = f.split;
+  if (f.split > 1) {
+    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + f.rows_bytes);
+    p.part_lse = p.part + (int64_t)f.split * Tq * Hq * D;
+  }
+  return dtype == GW_DTYPE_BF16 ? packed_fwd_dim<BF16>(p, D, f.qpw, s) : packed_fwd_dim<FP16>(p, D, f.qpw, s);
 }

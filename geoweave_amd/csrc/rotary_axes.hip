@@ -17,6 +17,7 @@
 // issued before the angles are formed. V is the widest of 8, 4, 2, 1 elements that divides every
 // half block and every stride.
 #include <math.h>
+#include <string.h>
 
 #include "gw_common.h"
 
@@ -178,6 +179,30 @@ __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(const RotParam
   }
 }
 
+// The angles' factors of the calling thread's last axes (64 powers cost more host time than the rest of a
+// call; a layer stack turns by the same axes throughout).
+struct RotFreqs {
+  int n_axes = -1;
+  int32_t dims[kRotMaxAxes];
+  double bases[kRotMaxAxes];
+  double freq[kRotMaxPairs];
+};
+
+const double* rot_freqs(int n_axes, const int32_t* dims, const double* bases) {
+  static thread_local RotFreqs t;
+  if (t.n_axes == n_axes && memcmp(t.dims, dims, n_axes * sizeof(int32_t)) == 0 &&
+      memcmp(t.bases, bases, n_axes * sizeof(double)) == 0)
+    return t.freq;
+  t.n_axes = n_axes;
+  int pair = 0;
+  for (int a = 0; a < n_axes; ++a) {
+    t.dims[a] = dims[a];
+    t.bases[a] = bases[a];
+    for (int i = 0; i < dims[a] / 2; ++i) t.freq[pair++] = pow(bases[a], -2.0 * i / dims[a]) / 6.283185307179586476925;
+  }
+  return t.freq;
+}
+
 template <typename E>
 int rot_launch(const RotParams& p, int V, hipStream_t stream) {
   const dim3 grid((p.T + p.TT - 1) / p.TT, p.B);
@@ -265,15 +290,13 @@ extern "C" int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strid
       p.pair[group] = (int16_t)(a < n_axes ? pair + i : kRotMaxPairs);
     }
     if (a < n_axes) {
-      for (int i = 0; i < half; ++i) {
-        p.axis[pair + i] = (uint8_t)a;
-        p.freq[pair + i] = pow(bases[a], -2.0 * i / n) / 6.283185307179586476925;
-      }
+      for (int i = 0; i < half; ++i) p.axis[pair + i] = (uint8_t)a;
       pair += half;
     }
     dim += n;
   }
   p.pairs = pair;
+  memcpy(p.freq, rot_freqs(n_axes, axis_dims, bases), pair * sizeof(double));
   p.groups = group;
   p.pos = pos;
   p.pos_type = pos_type;

@@ -91,9 +91,16 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
 struct RowsPart {
   int seq, tile;    // seq < 0: nothing to do
   int part, parts;  // of this row tile
-  int first;        // slot of the row tile's part 0
+  int first;        // where the part 0 of a cut row tile is kept
   int len;          // keys of a part
 };
+
+// Row tiles of a sequence: packed, those of the longer ones are another kernel's.
+template <bool PAGED>
+__device__ __forceinline__ int rows_tiles_of(const RowsParams& p, const RowsSeq& s) {
+  const int rows = s.lq * p.G;
+  return PAGED || rows <= kRowsMax ? (rows + kRows - 1) / kRows : 0;
+}
 
 // Keys of a part: about p.want parts over all row tiles.
 template <bool PAGED>
@@ -102,14 +109,14 @@ __device__ __forceinline__ int rows_part_len(const RowsParams& p, int lane) {
   int64_t total = 0;
   for (int i = lane; i < nseq; i += 64) {
     const RowsSeq s = rows_seq<PAGED>(p, i);
-    total += (int64_t)((s.lq * p.G + kRows - 1) / kRows) * s.lk;
+    total += (int64_t)rows_tiles_of<PAGED>(p, s) * s.lk;
   }
   total = wave_sum64(total);
   const int64_t len = (total + p.want - 1) / p.want;
   return (int)((max(len, (int64_t)kRowsPart) + kRowsPart - 1) / kRowsPart * kRowsPart);
 }
 
-// The part of slot `slot`, or (tile_index) all parts of the row tile of that number.
+// The part of slot `slot`, or (tile_index) the row tile of that number.
 template <bool PAGED>
 __device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, bool tile_index, int lane) {
   RowsPart r = {-1, 0, 0, 1, 0, 0x7fffff80};
@@ -117,38 +124,35 @@ __device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, boo
     const int rt = (p.Tq * p.G + kRows - 1) / kRows;
     r.seq = slot / rt;
     r.tile = slot - r.seq * rt;
-    r.first = slot;
     if (r.seq >= p.n) r.seq = -1;
     return r;
   }
   r.len = rows_part_len<PAGED>(p, lane);
   const int nseq = rows_nseq<PAGED>(p);
-  int before = 0, slots_before = 0;
+  int before = 0, cut_before = 0;
   for (int i0 = 0; i0 < nseq; i0 += 64) {
     const int i = i0 + lane;
     int tiles = 0, parts = 1;
     if (i < nseq) {
       const RowsSeq s = rows_seq<PAGED>(p, i);
-      tiles = (s.lq * p.G + kRows - 1) / kRows;
+      tiles = rows_tiles_of<PAGED>(p, s);
       parts = max(1, (int)(((int64_t)s.lk + r.len - 1) / r.len));
     }
-    const int mine = tile_index ? tiles : tiles * parts;
-    const int incl = wave_scan(mine, lane);
+    const int mine = tile_index ? tiles : tiles * parts, cut = parts > 1 ? tiles * parts : 0;
+    const int incl = wave_scan(mine, lane), cut_incl = wave_scan(cut, lane);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(before + incl > slot);
-    const int slots = tile_index ? wave_scan(tiles * parts, lane) : incl;
     if (hit) {
       const int l = __builtin_ctzll(hit);
       const int at = slot - before - (__shfl(incl, l) - __shfl(mine, l));
       r.parts = __shfl(parts, l);
       r.seq = i0 + l;
-      const int seq_first = slots_before + __shfl(slots, l) - __shfl(tiles * parts, l);
       r.tile = tile_index ? at : at / r.parts;
       r.part = tile_index ? 0 : at - r.tile * r.parts;
-      r.first = seq_first + r.tile * r.parts;
+      r.first = cut_before + (__shfl(cut_incl, l) - __shfl(cut, l)) + r.tile * r.parts;
       break;
     }
     before += __shfl(incl, 63);
-    slots_before += __shfl(slots, 63);
+    cut_before += __shfl(cut_incl, 63);
   }
   r.seq = __builtin_amdgcn_readfirstlane(r.seq);
   r.tile = __builtin_amdgcn_readfirstlane(r.tile);
@@ -380,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
   }
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
-  for (int u = 0; u < DV; ++u) out[u] *= inv;
+  for (int u = 0; u < DV; ++u) out[u] = lt == 0.f ? 0.f : out[u] * inv;
   const float l2 = lt == 0.f ? -INFINITY : mx + flog2(lt);
   if (pt.parts > 1) {
     const int64_t at = ((int64_t)(pt.first + pt.part) * p.Hk + hk) * kRows + row;
@@ -399,50 +403,79 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
   if (c == 0 && p.lse) p.lse[(int64_t)(PAGED ? pt.seq * p.Tq + tk : sq.q0 + tk) * p.H + hd] = l2 * kDLn2;
 }
 
-// Joins the parts of one row tile of one key head: 16 threads per row, parts in order.
+// Joins the parts of one row of a cut row tile. D / 4 threads hold four dims each; the groups of them
+// take the parts in turn, each part's row one 16-byte load per thread, and are summed in group order.
+constexpr int kJoinParts = 1024;  // weights kept in LDS at a time
+
 template <typename E, int D, bool PAGED>
 __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
-  constexpr int DV = D / 16;
-  const int lane = threadIdx.x & 63;
-  const int hk = blockIdx.x % p.Hk;
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR;
+  __shared__ float w[kJoinParts];
+  __shared__ float red[4];
+  __shared__ float4 so[GROUPS][LPR];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int hk = blockIdx.x % p.Hk, row = blockIdx.y;
   const RowsPart pt = rows_find<PAGED>(p, blockIdx.x / p.Hk, true, lane);
   if (pt.seq < 0 || pt.parts == 1) return;
   const RowsSeq sq = rows_seq<PAGED>(p, pt.seq);
-  const int row = threadIdx.x >> 4, c = threadIdx.x & 15;
   const int rr = pt.tile * kRows + row;
   if (rr >= sq.lq * p.G) return;
   const int64_t step = (int64_t)p.Hk * kRows;
   const int64_t at = ((int64_t)pt.first * p.Hk + hk) * kRows + row;
+  // The largest log2 sum (NaN if one is).
   float mx = -INFINITY;
-  bool nan = false;
-  for (int i = 0; i < pt.parts; ++i) {
+  for (int i = tid; i < pt.parts; i += 256) {
     const float x = p.part_lse[at + i * step];
-    nan |= x != x;
-    mx = fmaxf(mx, x);
+    mx = x > mx || x != x ? x : mx;
+    if (mx != mx) break;
   }
-  if (nan) mx = NAN;
-  float lt = 0.f, out[DV];
+  auto top = [](float a, float b) { return a != a || a > b ? a : b; };
 #pragma unroll
-  for (int u = 0; u < DV; ++u) out[u] = 0.f;
-  if (mx != -INFINITY) {
-    for (int i = 0; i < pt.parts; ++i) {
-      const float x = p.part_lse[at + i * step];
-      if (x == -INFINITY) continue;  // no key of this part is seen
-      const float f = fexp2(x - mx);
-      lt += f;
-      const float* src = p.part + (at + i * step) * D + c * DV;
-#pragma unroll
-      for (int u = 0; u < DV; ++u) out[u] = fmaf(src[u], f, out[u]);
+  for (int d = 1; d < 64; d <<= 1) mx = top(mx, __shfl_xor(mx, d));
+  if (lane == 0) red[wave] = mx;
+  __syncthreads();
+  mx = top(top(red[0], red[1]), top(red[2], red[3]));
+  const int c = tid % LPR, grp = tid / LPR;
+  float lt = 0.f;
+  float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < pt.parts; p0 += kJoinParts) {
+    const int np = min(kJoinParts, pt.parts - p0);
+    __syncthreads();
+    for (int i = tid; i < np; i += 256) {
+      const float x = p.part_lse[at + (p0 + i) * step];
+      w[i] = x == -INFINITY ? 0.f : fexp2(x - mx);  // a part of which nothing is seen
     }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = grp; i < np; i += GROUPS) {
+      const float f = w[i];
+      const float4 x = reinterpret_cast<const float4*>(p.part + (at + (p0 + i) * step) * D)[c];
+      lt += f;
+      out.x = fmaf(x.x, f, out.x);
+      out.y = fmaf(x.y, f, out.y);
+      out.z = fmaf(x.z, f, out.z);
+      out.w = fmaf(x.w, f, out.w);
+    }
+  }
+  __shared__ float sl[GROUPS];
+  so[grp][c] = out;
+  if (c == 0) sl[grp] = lt;
+  __syncthreads();
+  if (grp != 0) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) {
+    const float4 x = so[i][c];
+    lt += sl[i];
+    out.x += x.x;
+    out.y += x.y;
+    out.z += x.z;
+    out.w += x.w;
   }
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
   const int tk = rr / p.G, hd = hk * p.G + (rr - tk * p.G);
   const int64_t tg = PAGED ? (int64_t)pt.seq * p.osb + (int64_t)tk * p.ost : (int64_t)(sq.q0 + tk) * p.ost;
-  uint16_t* dst = p.o + tg + (int64_t)hd * p.osh + c * DV;
-#pragma unroll
-  for (int u = 0; u < DV; u += 4)
-    *reinterpret_cast<uint2*>(dst + u) =
-        make_uint2(pack_pair(E{}, out[u] * inv, out[u + 1] * inv), pack_pair(E{}, out[u + 2] * inv, out[u + 3] * inv));
+  *reinterpret_cast<uint2*>(p.o + tg + (int64_t)hd * p.osh + c * 4) =
+      make_uint2(pack_pair(E{}, out.x * inv, out.y * inv), pack_pair(E{}, out.z * inv, out.w * inv));
   if (c == 0 && p.lse)
     p.lse[(int64_t)(PAGED ? pt.seq * p.Tq + tk : sq.q0 + tk) * p.H + hd] =
         lt == 0.f ? -INFINITY : (mx + flog2(lt)) * kDLn2;
@@ -450,13 +483,19 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
 
 template <typename E, int D, bool PAGED>
 int rows_launch(const RowsParams& p, hipStream_t stream) {
-  const int64_t grid = rows_slots(p, PAGED) * p.Hk;
+  // Row tiles at most: packed, one or two of each sequence of at most kRowsMax rows (and no more than
+  // the rows in all allow).
+  int64_t tiles = PAGED ? (int64_t)p.n * (((int64_t)p.Tq * p.G + kRows - 1) / kRows)
+                        : (int64_t)p.Tq * p.G / kRows + p.n + 2;
+  if (!PAGED) tiles = tiles < 2ll * (p.n + 2) ? tiles : 2ll * (p.n + 2);
+  const int64_t grid = (tiles + (p.split ? p.want : 0)) * p.Hk;
   GW_CHECK_ARG(grid < (1ll << 31), "grid of %lld workgroups is too large", (long long)grid);
   hipLaunchKernelGGL((rows_attn_kernel<E, D, PAGED>), dim3((uint32_t)grid), dim3(256), 0, stream, p);
   GW_HIP_LAUNCH_CHECK("rows attention");
   if (p.split) {
-    const int64_t tiles = rows_tiles(PAGED, p.n, p.Tq, p.G) * p.Hk;
-    hipLaunchKernelGGL((rows_join_kernel<E, D, PAGED>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
+    const int64_t rows = (int64_t)p.Tq * p.G;
+    hipLaunchKernelGGL((rows_join_kernel<E, D, PAGED>), dim3((uint32_t)(tiles * p.Hk), (uint32_t)(rows < kRows ? rows : kRows)),
+                       dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("rows attention (join)");
   }
   return GW_OK;
@@ -470,38 +509,25 @@ int rows_dim(int D, bool paged, const RowsParams& p, hipStream_t s) {
 
 }  // namespace
 
-int64_t rows_tiles(bool paged, int64_t n, int64_t Tq, int64_t G) {
-  return paged ? n * ((Tq * G + kRows - 1) / kRows) : Tq * G / kRows + n + 2;
-}
-
-int64_t rows_slots(const RowsParams& p, bool paged) {
-  const int64_t tiles = rows_tiles(paged, p.n, p.Tq, p.G);
-  return p.split ? tiles + p.want : tiles;
-}
-
-size_t rows_workspace(int64_t slots, int64_t Hk, int64_t D) { return (size_t)slots * Hk * kRows * (D + 1) * sizeof(float); }
-
 int rows_attn(int dtype, int D, bool paged, RowsParams p, void* workspace, hipStream_t stream) {
   if (p.split) {
     p.part = static_cast<float*>(workspace);
-    p.part_lse = p.part + rows_slots(p, paged) * p.Hk * kRows * D;
+    p.part_lse = p.part + (int64_t)2 * p.want * p.Hk * kRows * D;
   }
   return dtype == GW_DTYPE_BF16 ? rows_dim<BF16>(D, paged, p, stream) : rows_dim<FP16>(D, paged, p, stream);
 }
 
 }  // namespace gw
 
-// Workgroups per key head to aim at: about 4 per CU over all heads. Row tiles that reach four times
-// that are not split.
-static int rows_want(int64_t Hk) { return (int)(1024 / Hk > 0 ? 1024 / Hk : 1); }
-static bool rows_split_paged(int64_t B, int64_t N, int64_t Hq, int64_t Hk) {
-  return gw::rows_tiles(true, B, N, Hq / Hk) * Hk < 4096;
+// Row tiles that reach sixteen workgroups per CU are not split.
+static bool paged_split(int64_t B, int64_t N, int64_t Hq, int64_t Hk) {
+  return B * ((N * (Hq / Hk) + gw::kRows - 1) / gw::kRows) * Hk < 4096;
 }
 
 extern "C" size_t gw_paged_attn_fwd_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D) {
   using namespace gw;
-  if (B < 1 || N < 1 || Hk < 1 || Hq < Hk || D < 1 || !rows_split_paged(B, N, Hq, Hk)) return 0;
-  return rows_workspace(rows_tiles(true, B, N, Hq / Hk) + rows_want(Hk), Hk, D);
+  if (B < 1 || N < 1 || Hk < 1 || Hq < Hk || D < 1 || !paged_split(B, N, Hq, Hk)) return 0;
+  return rows_workspace(Hk, D);
 }
 
 extern "C" int gw_paged_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
@@ -562,7 +588,7 @@ extern "C" int gw_paged_attn_fwd(int dtype, const void* q, const int64_t* q_stri
   p.vst = v_strides[1];
   p.vsh = v_strides[2];
   p.scale_log2 = softmax_scale * kDLog2e;
-  p.split = rows_split_paged(B, N, Hq, Hk);
+  p.split = paged_split(B, N, Hq, Hk);
   p.want = rows_want(Hk);
   const size_t need = gw_paged_attn_fwd_workspace_size(B, N, Hq, Hk, D);
   GW_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),

@@ -84,14 +84,15 @@ def _check_inputs(q, k, v, cu_q, cu_k, softmax_scale):
 
 def _prep(x: torch.Tensor) -> torch.Tensor:
     # 16-byte rows, and a token stride within the kernels' offsets.
-    if (x.stride(-1) != 1 or any(s % 8 for s in x.stride()[:-1]) or x.data_ptr() % 16
-            or not 0 <= x.stride(0) < MAX_ROW_STRIDE):
+    st, sh, sd = x.stride()
+    if sd != 1 or st % 8 or sh % 8 or not 0 <= st < MAX_ROW_STRIDE or x.data_ptr() % 16:
         x = x.contiguous()
     return x
 
 
 def _rows(x: torch.Tensor):
-    return x.data_ptr(), _lib.strides2(x.stride(0), x.stride(1))
+    st, sh, _ = x.stride()
+    return x.data_ptr(), _lib.strides2(st, sh)
 
 
 def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool):
@@ -102,11 +103,13 @@ def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool):
     if q.shape[0] == 0:
         return o, lse
     lib = _lib.load()
+    sizes = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+    nbytes = int(lib.gw_packed_attn_fwd_workspace_size(*sizes))
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     with _lib.on_device(q.device):
         rc = lib.gw_packed_attn_fwd(_lib.dtype_code(q.dtype), *_rows(q), *_rows(k), *_rows(v), cu_q.data_ptr(),
-                                    cu_k.data_ptr(), *_rows(o), _lib.ptr(lse), cu_q.numel() - 1, q.shape[0],
-                                    k.shape[0], q.shape[1], k.shape[1], q.shape[2], int(causal), scale,
-                                    _lib.stream_handle(q.device))
+                                    cu_k.data_ptr(), *_rows(o), _lib.ptr(lse), *sizes, int(causal), scale,
+                                    _lib.ptr(ws), nbytes, _lib.stream_handle(q.device))
     _lib.check(rc, "gw_packed_attn_fwd")
     return o, lse
 
@@ -167,7 +170,6 @@ def packed_flash_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu
     return PackedFlashAttnFunc.apply(q, k, v, cu_q, cu_k, bool(causal), scale)
 
 
-@torch.inference_mode()
 def packed_flash_attn_inference_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
                                      cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = False,
                                      softmax_scale: Optional[float] = None, return_lse: bool = False,

@@ -58,7 +58,6 @@ def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens):
             raise ValueError("caches need a unit last stride and 16-byte aligned rows")
 
 
-@torch.inference_mode()
 def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                                     block_table: torch.Tensor, cache_seqlens: torch.Tensor, causal: bool = True,
                                     softmax_scale: Optional[float] = None, return_lse: bool = False,

@@ -10,6 +10,7 @@ of a layer are turned in one launch that forms each angle once.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Sequence, Tuple, Union
 
@@ -39,12 +40,20 @@ def view_grid_positions(views: int, grid_h: int, grid_w: int, n_special: int = 5
     return torch.stack([view.repeat_interleave(row.numel()), row.repeat(views), col.repeat(views)], dim=-1)
 
 
-def _as4(x: torch.Tensor) -> torch.Tensor:
-    return x.unsqueeze(0) if x.dim() == 3 else x
+@functools.lru_cache(maxsize=256)
+def _axis_args(axis_dims: Tuple[int, ...], bases: Tuple[float, ...]):
+    n = len(axis_dims)
+    return n, (ctypes.c_int32 * n)(*axis_dims), (ctypes.c_double * n)(*bases)
+
+
+def _strides(x: torch.Tensor):
+    """{batch, token, head or axis} strides; a tensor without a batch has one of one."""
+    st = x.stride()
+    return _lib.strides3(0, *st[-3:-1]) if x.dim() == 3 else _lib.strides3(*st[:3])
 
 
 def _check(q, k, positions, axis_dims, bases):
-    """Checked (axis_dims, bases, positions [B, T, A] view, B)."""
+    """Checked (axis_dims, bases)."""
     if q.dim() not in (3, 4):
         raise ValueError(f"expected [T, H, D] or [B, T, H, D], got {tuple(q.shape)}")
     if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
@@ -75,37 +84,29 @@ def _check(q, k, positions, axis_dims, bases):
         raise ValueError(f"positions {shape} must be {want}" + (f" or {want[-2:]}" if len(want) == 3 else ""))
     if not (q.is_cuda and positions.device == q.device and (k is None or k.device == q.device)):
         raise ValueError("q, k and positions must be tensors of one GPU")
-    if q.dim() == 4:
-        if len(shape) == 2:
-            positions = positions.unsqueeze(0).expand(q.shape[0], -1, -1)
-    else:
-        positions = positions.unsqueeze(0)
-    return axis_dims, bases, positions
+    return tuple(axis_dims), tuple(bases)
 
 
 def _rotate(xs, positions, axis_dims, bases, inverse: bool):
     """Turned copies (contiguous) of one or two tensors."""
     xs = [x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous() for x in xs]
     ys = [torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in xs]
-    a4, b4 = [_as4(x) for x in xs], [_as4(y) for y in ys]
-    B, T, _, D = a4[0].shape
-    if B == 0 or T == 0 or all(x.shape[2] == 0 for x in a4):
+    B = xs[0].shape[0] if xs[0].dim() == 4 else 1
+    T, D = xs[0].shape[-3], xs[0].shape[-1]
+    if B == 0 or T == 0 or all(x.shape[-2] == 0 for x in xs):
         return ys
     args = []
-    for i in range(2):
-        if i < len(xs):
-            args += [a4[i].data_ptr(), _lib.strides3(*a4[i].stride()[:3]), b4[i].data_ptr(),
-                     _lib.strides3(*b4[i].stride()[:3]), a4[i].shape[2]]
-        else:
-            args += [None, None, None, None, 0]
-    n = len(axis_dims)
+    for x, y in zip(xs, ys):
+        args += [x.data_ptr(), _strides(x), y.data_ptr(), _strides(y), x.shape[-2]]
+    if len(xs) == 1:
+        args += [None, None, None, None, 0]
+    pos_strides = _lib.strides3(*positions.stride()) if positions.dim() == 3 else _lib.strides3(0, *positions.stride())
     dev = xs[0].device
     code = _lib.dtype_code(xs[0].dtype, allow_fp32=True)
     lib = _lib.load()
     with _lib.on_device(dev):
-        rc = lib.gw_rotary_axes(code, *args, _POS_CODES[positions.dtype], positions.data_ptr(),
-                                _lib.strides3(*positions.stride()), B, T, D, n, (ctypes.c_int32 * n)(*axis_dims),
-                                (ctypes.c_double * n)(*bases), int(inverse), _lib.stream_handle(dev))
+        rc = lib.gw_rotary_axes(code, *args, _POS_CODES[positions.dtype], positions.data_ptr(), pos_strides, B, T, D,
+                                *_axis_args(axis_dims, bases), int(inverse), _lib.stream_handle(dev))
     _lib.check(rc, "gw_rotary_axes")
     return ys
 
@@ -136,13 +137,13 @@ def rotary_axes_func(x: torch.Tensor, positions: torch.Tensor, axis_dims: Sequen
     of its block of ``d = axis_dims[a]`` dims by ``positions[..., a] * bases[a] ** (-2 i / d)``. The
     blocks lie one behind the other; dims behind the last are copied. The result is contiguous.
     Differentiable in ``x``."""
-    axis_dims, bases, pos = _check(x, None, positions, axis_dims, bases)
-    return RotaryAxesFunc.apply(pos, axis_dims, bases, x)[0]
+    axis_dims, bases = _check(x, None, positions, axis_dims, bases)
+    return RotaryAxesFunc.apply(positions, axis_dims, bases, x)[0]
 
 
 def rotary_axes_qk_func(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axis_dims: Sequence[int],
                         bases: Union[float, Sequence[float]] = 100.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`rotary_axes_func` of a layer's q and k (their numbers of heads may differ) in one launch;
     either may be a column block of a fused projection."""
-    axis_dims, bases, pos = _check(q, k, positions, axis_dims, bases)
-    return RotaryAxesFunc.apply(pos, axis_dims, bases, q, k)
+    axis_dims, bases = _check(q, k, positions, axis_dims, bases)
+    return RotaryAxesFunc.apply(positions, axis_dims, bases, q, k)

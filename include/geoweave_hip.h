@@ -666,13 +666,16 @@ int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strides, void* y
  * A row with no key, and a token in no sequence, gets o = 0, lse = -inf. lse (nullable): fp32
  * [Tq, Hq], natural log. Bounds outside [0, Tq] or [0, Tk] are clamped.
  * D in {64, 128}, bf16 or fp16, softmax_scale > 0; 16-byte aligned rows, token strides in [0, 2^24)
- * elements; tokens x Hq below 2^31. Nothing is read from the device by the host: a captured graph may
+ * elements; tokens x Hq below 2^31 - 2^12. workspace: gw_packed_attn_fwd_workspace_size(...) bytes,
+ * 16-byte aligned (parts of the keys, where they are split over workgroups). Nothing is read from the device by the host: a captured graph may
  * be replayed with other bounds of the same n.
  * ------------------------------------------------------------------------------------ */
+size_t gw_packed_attn_fwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
 int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                        const void* v, const int64_t* v_strides, const int32_t* cu_q, const int32_t* cu_k,
                        void* o, const int64_t* o_strides, float* lse, int64_t n, int64_t Tq, int64_t Tk,
-                       int64_t Hq, int64_t Hk, int64_t D, int causal, float softmax_scale, void* stream);
+                       int64_t Hq, int64_t Hk, int64_t D, int causal, float softmax_scale, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------
  * Backward of gw_packed_attn_fwd: dq [Tq, Hq, D], dk and dv [Tk, Hk, D] (each element written once;

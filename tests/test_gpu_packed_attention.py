@@ -22,6 +22,9 @@ LENS = {
     "odd": ([1, 0, 5, 64, 65, 127, 128, 129, 300], None),
     "two sides": ([5, 0, 3, 130, 1, 70], [0, 7, 64, 130, 700, 33]),
     "tiles": ([256, 513, 31], None),
+    "few rows": ([3, 1, 40, 0, 2, 17], [2000, 777, 1500, 600, 33, 1300]),
+    "few rows only": ([2], [2700]),
+    "keys split": ([140, 150], [5000, 1201]),
 }
 
 
