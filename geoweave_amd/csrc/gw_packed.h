@@ -125,6 +125,11 @@ __device__ __forceinline__ int pk_swz(int R) {
     return ((R & 3) << 2) | ((R >> 2) & 3);
 }
 
+template <int V>
+struct PkInt {
+  static constexpr int value = V;
+};
+
 // A descriptor of `bytes` bytes at a wave-uniform base: loads past them give zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t pk_rsrc(const char* base, int64_t bytes) {
   const uint32_t n = (uint32_t)min(max(bytes, (int64_t)0), (int64_t)0xFFFFFFFF);
@@ -168,29 +173,69 @@ struct PkRows {
   }
 };
 
-// Operand quads of a tile in LDS for the 32x32x16 products.
-// Rows: lane l supplies row 32 st + l % 32, elements 16 ks + 8 (l / 32) + 0..7.
+// Operand quads of a tile in LDS for the 32x32x16 products, at byte offsets that a lane forms once (the
+// empty asm keeps the compiler from forming them again at every read). D = 128 keeps one offset of each
+// kind and flips its chunk bits per read.
 template <int D>
-__device__ __forceinline__ uint4 pk_row_quad(const uint8_t* tile, int st, int ks, int lane) {
-  const int col = lane & 31, half = lane >> 5;
-  return *reinterpret_cast<const uint4*>(tile + st * 32 * 2 * D + col * 2 * D + (((2 * ks + half) ^ pk_swz<D>(col)) << 4));
-}
-// Columns: lane l supplies column 32 db + l % 32 of rows 32 st + 16 ks + 4 (l / 32) + {0..3, 8..11}: the
-// rows that the accumulator entries 8 ks + 0..7 of lane l stand for, so that those, packed to 16
-// bits, are the other operand as they are. Two transposing reads (16 lanes read 4 rows of 32 bytes
-// and receive a column each).
-template <int D>
-__device__ __forceinline__ uint4 pk_col_quad(const uint8_t* tile, int st, int ks, int db, int lane) {
-  const int i = lane & 15, dh = (lane >> 4) & 1, half = lane >> 5;
-  uint2 q[2];
+struct PkLane {
+  static constexpr bool kKeep = D == 64;
+  static constexpr int kRowOffs = kKeep ? D / 16 : 1, kColOffs = kKeep ? D / 32 * 2 : 1;
+  static constexpr uint32_t kNext8 = D == 64 ? 16u : 32u;  // the swizzle of a row eight further on
+  uint32_t row_[kRowOffs], col_[kColOffs];
+
+  __device__ __forceinline__ explicit PkLane(int lane) {
+    const int col = lane & 31, half = lane >> 5;
+    const uint32_t r0 = (uint32_t)(col * 2 * D + ((half ^ pk_swz<D>(col)) << 4));
+    const int i = lane & 15, dh = (lane >> 4) & 1, r = 4 * half + (i >> 2);
+    const uint32_t c0 = (uint32_t)(r * 2 * D + (((2 * dh + ((i & 3) >> 1)) ^ pk_swz<D>(r)) << 4) + 8 * (i & 1));
 #pragma unroll
-  for (int jj = 0; jj < 2; ++jj) {
-    const int r = 8 * jj + 4 * half + (i >> 2);  // within 16 rows
-    const int c = 4 * db + 2 * dh + ((i & 3) >> 1);
-    const uint8_t* a = tile + (32 * st + 16 * ks + r) * 2 * D + ((c ^ pk_swz<D>(r)) << 4) + 8 * (i & 1);
-    q[jj] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_pk_h4*)(a)));
+    for (int ks = 0; ks < kRowOffs; ++ks) {
+      row_[ks] = r0 ^ (uint32_t)(ks << 5);
+      asm("" : "+v"(row_[ks]));
+    }
+#pragma unroll
+    for (int x = 0; x < kColOffs; ++x) {
+      col_[x] = c0 ^ (uint32_t)((x >> 1) << 6) ^ ((x & 1) ? kNext8 : 0u);
+      asm("" : "+v"(col_[x]));
+    }
   }
-  return make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
+  // Rows: lane l supplies row 32 st + l % 32, elements 16 ks + 8 (l / 32) + 0..7.
+  __device__ __forceinline__ uint4 row(const uint8_t* tile, int st, int ks) const {
+    const uint32_t o = kKeep ? row_[kKeep ? ks : 0] : row_[0] ^ (uint32_t)(ks << 5);
+    return *reinterpret_cast<const uint4*>(tile + st * 64 * D + o);
+  }
+  // Columns: lane l supplies column 32 db + l % 32 of rows 32 st + 16 ks + 4 (l / 32) + {0..3, 8..11}: the
+  // rows that the accumulator entries 8 ks + 0..7 of lane l stand for, so that those, packed to 16
+  // bits, are the other operand as they are. Two transposing reads (16 lanes read 4 rows of 32 bytes
+  // and receive a column each).
+  __device__ __forceinline__ uint4 col(const uint8_t* tile, int st, int ks, int db) const {
+    uint2 q[2];
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      const uint32_t o = kKeep ? col_[kKeep ? 2 * db + jj : 0] : col_[0] ^ (uint32_t)(db << 6) ^ (jj ? kNext8 : 0u);
+      q[jj] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                                            (lds_pk_h4*)(tile + (32 * st + 16 * ks + 8 * jj) * 2 * D + o)));
+    }
+    return make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
+  }
+};
+
+// Runs tiles 0..ntk - 1 in turn, the first nfull of them as tile(integral_constant 0, ...), the others as
+// (1, ...) (their entries need a mask), alternating between two buffers (an even tile in buffer 0).
+template <typename F>
+__device__ __forceinline__ void pk_tiles(int ntk, int nfull, F&& tile) {
+  int n = 0;
+#pragma unroll 1
+  for (; n + 1 < nfull; n += 2) {
+    tile(PkInt<0>{}, PkInt<0>{}, n);
+    tile(PkInt<0>{}, PkInt<1>{}, n + 1);
+  }
+#pragma unroll 1
+  for (; n + 1 < ntk; n += 2) {
+    tile(PkInt<1>{}, PkInt<0>{}, n);
+    tile(PkInt<1>{}, PkInt<1>{}, n + 1);
+  }
+  if (n < ntk) tile(PkInt<1>{}, PkInt<0>{}, n);
 }
 
 // Stores a lane's column of a transposed accumulator (32 dims of one row) scaled by f: lanes l and

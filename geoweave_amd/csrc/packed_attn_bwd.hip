@@ -35,9 +35,14 @@ struct PackedBwdParams {
   uint16_t* dq;
   uint16_t* dk;
   uint16_t* dv;
-  float2* stats;      // [H][Tq] {lse log2(e), +inf for a row without keys; delta}
+  float* nlse;        // [H][Tq] -lse / scale (fp16: + 14 / (scale log2 e)), -inf for a row without keys: the
+                      // products' start of S - lse / scale
+  float* ndelta;      // [H][Tq] -delta
   uint32_t* max_do;   // [n + 2][Hk] largest |do_i| of a sequence's rows, as float bits (fp16 only)
   uint32_t* max_v;    // [n + 2][Hk] largest |v_j|
+  int split_dq, split_dkv;  // parts that the passes' inner loops are cut into
+  float* part_dq;     // split_dq > 1: [part][Tq][H][D]
+  float* part_dkv;    // split_dkv > 1: [part][dk, dv][Tk][Hk][D]
   const int32_t* cu_q;
   const int32_t* cu_k;
   int n, Tq, Tk, H, Hk, G, causal;
@@ -45,6 +50,10 @@ struct PackedBwdParams {
   int64_t dqst, dqsh, dkst, dksh, dvst, dvsh;
   float scale, scale_log2;
 };
+
+// fp16: P enters its product times 2^14.
+template <typename E>
+constexpr float kPScale = __is_same(E, FP16) ? 14.f : 0.f;
 
 // Exponent e with 2 bound 2^e <= 2^15 (0 where there is no bound to speak of).
 __device__ __forceinline__ int pk_scale_exp(float bound) {
@@ -86,7 +95,9 @@ __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdPa
     if (MAXIMA) nn = group_sum<LPR>(nn);
     if (li == 0) {
       const float l = p.lse[(int64_t)t * p.H + h];
-      p.stats[(int64_t)h * p.Tq + t] = make_float2(l == -INFINITY ? INFINITY : l * kDLog2e, s);
+      const int64_t at = (int64_t)h * p.Tq + t;
+      p.nlse[at] = l == -INFINITY ? -INFINITY : (kPScale<E> - l * kDLog2e) / p.scale_log2;
+      p.ndelta[at] = -s;
       if (MAXIMA && nn < INFINITY) atomicMax(p.max_do + (int64_t)pt.seq * p.Hk + h / p.G, __float_as_uint(sqrtf(nn)));
     }
   }
@@ -111,12 +122,21 @@ __global__ __launch_bounds__(256) void packed_bwd_vmax_kernel(const PackedBwdPar
   }
 }
 
+// The same column in fp32.
+__device__ __forceinline__ void pk_store_part(float* row, const f32x16& acc, float f, int half, bool on) {
+  if (!on) return;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    *reinterpret_cast<float4*>(row + 8 * g + 4 * half) =
+        make_float4(acc[4 * g] * f, acc[4 * g + 1] * f, acc[4 * g + 2] * f, acc[4 * g + 3] * f);
+}
+
 // ---------------------------------------------------------------------------------------
 // dQ: the forward's decomposition.
 // ---------------------------------------------------------------------------------------
-template <typename E, int D, int QPW>
-__global__ __launch_bounds__(256, 2) void packed_bwd_dq_kernel(const PackedBwdParams p) {
-  constexpr int KS = D / 16, DB = D / 32, BM = 128 * QPW;
+template <typename E, int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(const PackedBwdParams p) {
+  constexpr int KS = D / 16, DB = D / 32, BM = 128;
   constexpr int kTileBytes = 64 * 2 * D;
   constexpr bool kFp16 = __is_same(E, FP16);
   __shared__ __align__(16) uint8_t kt0[kTileBytes], kt1[kTileBytes], vt0[kTileBytes], vt1[kTileBytes];
@@ -135,157 +155,168 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dq_kernel(const PackedBwdPa
   const int shift = lk - pt.len;
   const float sl2 = p.scale_log2;
 
-  int lim[QPW], lim_lo[QPW], tok[QPW], head[QPW];
-  bool on[QPW];
-  uint4 qa[QPW][KS], ga[QPW][KS];
-  float nlse[QPW], delta[QPW], unscale[QPW];
-#pragma unroll
-  for (int a = 0; a < QPW; ++a) {
-    const int base = row0 + (wave * QPW + a) * 32;
-    const int r = min(base + col, rows - 1);
-    on[a] = base + col < rows;
-    tok[a] = r / p.G;
-    head[a] = hk * p.G + (r - tok[a] * p.G);
-    lim[a] = p.causal ? min(tok[a] + shift, lk - 1) : lk - 1;
-    lim_lo[a] = __builtin_amdgcn_readfirstlane(lim[a]);
-    const int64_t t = pt.start + tok[a];
-    const uint16_t* qr = p.q + t * p.qst + (int64_t)head[a] * p.qsh + half * 8;
-    const uint16_t* gr = p.dout + t * p.gst + (int64_t)head[a] * p.gsh + half * 8;
-    float nn = 0.f;
+  const int base = row0 + wave * 32;
+  const bool on = base + col < rows;
+  const int row = min(base + col, rows - 1);
+  const int tok = row / p.G, head = hk * p.G + (row - tok * p.G);
+  const int lim = p.causal ? min(tok + shift, lk - 1) : lk - 1;
+  const int64_t t = pt.start + tok;
+  uint4 qa[KS], ga[KS];
+  float nn = 0.f;
+  {
+    const uint16_t* qr = p.q + t * p.qst + (int64_t)head * p.qsh + half * 8;
+    const uint16_t* gr = p.dout + t * p.gst + (int64_t)head * p.gsh + half * 8;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      qa[a][ks] = *reinterpret_cast<const uint4*>(qr + ks * 16);
-      ga[a][ks] = *reinterpret_cast<const uint4*>(gr + ks * 16);
-      if (kFp16) nn = dot2(E{}, ga[a][ks].x, ga[a][ks].x, dot2(E{}, ga[a][ks].y, ga[a][ks].y,
-                      dot2(E{}, ga[a][ks].z, ga[a][ks].z, dot2(E{}, ga[a][ks].w, ga[a][ks].w, nn))));
+      qa[ks] = *reinterpret_cast<const uint4*>(qr + ks * 16);
+      ga[ks] = *reinterpret_cast<const uint4*>(gr + ks * 16);
+      if (kFp16) nn += dot8<E>(ga[ks], ga[ks]);
     }
-    const float2 st = p.stats[(int64_t)head[a] * p.Tq + t];
-    int e = 0;
-    if (kFp16) e = pk_scale_exp(sqrtf(pair_sum(nn)) * __uint_as_float(p.max_v[(int64_t)pt.seq * p.Hk + hk]));
-    nlse[a] = (float)e - st.x;  // p 2^e = 2^(s - lse + e)
-    delta[a] = st.y;
-    unscale[a] = ldexpf(p.scale, -e);
   }
+  int e = 0;
+  if (kFp16) e = pk_scale_exp(sqrtf(pair_sum(nn)) * __uint_as_float(p.max_v[(int64_t)pt.seq * p.Hk + hk]));
+  const int64_t srow = (int64_t)head * p.Tq + t;
+  const float nlse = p.nlse[srow] * sl2 - kPScale<E> + (float)e;  // p 2^e = 2^(s - lse + e)
+  // dP - delta: delta is where the products start, in a register block of its own; fp16, whose scale takes
+  // more registers, adds it afterwards.
+  const float ndelta = p.ndelta[srow];
+  f32x16 dp0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) dp0[r] = kFp16 ? 0.f : ndelta;
+  const float unscale = ldexpf(p.scale, -e);
   auto last_key = [&](int r) { return p.causal ? min(min(r, rows - 1) / p.G + shift, lk - 1) : lk - 1; };
-  const int lim_wave = row0 + wave * QPW * 32 < rows ? last_key(row0 + (wave + 1) * QPW * 32 - 1) : -1;
+  const int lim_wave = base < rows ? last_key(base + 31) : -1;
   const int keys = last_key(row0 + BM - 1) + 1;
-  const int ntk = keys > 0 ? (keys + 63) >> 6 : 0;
+  // This part's tiles of 64 keys.
+  const int all = keys > 0 ? (keys + 63) >> 6 : 0;
+  const int per = p.split_dq > 1 ? (all + p.split_dq - 1) / p.split_dq : all;
+  const int tk0 = min((int)blockIdx.y * per, all), ntk = min(per, all - tk0);
 
-  f32x16 acc[QPW][DB];
+  f32x16 acc[DB];
 #pragma unroll
-  for (int a = 0; a < QPW; ++a)
+  for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[a][db][r] = 0.f;
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
 
   PkRows<D, 256> krows, vrows;
   krows.init(p.k + (int64_t)k0 * p.kst + (int64_t)hk * p.ksh, p.kst, lk, tid);
   vrows.init(p.v + (int64_t)k0 * p.vst + (int64_t)hk * p.vsh, p.vst, lk, tid);
 
-  auto sub = [&](const uint8_t* kt, const uint8_t* vt, int st, int j0) __attribute__((always_inline)) {
-    f32x16 s[QPW], dp[QPW];
-#pragma unroll
-    for (int a = 0; a < QPW; ++a)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[a][r] = 0.f;
-        dp[a][r] = -delta[a];
-      }
+  const PkLane<D> at(lane);
+  struct Rows {
+    uint4 k[KS], v[KS];
+  };
+  auto fetch = [&](const uint8_t* kt, const uint8_t* vt, int st, Rows& r) __attribute__((always_inline)) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const uint4 ka = pk_row_quad<D>(kt, st, ks, lane);
-      const uint4 va = pk_row_quad<D>(vt, st, ks, lane);
-#pragma unroll
-      for (int a = 0; a < QPW; ++a) s[a] = mma(E{}, ka, qa[a][ks], s[a]);
-#pragma unroll
-      for (int a = 0; a < QPW; ++a) dp[a] = mma(E{}, va, ga[a][ks], dp[a]);
+      r.k[ks] = at.row(kt, st, ks);
+      r.v[ks] = at.row(vt, st, ks);
     }
+  };
+  // Three steps: the products S and dP while the column operands of K are read; dS; the product dQ while
+  // `next` reads the next sub-tile's row operands. Kept in this order at D = 64, where that fits three
+  // waves per SIMD (6 scenes of 2 to 8 views: 544 us, 583 with two; left to the compiler 546 with two).
+  auto step = []() __attribute__((always_inline)) {
+    if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
+  };
+  auto sub = [&](auto masked, const uint8_t* kt, int st, int j0, Rows& r, auto&& next) __attribute__((always_inline)) {
     uint4 kc[DB][2];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) kc[db][ks] = pk_col_quad<D>(kt, st, ks, db, lane);
+      for (int ks = 0; ks < 2; ++ks) kc[db][ks] = at.col(kt, st, ks, db);
+    f32x16 s, dp = dp0;
 #pragma unroll
-    for (int a = 0; a < QPW; ++a) {
-      float ds[16];
+    for (int x = 0; x < 16; ++x) s[x] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = fexp2(fmaf(s[a][r], sl2, nlse[a])) * dp[a][r];
-      if (j0 + 31 > lim_lo[a]) {
-        const int room = lim[a] - j0 - 4 * half;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ds[r] = 8 * (r / 4) + r % 4 <= room ? ds[r] : 0.f;
-      }
-      const uint4 b0 = pack_quad<E>(ds), b1 = pack_quad<E>(ds + 8);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) acc[a][db] = mma(E{}, kc[db][0], b0, acc[a][db]);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) acc[a][db] = mma(E{}, kc[db][1], b1, acc[a][db]);
+    for (int ks = 0; ks < KS; ++ks) {
+      s = mma(E{}, r.k[ks], qa[ks], s);
+      dp = mma(E{}, r.v[ks], ga[ks], dp);
     }
+    step();
+    float ds[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) ds[x] = fexp2(fmaf(s[x], sl2, nlse)) * (kFp16 ? dp[x] + ndelta : dp[x]);
+    if constexpr (decltype(masked)::value) {
+      const int room = lim - j0 - 4 * half;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) ds[x] = 8 * (x / 4) + x % 4 <= room ? ds[x] : 0.f;
+    }
+    const uint4 b[2] = {pack_quad<E>(ds), pack_quad<E>(ds + 8)};
+    step();
+    next();
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = mma(E{}, kc[db][ks], b[ks], acc[db]);
+    step();
   };
 
   if (ntk > 0) {
-    krows.load(0, kt0);
-    vrows.load(0, vt0);
+    krows.load(tk0, kt0);
+    vrows.load(tk0, vt0);
     pk_tile_barrier();
-    auto tile = [&](int n, const uint8_t* kc, const uint8_t* vc, uint8_t* kn, uint8_t* vn) __attribute__((always_inline)) {
-      krows.load(min(n + 1, ntk - 1), kn);
-      vrows.load(min(n + 1, ntk - 1), vn);
-      if (64 * n <= lim_wave) {
-        sub(kc, vc, 0, 64 * n);
-        sub(kc, vc, 1, 64 * n + 32);
+    const int full = min(max(((last_key(row0) + 1) >> 6) - tk0, 0), ntk);  // tiles that every row sees whole
+    pk_tiles(ntk, full, [&](auto masked, auto buf, int n) __attribute__((always_inline)) {
+      constexpr int B = decltype(buf)::value;
+      const uint8_t *kc = B ? kt1 : kt0, *vc = B ? vt1 : vt0;
+      krows.load(tk0 + min(n + 1, ntk - 1), B ? kt0 : kt1);
+      vrows.load(tk0 + min(n + 1, ntk - 1), B ? vt0 : vt1);
+      const int j0 = 64 * (tk0 + n);
+      if (j0 <= lim_wave) {
+        Rows r0, r1;
+        fetch(kc, vc, 0, r0);
+        sub(masked, kc, 0, j0, r0, [&]() __attribute__((always_inline)) { fetch(kc, vc, 1, r1); });
+        sub(masked, kc, 1, j0 + 32, r1, []() {});
       }
       pk_tile_barrier();
-    };
-    int n = 0;
-#pragma unroll 1
-    for (; n + 1 < ntk; n += 2) {
-      tile(n, kt0, vt0, kt1, vt1);
-      tile(n + 1, kt1, vt1, kt0, vt0);
-    }
-    if (n < ntk) tile(n, kt0, vt0, kt1, vt1);
+    });
   }
+  if (p.split_dq > 1) {
+    float* dst = p.part_dq + (((int64_t)blockIdx.y * p.Tq + t) * p.H + head) * D;
 #pragma unroll
-  for (int a = 0; a < QPW; ++a) {
-    uint16_t* row = p.dq + (int64_t)(pt.start + tok[a]) * p.dqst + (int64_t)head[a] * p.dqsh;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) pk_store_col<E>(row + 32 * db, acc[a][db], unscale[a], half, on[a]);
+    for (int db = 0; db < DB; ++db) pk_store_part(dst + 32 * db, acc[db], unscale, half, on);
+    return;
   }
+  uint16_t* dst = p.dq + t * p.dqst + (int64_t)head * p.dqsh;
+#pragma unroll
+  for (int db = 0; db < DB; ++db) pk_store_col<E>(dst + 32 * db, acc[db], unscale, half, on);
 }
 
 // ---------------------------------------------------------------------------------------
-// dK and dV: 4 waves x 32 keys of one key head; tiles of 64 query tokens of each head of the group.
-// A lane holds one key and 16 queries of S = Q K^T and dP = dO V^T.
+// dK and dV: 4 waves x 32 keys of one key head; tiles of 64 query tokens of each head of the group. A
+// lane holds one key and 16 queries of S = Q K^T and dP = dO V^T, whose products start at -lse / scale
+// and -delta. (64 keys per wave, one wave per SIMD, read half as much from LDS and took 20 % longer: the
+// products and the weights of one wave do not overlap enough.)
 // ---------------------------------------------------------------------------------------
-constexpr int kBwdKeys = 128;
-
 template <typename E, int D>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedBwdParams p) {
-  constexpr int KS = D / 16, DB = D / 32;
+  constexpr int KS = D / 16, DB = D / 32, BN = 128;
   constexpr int kTileBytes = 64 * 2 * D;
   constexpr bool kFp16 = __is_same(E, FP16);
   __shared__ __align__(16) uint8_t qt0[kTileBytes], qt1[kTileBytes], gt0[kTileBytes], gt1[kTileBytes];
-  __shared__ __align__(16) float2 st0[64], st1[64];
+  __shared__ __align__(16) float nl0[64], nl1[64], nd0[64], nd1[64];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int hk = blockIdx.x % p.Hk;
-  const PackedTile pt = pk_find_tile(p.cu_k, p.n, p.Tk, 1, kBwdKeys, blockIdx.x / p.Hk);
-  const int key0 = pt.tile * kBwdKeys;
+  const PackedTile pt = pk_find_tile(p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk);
+  const int key0 = pt.tile * BN;
   if (key0 >= pt.len) return;
   int q0, lq;
   pk_other(p.cu_q, p.n, p.Tq, pt.seq, q0, lq);
   const int shift = pt.len - lq;  // causal: key j is seen by tokens i >= j - shift
   const float sl2 = p.scale_log2;
   const int wkey = key0 + wave * 32;
+
   const int key = wkey + col;
   const bool on = key < pt.len;
 
   // Stationary operands: K and V rows of this lane's key.
   uint4 kb[KS], vb[KS];
   {
-    const int64_t t = pt.start + (on ? key : pt.len - 1);
+    const int64_t t = pt.start + min(key, pt.len - 1);
     const uint16_t* kr = p.k + t * p.kst + (int64_t)hk * p.ksh + half * 8;
     const uint16_t* vr = p.v + t * p.vst + (int64_t)hk * p.vsh + half * 8;
 #pragma unroll
@@ -311,89 +342,104 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
   const int first = p.causal ? max(0, key0 - shift) >> 6 : 0;  // first tile with a query that sees a key
   const int ntq = (lq + 63) >> 6;
   const int per = ntq > first ? ntq - first : 0;
-  const int total = per * p.G;
+  // This part's tiles, head by head of the group.
+  const int64_t all = (int64_t)per * p.G;
+  const int64_t share = p.split_dkv > 1 ? (all + p.split_dkv - 1) / p.split_dkv : all;
+  const int64_t t0 = min((int64_t)blockIdx.y * share, all);
+  const int total = (int)min(share, all - t0);
 
   PkRows<D, 256> qrows, grows;
   const uint16_t* qbase = p.q + (int64_t)q0 * p.qst + (int64_t)hk * p.G * p.qsh;
   const uint16_t* gbase = p.dout + (int64_t)q0 * p.gst + (int64_t)hk * p.G * p.gsh;
-  const float2* sbase = p.stats + (int64_t)hk * p.G * p.Tq + q0;
+  const int64_t sbase = (int64_t)hk * p.G * p.Tq + q0;
   qrows.init(qbase, p.qst, lq, tid);
   grows.init(gbase, p.gst, lq, tid);
   // The tile that is loaded next: head of the group and tile of its queries.
-  int ld_h = 0, ld_t = first;
-  auto load = [&](uint8_t* qd, uint8_t* gd, float2* sd) __attribute__((always_inline)) {
+  int ld_h = per > 0 ? (int)(t0 / per) : 0;
+  int ld_t = first + (int)(t0 - (int64_t)ld_h * per);
+  auto load = [&](uint8_t* qd, uint8_t* gd, float* ld, float* dd) __attribute__((always_inline)) {
     qrows.base = uniform_ptr(reinterpret_cast<const char*>(qbase + (int64_t)ld_h * p.qsh));
     grows.base = uniform_ptr(reinterpret_cast<const char*>(gbase + (int64_t)ld_h * p.gsh));
     qrows.load(ld_t, qd);
     grows.load(ld_t, gd);
-    const char* sp = reinterpret_cast<const char*>(sbase + (int64_t)ld_h * p.Tq + ld_t * 64);
-    const __amdgpu_buffer_rsrc_t rs = pk_rsrc(sp, (int64_t)(lq - ld_t * 64) * 8);
-    // 64 {lse, delta} pairs, 4 bytes a lane (their start is only 8-byte aligned): waves 0 and 1.
-    if (wave < 2)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rs, (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(sd) + wave * 256), 4,
-          wave * 256 + lane * 4, 0, 0, 0);
+    // 64 lse and 64 delta, 4 bytes a lane (their start is only 4-byte aligned): waves 0 and 1. Zeros behind
+    // the last query, whose Q and dO are zero as well.
+    const int64_t sat = sbase + (int64_t)ld_h * p.Tq + ld_t * 64;
+    const int64_t left = (int64_t)(lq - ld_t * 64) * 4;
+    if (wave == 0)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.nlse + sat), left),
+                                               (__attribute__((address_space(3))) void*)ld, 4, lane * 4, 0, 0, 0);
+    if (wave == 1)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.ndelta + sat), left),
+                                               (__attribute__((address_space(3))) void*)dd, 4, lane * 4, 0, 0, 0);
     if (++ld_t == ntq) {
       ld_t = first;
       if (++ld_h == p.G) ld_h = p.G - 1;  // past the end: a tile again that no wave uses
     }
   };
 
-  auto sub = [&](const uint8_t* qt, const uint8_t* gt, const float2* sd, int st, int i0) __attribute__((always_inline)) {
+  const PkLane<D> at(lane);
+  // A sub-tile of 32 queries. Entry x of this lane is query i0 + 8 (x / 4) + 4 half + x % 4.
+  auto sub = [&](auto masked, const uint8_t* qt, const uint8_t* gt, const float* nl, const float* nd, int st, int i0)
+                 __attribute__((always_inline)) {
     f32x16 s, dp;
-    float nl[16];
-    // Entry r of this lane is query i0 + 8 (r / 4) + 4 half + r % 4.
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4* sp = reinterpret_cast<const float4*>(sd + 32 * st + 8 * g + 4 * half);
-      const float4 a = sp[0], b = sp[1];
-      nl[4 * g] = a.x;
-      nl[4 * g + 1] = a.z;
-      nl[4 * g + 2] = b.x;
-      nl[4 * g + 3] = b.z;
-      dp[4 * g] = -a.y;
-      dp[4 * g + 1] = -a.w;
-      dp[4 * g + 2] = -b.y;
-      dp[4 * g + 3] = -b.w;
+      const float4 x = *reinterpret_cast<const float4*>(nl + 32 * st + 8 * g + 4 * half);
+      const float4 y = *reinterpret_cast<const float4*>(nd + 32 * st + 8 * g + 4 * half);
+      s[4 * g] = x.x;
+      s[4 * g + 1] = x.y;
+      s[4 * g + 2] = x.z;
+      s[4 * g + 3] = x.w;
+      dp[4 * g] = y.x;
+      dp[4 * g + 1] = y.y;
+      dp[4 * g + 2] = y.z;
+      dp[4 * g + 3] = y.w;
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    for (int ks = 0; ks < KS; ++ks) s = mma(E{}, at.row(qt, st, ks), kb[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      s = mma(E{}, pk_row_quad<D>(qt, st, ks, lane), kb[ks], s);
-      dp = mma(E{}, pk_row_quad<D>(gt, st, ks, lane), vb[ks], dp);
-    }
+    for (int ks = 0; ks < KS; ++ks) dp = mma(E{}, at.row(gt, st, ks), vb[ks], dp);
     float w[16], ds[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) w[r] = fexp2(fmaf(s[r], sl2, (kFp16 ? 14.f : 0.f) - nl[r]));
-    if (p.causal && i0 < wkey + 31 - shift) {
+    for (int x = 0; x < 16; ++x) w[x] = fexp2(s[x] * sl2);
+    if constexpr (decltype(masked)::value) {
       const int need = key - shift - i0 - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) w[r] = 8 * (r / 4) + r % 4 >= need ? w[r] : 0.f;
+      for (int x = 0; x < 16; ++x) w[x] = 8 * (x / 4) + x % 4 >= need ? w[x] : 0.f;
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) ds[r] = kFp16 ? w[r] * dscale * dp[r] : w[r] * dp[r];
+    for (int x = 0; x < 16; ++x) ds[x] = kFp16 ? w[x] * dscale * dp[x] : w[x] * dp[x];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const uint4 pb = pack_quad<E>(w + 8 * ks), db_ = pack_quad<E>(ds + 8 * ks);
+      const uint4 pb = pack_quad<E>(w + 8 * ks), sb = pack_quad<E>(ds + 8 * ks);
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        av[db] = mma(E{}, pk_col_quad<D>(gt, st, ks, db, lane), pb, av[db]);
-        ak[db] = mma(E{}, pk_col_quad<D>(qt, st, ks, db, lane), db_, ak[db]);
+        av[db] = mma(E{}, at.col(gt, st, ks, db), pb, av[db]);
+        ak[db] = mma(E{}, at.col(qt, st, ks, db), sb, ak[db]);
       }
     }
   };
 
   if (total > 0) {
-    load(qt0, gt0, st0);
+    load(qt0, gt0, nl0, nd0);
     pk_tile_barrier();
-    int cur = first;  // the tile that is computed
-    auto tile = [&](const uint8_t* qc, const uint8_t* gc, const float2* sc, uint8_t* qn, uint8_t* gn, float2* sn)
-                    __attribute__((always_inline)) {
-      load(qn, gn, sn);
-      if (wkey < pt.len && (!p.causal || 64 * cur + 63 + shift >= wkey)) {
-        sub(qc, gc, sc, 0, 64 * cur);
-        sub(qc, gc, sc, 1, 64 * cur + 32);
+    int cur = first + (int)(t0 % per);  // the tile that is computed
+    // Queries of tiles from `full` on see every key of the workgroup's block.
+    const int full = p.causal ? (key0 + BN - 1 - shift + 63) >> 6 : first;
+    auto tile = [&](auto buf) __attribute__((always_inline)) {
+      constexpr int B = decltype(buf)::value;
+      const uint8_t *qc = B ? qt1 : qt0, *gc = B ? gt1 : gt0;
+      const float *lc = B ? nl1 : nl0, *dc = B ? nd1 : nd0;
+      load(B ? qt0 : qt1, B ? gt0 : gt1, B ? nl0 : nl1, B ? nd0 : nd1);
+      if (wkey < pt.len) {
+        if (cur >= full) {
+          sub(PkInt<0>{}, qc, gc, lc, dc, 0, 64 * cur);
+          sub(PkInt<0>{}, qc, gc, lc, dc, 1, 64 * cur + 32);
+        } else if (64 * cur + 63 + shift >= wkey) {
+          sub(PkInt<1>{}, qc, gc, lc, dc, 0, 64 * cur);
+          sub(PkInt<1>{}, qc, gc, lc, dc, 1, 64 * cur + 32);
+        }
       }
       if (++cur == ntq) cur = first;
       pk_tile_barrier();
@@ -401,15 +447,25 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
     int n = 0;
 #pragma unroll 1
     for (; n + 1 < total; n += 2) {
-      tile(qt0, gt0, st0, qt1, gt1, st1);
-      tile(qt1, gt1, st1, qt0, gt0, st0);
+      tile(PkInt<0>{});
+      tile(PkInt<1>{});
     }
-    if (n < total) tile(qt0, gt0, st0, qt1, gt1, st1);
+    if (n < total) tile(PkInt<0>{});
   }
+  const float fk = kFp16 ? ldexpf(p.scale, -e) : p.scale, fv = kFp16 ? ldexpf(1.f, -14) : 1.f;
   const int64_t t = pt.start + (on ? key : 0);
+  if (p.split_dkv > 1) {
+    const int64_t part = (int64_t)p.Tk * p.Hk * D;
+    float* dst = p.part_dkv + 2 * blockIdx.y * part + (t * p.Hk + hk) * D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      pk_store_part(dst + 32 * db, ak[db], fk, half, on);
+      pk_store_part(dst + part + 32 * db, av[db], fv, half, on);
+    }
+    return;
+  }
   uint16_t* dkr = p.dk + t * p.dkst + (int64_t)hk * p.dksh;
   uint16_t* dvr = p.dv + t * p.dvst + (int64_t)hk * p.dvsh;
-  const float fk = kFp16 ? ldexpf(p.scale, -e) : p.scale, fv = kFp16 ? ldexpf(1.f, -14) : 1.f;
 #pragma unroll
   for (int db = 0; db < DB; ++db) {
     pk_store_col<E>(dkr + 32 * db, ak[db], fk, half, on);
@@ -417,10 +473,58 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
   }
 }
 
-template <typename E, int D, int QPW>
+// Sums the parts of a gradient [T, H, D], in order: part i at src + i * step.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void packed_bwd_join_kernel(const float* __restrict__ src, int64_t step, int parts,
+                                                              int64_t rows, int H, uint16_t* __restrict__ dst,
+                                                              int64_t st, int64_t sh) {
+  constexpr int LPR = D / 4;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int c = threadIdx.x % LPR;
+  if (row >= rows) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float4 x = reinterpret_cast<const float4*>(src + i * step + row * D)[c];
+    s.x += x.x;
+    s.y += x.y;
+    s.z += x.z;
+    s.w += x.w;
+  }
+  const int64_t t = row / H;
+  *reinterpret_cast<uint2*>(dst + t * st + (row - t * H) * sh + 4 * c) =
+      make_uint2(pack_pair(E{}, s.x, s.y), pack_pair(E{}, s.z, s.w));
+}
+
+// Parts that the keys of the dQ pass and the queries of the dK/dV pass are cut into, where the tiles
+// alone leave workgroup slots empty (two per CU), from the sizes that the host knows; a part has at
+// least 512 keys or queries on average. The parts' fp32 sums are joined in order by another launch.
+struct BwdPlan {
+  int dq, dkv;
+  size_t dq_bytes, dkv_bytes;
+};
+
+BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
+  const int64_t G = Hq / Hk, seqs = n > 0 ? n : 1;
+  auto parts = [&](int64_t rows, int64_t other) {
+    // Tiles: at least one per sequence that has rows, and the last one of a sequence half full.
+    const int64_t wgs = (rows / 128 + (rows < 128 * n ? n : n / 2) + 1) * Hk;
+    int64_t s = 512 / (wgs > 0 ? wgs : 1);
+    if (s > other / seqs / 512) s = other / seqs / 512;
+    return (int)(s > 16 ? 16 : s > 1 ? s : 1);
+  };
+  BwdPlan b = {};
+  b.dq = parts(Tq * G, Tk);
+  b.dkv = parts(Tk, Tq * G);
+  b.dq_bytes = b.dq > 1 ? (size_t)b.dq * Tq * Hq * D * sizeof(float) : 0;
+  b.dkv_bytes = b.dkv > 1 ? (size_t)b.dkv * 2 * Tk * Hk * D * sizeof(float) : 0;
+  return b;
+}
+
+template <typename E, int D>
 int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
   constexpr bool kFp16 = __is_same(E, FP16);
-  const int64_t qslots = (int64_t)p.Tq * p.G / (128 * QPW) + p.n + 2, kslots = (int64_t)p.Tk / kBwdKeys + p.n + 2;
+  const int64_t qslots = (int64_t)p.Tq * p.G / 128 + p.n + 2, kslots = (int64_t)p.Tk / 128 + p.n + 2;
   GW_CHECK_ARG(qslots * p.Hk < (1ll << 31) && kslots * p.Hk < (1ll << 31), "the grid is too large");
   if (kFp16) {
     const int64_t words = 2 * (int64_t)(p.n + 2) * p.Hk;  // max_do and max_v, one behind the other
@@ -436,19 +540,35 @@ int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D, kFp16>), dim3((uint32_t)(p.Tq / kStatTokens + p.n + 2)), dim3(256), 0,
                        stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (rows)");
-    hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D, QPW>), dim3((uint32_t)(qslots * p.Hk)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)(qslots * p.Hk), p.split_dq), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq)");
+    if (p.split_dq > 1) {
+      const int64_t rows = (int64_t)p.Tq * p.H;
+      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D>), dim3((uint32_t)((rows * (D / 4) + 255) / 256)), dim3(256), 0, stream,
+                         p.part_dq, rows * D, p.split_dq, rows, p.H, p.dq, p.dqst, p.dqsh);
+      GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq join)");
+    }
   }
   if (p.Tk > 0) {
-    hipLaunchKernelGGL((packed_bwd_dkv_kernel<E, D>), dim3((uint32_t)(kslots * p.Hk)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((packed_bwd_dkv_kernel<E, D>), dim3((uint32_t)(kslots * p.Hk), p.split_dkv), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk, dv)");
+    if (p.split_dkv > 1) {
+      const int64_t rows = (int64_t)p.Tk * p.Hk;
+      const dim3 grid((uint32_t)((rows * (D / 4) + 255) / 256));
+      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D>), grid, dim3(256), 0, stream, p.part_dkv, 2 * rows * D, p.split_dkv,
+                         rows, p.Hk, p.dk, p.dkst, p.dksh);
+      GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk join)");
+      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D>), grid, dim3(256), 0, stream, p.part_dkv + rows * D, 2 * rows * D,
+                         p.split_dkv, rows, p.Hk, p.dv, p.dvst, p.dvsh);
+      GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dv join)");
+    }
   }
   return GW_OK;
 }
 
 template <typename E>
 int packed_bwd_dim(const PackedBwdParams& p, int64_t D, hipStream_t stream) {
-  return D == 64 ? packed_bwd_launch<E, 64, 2>(p, stream) : packed_bwd_launch<E, 128, 1>(p, stream);
+  return D == 64 ? packed_bwd_launch<E, 64>(p, stream) : packed_bwd_launch<E, 128>(p, stream);
 }
 
 inline size_t pk_align(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -457,10 +577,10 @@ inline size_t pk_align(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace gw
 
 extern "C" size_t gw_packed_attn_bwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
-  (void)Tk;
-  (void)D;
-  if (n < 0 || Tq < 0 || Hq < 1 || Hk < 1) return 0;
-  return gw::pk_align((size_t)Tq * Hq * 8) + gw::pk_align((size_t)(n + 2) * Hk * 8);
+  if (n < 0 || Tq < 0 || Tk < 0 || Hk < 1 || Hq < Hk || D < 1) return 0;
+  const gw::BwdPlan b = gw::packed_bwd_plan(n, Tq, Tk, Hq, Hk, D);
+  return gw::pk_align((size_t)Tq * Hq * 8) + gw::pk_align((size_t)(n + 2) * Hk * 8) + gw::pk_align(b.dq_bytes) +
+         gw::pk_align(b.dkv_bytes);
 }
 
 extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
@@ -498,9 +618,15 @@ extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_str
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
   char* ws = static_cast<char*>(workspace);
-  p.stats = reinterpret_cast<float2*>(ws);
+  p.nlse = reinterpret_cast<float*>(ws);
+  p.ndelta = p.nlse + Tq * Hq;
   p.max_do = reinterpret_cast<uint32_t*>(ws + pk_align((size_t)Tq * Hq * 8));
   p.max_v = p.max_do + (n + 2) * Hk;
+  const BwdPlan b = packed_bwd_plan(n, Tq, Tk, Hq, Hk, D);
+  p.split_dq = b.dq;
+  p.split_dkv = b.dkv;
+  p.part_dq = reinterpret_cast<float*>(ws + pk_align((size_t)Tq * Hq * 8) + pk_align((size_t)(n + 2) * Hk * 8));
+  p.part_dkv = p.part_dq + pk_align(b.dq_bytes) / sizeof(float);
   p.cu_q = cu_q;
   p.cu_k = cu_k;
   p.n = (int)n;

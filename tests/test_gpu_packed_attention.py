@@ -25,6 +25,7 @@ LENS = {
     "few rows": ([3, 1, 40, 0, 2, 17], [2000, 777, 1500, 600, 33, 1300]),
     "few rows only": ([2], [2700]),
     "keys split": ([140, 150], [5000, 1201]),
+    "queries split": ([2500, 1700, 0], [40, 90, 3]),
 }
 
 
