@@ -238,6 +238,51 @@ __device__ __forceinline__ void pk_tiles(int ntk, int nfull, F&& tile) {
   if (n < ntk) tile(PkInt<1>{}, PkInt<0>{}, n);
 }
 
+// inf and NaN in places that a row does not see. A masked weight is 0, but 0 * inf is NaN: in tiles
+// that some rows see only in part, inf and NaN among the second operand's entries are cleared before the
+// product, and once it is known that there were any (never, in healthy data), a pass over those tiles
+// adds them to the rows that do see them.
+template <typename E>
+constexpr uint32_t kPkExp = __is_same(E, FP16) ? 0x7C00u : 0x7F80u;
+
+template <typename E>
+__device__ __forceinline__ bool pk_not_finite(uint32_t half) { return (half & kPkExp<E>) == kPkExp<E>; }
+
+template <typename E>
+__device__ __forceinline__ uint32_t pk_finite_word(uint32_t w) {
+  return (pk_not_finite<E>(w) ? 0u : w & 0xFFFFu) | (pk_not_finite<E>(w >> 16) ? 0u : w & 0xFFFF0000u);
+}
+// Clears the entries that are not finite; whether there were any in the wave.
+template <typename E, int N>
+__device__ __forceinline__ bool pk_clear_not_finite(uint4 (&q)[N]) {
+  uint32_t any = 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    any |= nonfinite2(q[i].x, kPkExp<E>) | nonfinite2(q[i].y, kPkExp<E>) | nonfinite2(q[i].z, kPkExp<E>) |
+           nonfinite2(q[i].w, kPkExp<E>);
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(any != 0u) == 0ull, 1)) return false;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    q[i] = make_uint4(pk_finite_word<E>(q[i].x), pk_finite_word<E>(q[i].y), pk_finite_word<E>(q[i].z),
+                      pk_finite_word<E>(q[i].w));
+  return true;
+}
+// Adds the entries of a memory row that are not finite to a lane's accumulator entries (dims 32 db + 8 g + 4 half
+// + 0..3), where `seen`.
+template <typename E, int DB>
+__device__ __forceinline__ void pk_add_not_finite(const uint16_t* row, int half, bool seen, f32x16 (&acc)[DB]) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint2 w = *reinterpret_cast<const uint2*>(row + 32 * db + 8 * g + 4 * half);
+      const uint32_t h[4] = {w.x & 0xFFFFu, w.x >> 16, w.y & 0xFFFFu, w.y >> 16};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (seen && pk_not_finite<E>(h[i])) acc[db][4 * g + i] += in_to_float(__is_same(E, FP16), h[i]);
+    }
+}
+
 // Stores a lane's column of a transposed accumulator (32 dims of one row) scaled by f: lanes l and
 // l ^ 32 exchange quads so that each stores eight consecutive dims.
 template <typename E>

@@ -177,12 +177,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   if (kFp16) e = pk_scale_exp(sqrtf(pair_sum(nn)) * __uint_as_float(p.max_v[(int64_t)pt.seq * p.Hk + hk]));
   const int64_t srow = (int64_t)head * p.Tq + t;
   const float nlse = p.nlse[srow] * sl2 - kPScale<E> + (float)e;  // p 2^e = 2^(s - lse + e)
-  // dP - delta: delta is where the products start, in a register block of its own; fp16, whose scale takes
-  // more registers, adds it afterwards.
+  // dP - delta: delta is where the products start, in a register block of its own; fp16 at D = 64, whose
+  // scale takes the registers, adds it afterwards.
+  constexpr bool kAddDelta = kFp16 && D == 64;
   const float ndelta = p.ndelta[srow];
   f32x16 dp0;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) dp0[r] = kFp16 ? 0.f : ndelta;
+  for (int r = 0; r < 16; ++r) dp0[r] = kAddDelta ? 0.f : ndelta;
   const float unscale = ldexpf(p.scale, -e);
   auto last_key = [&](int r) { return p.causal ? min(min(r, rows - 1) / p.G + shift, lk - 1) : lk - 1; };
   const int lim_wave = base < rows ? last_key(base + 31) : -1;
@@ -220,11 +221,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
     if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
   };
   auto sub = [&](auto masked, const uint8_t* kt, int st, int j0, Rows& r, auto&& next) __attribute__((always_inline)) {
-    uint4 kc[DB][2];
+    uint4 kc[2 * DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) kc[db][ks] = at.col(kt, st, ks, db);
+      for (int ks = 0; ks < 2; ++ks) kc[2 * db + ks] = at.col(kt, st, ks, db);
     f32x16 s, dp = dp0;
 #pragma unroll
     for (int x = 0; x < 16; ++x) s[x] = 0.f;
@@ -236,11 +237,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
     step();
     float ds[16];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) ds[x] = fexp2(fmaf(s[x], sl2, nlse)) * (kFp16 ? dp[x] + ndelta : dp[x]);
+    for (int x = 0; x < 16; ++x) ds[x] = fexp2(fmaf(s[x], sl2, nlse)) * (kAddDelta ? dp[x] + ndelta : dp[x]);
     if constexpr (decltype(masked)::value) {
       const int room = lim - j0 - 4 * half;
 #pragma unroll
       for (int x = 0; x < 16; ++x) ds[x] = 8 * (x / 4) + x % 4 <= room ? ds[x] : 0.f;
+      // Rows that see such a key have a NaN score and so a NaN dS.
+      if (p.causal) pk_clear_not_finite<E>(kc);
     }
     const uint4 b[2] = {pack_quad<E>(ds), pack_quad<E>(ds + 8)};
     step();
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] = mma(E{}, kc[db][ks], b[ks], acc[db]);
+      for (int db = 0; db < DB; ++db) acc[db] = mma(E{}, kc[2 * db + ks], b[ks], acc[db]);
     step();
   };
 
@@ -379,6 +382,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
   };
 
   const PkLane<D> at(lane);
+  bool unclean = false;  // dO holds inf or NaN in tiles that see some keys only in part
   // A sub-tile of 32 queries. Entry x of this lane is query i0 + 8 (x / 4) + 4 half + x % 4.
   auto sub = [&](auto masked, const uint8_t* qt, const uint8_t* gt, const float* nl, const float* nd, int st, int i0)
                  __attribute__((always_inline)) {
@@ -403,20 +407,34 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
     float w[16], ds[16];
 #pragma unroll
     for (int x = 0; x < 16; ++x) w[x] = fexp2(s[x] * sl2);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) ds[x] = kFp16 ? w[x] * dscale * dp[x] : w[x] * dp[x];
     if constexpr (decltype(masked)::value) {
       const int need = key - shift - i0 - 4 * half;
 #pragma unroll
-      for (int x = 0; x < 16; ++x) w[x] = 8 * (x / 4) + x % 4 >= need ? w[x] : 0.f;
+      for (int x = 0; x < 16; ++x) {
+        const bool sees = 8 * (x / 4) + x % 4 >= need;
+        w[x] = sees ? w[x] : 0.f;
+        ds[x] = sees ? ds[x] : 0.f;
+      }
     }
-#pragma unroll
-    for (int x = 0; x < 16; ++x) ds[x] = kFp16 ? w[x] * dscale * dp[x] : w[x] * dp[x];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const uint4 pb = pack_quad<E>(w + 8 * ks), sb = pack_quad<E>(ds + 8 * ks);
+      uint4 gc[DB], qc[DB];
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        av[db] = mma(E{}, at.col(gt, st, ks, db), pb, av[db]);
-        ak[db] = mma(E{}, at.col(qt, st, ks, db), sb, ak[db]);
+        gc[db] = at.col(gt, st, ks, db);
+        qc[db] = at.col(qt, st, ks, db);
+      }
+      if constexpr (decltype(masked)::value) {
+        unclean |= pk_clear_not_finite<E>(gc);
+        pk_clear_not_finite<E>(qc);  // keys that such a query sees have a NaN dS
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        av[db] = mma(E{}, gc[db], pb, av[db]);
+        ak[db] = mma(E{}, qc[db], sb, ak[db]);
       }
     }
   };
@@ -451,6 +469,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
       tile(PkInt<1>{});
     }
     if (n < total) tile(PkInt<0>{});
+    if (__builtin_expect(unclean, 0)) {
+      for (int64_t x = t0; x < t0 + total; ++x) {
+        const int h = (int)(x / per), i0 = 64 * (first + (int)(x % per));
+        for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i)
+          pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, av);
+      }
+    }
   }
   const float fk = kFp16 ? ldexpf(p.scale, -e) : p.scale, fv = kFp16 ? ldexpf(1.f, -14) : 1.f;
   const int64_t t = pt.start + (on ? key : 0);

@@ -132,12 +132,16 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
       }
     }
   };
-  auto sub_pv = [&](const uint8_t* vt, int st, f32x16 (&s)[QPW]) __attribute__((always_inline)) {
-    uint4 va[DB][2];
+  bool unclean = false;  // V holds inf or NaN in tiles that some rows see only in part
+  auto sub_pv = [&](auto masked, const uint8_t* vt, int st, f32x16 (&s)[QPW]) __attribute__((always_inline)) {
+    uint4 va[2 * DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) va[db][ks] = at.col(vt, st, ks, db);
+      for (int ks = 0; ks < 2; ++ks) va[2 * db + ks] = at.col(vt, st, ks, db);
+    if constexpr (decltype(masked)::value) {
+      if (p.causal) unclean |= pk_clear_not_finite<E>(va);
+    }
 #pragma unroll
     for (int a = 0; a < QPW; ++a) {
       uint4 pb[2];
@@ -176,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) acc[a][db] = mma(E{}, va[db][ks], pb[ks], acc[a][db]);
+        for (int db = 0; db < DB; ++db) acc[a][db] = mma(E{}, va[2 * db + ks], pb[ks], acc[a][db]);
     }
   };
 
@@ -196,11 +200,19 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
         f32x16 s0[QPW], s1[QPW];
         sub_qk(masked, kc, 0, j0, s0);
         sub_qk(masked, kc, 1, j0 + 32, s1);
-        sub_pv(vc, 0, s0);
-        sub_pv(vc, 1, s1);
+        sub_pv(masked, vc, 0, s0);
+        sub_pv(masked, vc, 1, s1);
       }
       pk_tile_barrier();
     });
+    if (__builtin_expect(unclean, 0)) {
+      const int end = min(64 * (tk0 + ntk), min(lk, lim_wave + 1));
+      for (int j = 64 * (tk0 + (full & ~1)); j < end; ++j) {  // pk_tiles masks from an even tile on
+        const uint16_t* vr = p.v + (int64_t)(k0 + j) * p.vst + (int64_t)hk * p.vsh;
+#pragma unroll
+        for (int a = 0; a < QPW; ++a) pk_add_not_finite<E>(vr, half, j <= lim[a], acc[a]);
+      }
+    }
   }
 
   // o = O / l, lse = (m + log2 l) ln 2; a part keeps its o in fp32 and its log2 sum.

@@ -22,7 +22,7 @@
 // in such a page) are masked, and their V registers are cleared: what lies there cannot reach a result.
 #include <math.h>
 
-#include "gw_mma.h"
+#include "gw_packed.h"
 #include "gw_rows.h"
 
 namespace gw {
@@ -277,6 +277,7 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
       b.v[j].load(vbase + (PAGED ? page * p.vsp : 0) + at * p.vst + DV * i16);
     }
   };
+  bool unclean = false;
   auto compute = [&](int j0, uint32_t ok, Block& b) __attribute__((always_inline)) {
     f32x4 s[2];
 #pragma unroll
@@ -298,6 +299,20 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
 #pragma unroll
           for (int u = 0; u < DV / 2; ++u) b.v[j].w[u] = 0u;
         }
+      if (j0 + 31 > lim_lo) {  // some rows see some of these keys only: see pk_clear_not_finite
+        uint32_t any = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int u = 0; u < DV / 2; ++u) any |= nonfinite2(b.v[j].w[u], kPkExp<E>);
+        if (__builtin_amdgcn_ballot_w64(any != 0u) != 0ull) {
+          unclean = true;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int u = 0; u < DV / 2; ++u) b.v[j].w[u] = pk_finite_word<E>(b.v[j].w[u]);
+        }
+      }
     }
     float w[8];
     auto weights = [&](float nm) __attribute__((always_inline)) {
@@ -352,6 +367,30 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
       w1 = w0;
       w0 = w2;
       j += 256;
+    }
+  }
+
+  if (__builtin_expect(unclean, 0)) {
+    // This wave's blocks behind the first row's last key: their V entries that are not finite go to the rows
+    // that see them.
+    for (int j0 = j_first; j0 < ke; j0 += 128) {
+      if (j0 + 31 <= lim_lo) continue;
+      const Where w = where(j0);
+      for (int i = 0; i < 32; ++i) {
+        if (!((w.ok >> i) & 1u)) continue;
+        const int64_t page = __shfl(w.page, i), at = __shfl(w.at, i);
+        const uint16_t* row = vbase + (PAGED ? page * p.vsp : 0) + at * p.vst + 4 * DV * g;
+        for (int x = 0; x < 4 * DV; ++x) {
+          const uint32_t h = row[x];
+          if (!pk_not_finite<E>(h) || j0 + i > lim) continue;
+          const float f = in_to_float(__is_same(E, FP16), h);
+#pragma unroll
+          for (int u = 0; u < DV; ++u)
+#pragma unroll
+            for (int rr = 0; rr < 4; ++rr)
+              if (rr * DV + u == x) acc[u][rr] += f;
+        }
+      }
     }
   }
 

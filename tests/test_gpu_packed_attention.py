@@ -61,6 +61,11 @@ def check(got, ref, name, dtype, d, times=1):
     assert worst <= 1.0, f"{name}: {float(worst):.2f} of the bound, largest error {float(err.max()):.3g}"
 
 
+def part(ref, name, rows):
+    """The oracle's ``name`` of some rows."""
+    return {"s_mag": ref["s_mag"], name: ref[name][rows], name + "_mag": ref[name + "_mag"][rows]}
+
+
 def check_lse(lse, ref):
     a, b = lse.double().cpu(), ref["lse"]
     assert torch.equal(a == -math.inf, b == -math.inf)
@@ -136,10 +141,10 @@ def test_tokens_behind_the_last_bound_and_between(gpu_device, causal):
     o, dq, dk, dv = step(args, gpu_device, causal)
     for name, got, times in (("o", o, 1), ("dq", dq, 3)):
         assert (got[103:] == 0).all()
-        check(got[:103], {n: t[:103] for n, t in ref.items()}, name, torch.bfloat16, 64, times)
+        check(got[:103], part(ref, name, slice(103)), name, torch.bfloat16, 64, times)
     for name, got, times in (("dk", dk, 3), ("dv", dv, 1)):
         assert (got[105:] == 0).all()
-        check(got[:105], {n: t[:105] for n, t in ref.items()}, name, torch.bfloat16, 64, times)
+        check(got[:105], part(ref, name, slice(105)), name, torch.bfloat16, 64, times)
 
 
 def test_a_sequence_with_nan_leaves_the_others_alone(gpu_device):
@@ -151,6 +156,47 @@ def test_a_sequence_with_nan_leaves_the_others_alone(gpu_device):
     for a, b in zip(clean, out):
         assert torch.equal(a[:65], b[:65]) and torch.equal(a[105:], b[105:])
         assert b[65:105].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hq,hk", [(64, 2, 2), (128, 4, 2)])
+@pytest.mark.parametrize("lens_q,lens_k", [([300, 77], None), ([9, 3], [1500, 800]), ([200], [3300])])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_what_a_causal_row_does_not_see(gpu_device, dtype, d, hq, hk, lens_q, lens_k, value):
+    """inf and NaN in later values change no bit of the rows before them, and reach those behind; in a
+    query's q and dO they change no bit of the gradients of the keys that it does not see."""
+    args = make(lens_q, lens_k, hq, hk, d, dtype, 11)
+    ref = packed_attention(*args[:3], args[4], args[5], True, do=args[3])
+    clean = step(args, gpu_device, True)
+    n_q, n_k = lens_q[0], (lens_k or lens_q)[0]
+    shift = n_k - n_q
+    for cut in (1, n_q // 2, n_q - 1):  # the first query that sees what is planted
+        q, k, v, do, cu_q, cu_k = (t.clone() if torch.is_tensor(t) else t for t in args)
+        v[cut + shift, 0, 5] = value
+        out = step((q, k, v, do, cu_q, cu_k), gpu_device, True)
+        for a, b in zip(clean[:2], out[:2]):
+            assert torch.equal(a[:cut], b[:cut]) and torch.equal(a[n_q:], b[n_q:])
+        assert not torch.isfinite(out[0][cut:n_q, 0, 5]).any()
+        if value == value:
+            assert (out[0][cut:n_q, 0, 5] == value).all()
+        # A key: the rows of a block raise their running reference together, so rows beside one that sees
+        # the key are rounded otherwise, within the bounds.
+        k[cut + shift] = value
+        out = step((q, k, v, do, cu_q, cu_k), gpu_device, True)
+        for name, got, times in (("o", out[0], 1), ("dq", out[1], 3)):
+            check(got[:cut], part(ref, name, slice(cut)), name, dtype, d, times)
+            check(got[n_q:], part(ref, name, slice(n_q, None)), name, dtype, d, times)
+        q, k, v, do, cu_q, cu_k = (t.clone() if torch.is_tensor(t) else t for t in args)
+        do[cut - 1, :, 3] = value
+        out = step((q, k, v, do, cu_q, cu_k), gpu_device, True)
+        for a, b in zip(clean, out):
+            if a.shape[0] == cu_k[-1] and a.shape[1] == hk:
+                assert torch.equal(a[cut + shift:], b[cut + shift:])
+        assert not torch.isfinite(out[3][:cut + shift, :, 3]).any()
+        q[cut - 1] = value
+        out = step((q, k, v, do, cu_q, cu_k), gpu_device, True)
+        for name, got, times in (("dk", out[2], 3), ("dv", out[3], 1)):
+            check(got[cut + shift:], part(ref, name, slice(cut + shift, None)), name, dtype, d, times)
 
 
 def test_strides_layouts_and_broadcast_heads(gpu_device):

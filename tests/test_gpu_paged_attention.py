@@ -102,6 +102,26 @@ def test_unused_slots_and_pages_outside_the_pool(gpu_device):
     assert (o[3] == 0).all() and (lse[3] == -math.inf).all()
 
 
+@pytest.mark.parametrize("d,hk", [(64, 2), (128, 1)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("n", [40, 1003])
+def test_what_a_new_token_does_not_see(gpu_device, d, hk, value, n):
+    """inf and NaN in the newest tokens' keys and values reach the tokens that see them and no other."""
+    q, k, v, table, lens = make([n, 20], 6, 4, hk, d, 16, torch.float16, 8)
+    clean, lse = run((q, k, v, table, lens), gpu_device)
+    j = n - 3  # seen by new tokens 3, 4 and 5
+    page, slot = int(table[0, j // 16]), j % 16
+    v[page, slot, :, 7] = value
+    o, lse2 = run((q, k, v, table, lens), gpu_device)
+    assert torch.equal(clean[0, :3], o[0, :3]) and torch.equal(clean[1], o[1]) and torch.equal(lse, lse2)
+    assert torch.equal(clean[0, :, :, :7], o[0, :, :, :7]) and torch.equal(clean[0, :, :, 8:], o[0, :, :, 8:])
+    got = o[0, 3:, :, 7]
+    assert (got == value).all() if value == value else got.isnan().all()
+    k[page, slot] = value
+    o, lse2 = run((q, k, v, table, lens), gpu_device)
+    assert torch.equal(clean[0, :3], o[0, :3]) and torch.equal(lse[0, :3], lse2[0, :3])
+
+
 def test_lengths_outside_the_table(gpu_device):
     args = list(make([60, 60, 60], 2, 2, 2, 64, 20, torch.float16, 4, width=0))
     args[4] = torch.tensor([-3, 61, 2 ** 31 - 1], dtype=torch.int32)
