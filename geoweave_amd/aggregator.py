@@ -34,6 +34,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import dsa_layer, source_downsample
+from .custom_flash_attn.packed_flash_attn import packed_flash_attn_func, packed_flash_attn_inference_func
+from .rotary import rotary_axes_qk_func
 
 __all__ = ["parse_indexer_layers", "parse_reuse_topk_groups", "slice_expand_and_flatten", "Aggregator",
            "AggregatorGraph"]
@@ -144,7 +146,11 @@ class Mlp(nn.Module):
 
 class DenseAttention(nn.Module):
     """Reference ``layers/attention.py:38-98`` (fused path): qkv, q/k LayerNorm, 2D RoPE,
-    scaled-dot-product attention, proj. q/k LayerNorm + RoPE run in the HIP glue kernel."""
+    scaled-dot-product attention, proj. q/k LayerNorm + RoPE run in the HIP glue kernel.
+
+    With ``cu_seqlens`` (int32 ``[n + 1]`` on the GPU) x is a packed batch ``[1, T, dim]`` of n sequences
+    of different lengths and each attends within itself (``packed_flash_attn``). ``forward_train`` is the
+    differentiable form on a packed batch, with any number of rotary axes."""
 
     def __init__(self, dim: int, num_heads: int, qk_norm: bool, rope_base: Optional[float]):
         super().__init__()
@@ -157,8 +163,10 @@ class DenseAttention(nn.Module):
         self.rope_base = rope_base
         self.layout = dsa_layer.GlueLayout(num_heads, self.head_dim, 0, 64)
 
-    def forward(self, x, pos=None, rope_len=None):
+    def forward(self, x, pos=None, rope_len=None, cu_seqlens=None):
         B, N, C = x.shape
+        if cu_seqlens is not None and B != 1:
+            raise ValueError(f"a packed batch is [1, T, dim], got {tuple(x.shape)}")
         y = self.qkv(x)
         use_glue = not (isinstance(self.q_norm, nn.Identity) and (self.rope_base is None or pos is None))
         if use_glue:
@@ -167,8 +175,29 @@ class DenseAttention(nn.Module):
                 (None, None), 1e-5, pos if self.rope_base else None, self.rope_base or 100.0, rope_len)
         else:
             q, k, v = y.view(B, N, 3, self.num_heads, self.head_dim).unbind(2)
+        if cu_seqlens is not None:
+            o, _ = packed_flash_attn_inference_func(q[0], k[0], v[0], cu_seqlens)
+            return self.proj(o.view(1, N, C))
         o = _sdpa(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
         return self.proj(o.transpose(1, 2).reshape(B, N, C))
+
+    def forward_train(self, x, pos=None, cu_seqlens=None, axis_dims=None, bases=None, causal=False):
+        """x ``[T, dim]`` (packed tokens), pos ``[T, A]`` positions, cu_seqlens int32 ``[n + 1]`` (None: one
+        sequence) -> ``[T, dim]``, differentiable in x and every parameter. ``axis_dims``: dims of each
+        position axis's block of a head (default: equal shares, the two halves of the reference's
+        ``rope.py:62-188`` for (row, column)), ``bases``: their bases (default: the layer's)."""
+        T, C = x.shape
+        q, k, v = self.qkv(x).view(T, 3, self.num_heads, self.head_dim).unbind(1)
+        # one rounding to the activations' type behind the norm
+        q, k = self.q_norm(q).to(x.dtype), self.k_norm(k).to(x.dtype)
+        if pos is not None and (self.rope_base is not None or bases is not None):
+            axes = pos.shape[-1]
+            dims = axis_dims if axis_dims is not None else [self.head_dim // axes // 2 * 2] * axes
+            q, k = rotary_axes_qk_func(q, k, pos, dims, self.rope_base if bases is None else bases)
+        if cu_seqlens is None:
+            cu_seqlens = torch.tensor([0, T], dtype=torch.int32, device=x.device)
+        o = packed_flash_attn_func(q, k, v, cu_seqlens, causal=causal)
+        return self.proj(o.view(T, C))
 
 
 class Block(nn.Module):
@@ -192,8 +221,10 @@ class Block(nn.Module):
 
     timing = None  # a list to collect (start, end) HIP events around the attention call
 
-    def forward(self, x, pos=None, rope_len=None, topk_indices=None, source_downsample=None):
+    def forward(self, x, pos=None, rope_len=None, topk_indices=None, source_downsample=None, cu_seqlens=None):
         idx = None
+        if self.sparse and cu_seqlens is not None:
+            raise NotImplementedError("the sparse global attention takes one scene at a time")
         h = self.norm1(x)
         ev = None
         if self.timing is not None:
@@ -203,7 +234,7 @@ class Block(nn.Module):
             a, idx = self.attn(h, pos, return_topk=True, topk_indices=topk_indices, rope_len=rope_len,
                                source_downsample=source_downsample)
         else:
-            a = self.attn(h, pos, rope_len)
+            a = self.attn(h, pos, rope_len, cu_seqlens)
         if ev is not None:
             ev[1].record()
             self.timing.append(ev)
@@ -332,6 +363,62 @@ class Aggregator(nn.Module):
             if blk.sparse and i in sources:
                 cached[i] = idx
             outputs.append(torch.cat([frame_out, tokens.reshape(B, S, P, C)], dim=-1))
+        return outputs, self.patch_start_idx
+
+
+    @torch.no_grad()
+    def forward_scenes(self, images: torch.Tensor, views: Sequence[int]) -> Tuple[List[torch.Tensor], int]:
+        """Scenes of different numbers of views in one pass: images ``[V, 3, 518, 518]``, scene after
+        scene, ``views`` the number of views of each (their sum V) -> (list of depth tensors
+        ``[V, P, 2*dim]``, patch_start_idx). Patch embedding, frame blocks, MLPs and the dense global
+        layers run on all scenes together, the latter's attention packed (``cu_seqlens``), with no padding;
+        the sparse global layers select and attend scene by scene. Each scene's rows are those of
+        :meth:`forward` on it, up to the rounding of the dense attention kernels."""
+        views = [int(n) for n in views]
+        V, C_in, H, W = images.shape
+        if C_in != 3:
+            raise ValueError(f"expected 3 input channels, got {C_in}")
+        if sum(views) != V or any(n < 1 for n in views):
+            raise ValueError(f"scenes of {views} views do not make up {V} images")
+        dtype = self.frame_blocks[0].norm1.weight.dtype
+        x = ((images - self._resnet_mean[0]) / self._resnet_std[0]).to(dtype)
+        patch_tokens = self.patch_embed(x)
+        sp = self.special_tokens
+        tokens = torch.cat([torch.cat([slice_expand_and_flatten(t, 1, n) for n in views])
+                            for t in (sp.camera_token, sp.register_token)] + [patch_tokens], dim=1)
+        P, C = tokens.shape[1], tokens.shape[2]
+        grid = H // self.patch_size
+        pos = self.positions(1, V, grid, images.device)
+        rope_len = grid + 1
+        bounds = [0]
+        for n in views:
+            bounds.append(bounds[-1] + n * P)
+        cu = torch.tensor(bounds, dtype=torch.int32, device=images.device)
+        scenes = list(zip(bounds[:-1], bounds[1:]))
+        pos_global = pos.reshape(1, V * P, 2)
+        sd = [None] * len(views)
+        if self.source_downsample_factor > 1:
+            sd = [source_downsample.SourceDownsample(tokens_per_view=P, num_views=n,
+                                                     patch_start_idx=self.patch_start_idx,
+                                                     factor=self.source_downsample_factor, grid_h=grid, grid_w=grid,
+                                                     **self.source_downsample_options) for n in views]
+        cached: Dict[int, List[torch.Tensor]] = {}
+        sources = set(self.reuse_topk_source_by_layer.values())
+        outputs = []
+        for i in range(self.depth):
+            frame_out, _ = self.frame_blocks[i](tokens.reshape(V, P, C), pos, rope_len)
+            tokens = frame_out.reshape(1, V * P, C)
+            blk = self.global_blocks[i]
+            if blk.sparse:
+                reuse = cached.get(self.reuse_topk_source_by_layer.get(i, -1), [None] * len(views))
+                done = [blk(tokens[:, a:b], pos_global[:, a:b], rope_len, topk_indices=r, source_downsample=s)
+                        for (a, b), r, s in zip(scenes, reuse, sd)]
+                tokens = torch.cat([t for t, _ in done], 1)
+                if i in sources:
+                    cached[i] = [idx for _, idx in done]
+            else:
+                tokens, _ = blk(tokens, pos_global, rope_len, cu_seqlens=cu)
+            outputs.append(torch.cat([frame_out, tokens.reshape(V, P, C)], dim=-1))
         return outputs, self.patch_start_idx
 
 

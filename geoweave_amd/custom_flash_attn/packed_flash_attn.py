@@ -77,9 +77,10 @@ def _check_inputs(q, k, v, cu_q, cu_k, softmax_scale):
         raise ValueError(f"cu_seqlens of {cu_q.numel() - 1} and {cu_k.numel() - 1} sequences")
     if max(q.shape[0], k.shape[0]) * q.shape[1] > MAX_TOKEN_HEADS:
         raise ValueError(f"tokens x query heads must not exceed {MAX_TOKEN_HEADS}")
+    scale = _check_scale(softmax_scale, q.shape[-1])
     if not (q.is_cuda and all(t.device == q.device for t in (k, v, cu_q, cu_k))):
         raise ValueError("q, k, v and cu_seqlens must be tensors of one GPU")
-    return cu_q.contiguous(), cu_k.contiguous(), _check_scale(softmax_scale, q.shape[-1])
+    return cu_q.contiguous(), cu_k.contiguous(), scale
 
 
 def _prep(x: torch.Tensor) -> torch.Tensor:

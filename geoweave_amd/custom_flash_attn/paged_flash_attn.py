@@ -32,7 +32,7 @@ __all__ = ["paged_flash_attn_inference_func"]
 MAX_KEYS = 0x7FFFF000
 
 
-def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens):
+def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale) -> float:
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, Hq, D] or [B, N, Hq, D], got {tuple(q.shape)}")
     if k_cache.dim() != 4:
@@ -50,12 +50,14 @@ def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens):
                          f"[{q.shape[0]}, W] and [{q.shape[0]}]")
     if block_table.shape[1] * k_cache.shape[1] > MAX_KEYS or q.numel() // d > MAX_KEYS:
         raise ValueError(f"keys of a sequence, and new tokens x heads, must not exceed {MAX_KEYS}")
+    scale = _check_scale(softmax_scale, d)
     if not (q.is_cuda and all(t.device == q.device for t in (k_cache, v_cache, block_table, cache_seqlens))):
         raise ValueError("q, the caches, block_table and cache_seqlens must be tensors of one GPU")
     for c in (k_cache, v_cache):
         # Copying a cache to align it would cost more than the call: the caller lays it out.
         if c.numel() and (c.stride(-1) != 1 or any(s % 8 for s in c.stride()[:-1]) or c.data_ptr() % 16):
             raise ValueError("caches need a unit last stride and 16-byte aligned rows")
+    return scale
 
 
 def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -63,8 +65,7 @@ def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_ca
                                     softmax_scale: Optional[float] = None, return_lse: bool = False,
                                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(o in q's shape and dtype, lse fp32 ``q.shape[:-1]`` where asked for); see the module docstring."""
-    _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens)
-    scale = _check_scale(softmax_scale, q.shape[-1])
+    scale = _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale)
     if q.stride(-1) != 1 or any(s % 8 for s in q.stride()[:-1]) or q.data_ptr() % 16:
         q = q.contiguous()
     if block_table.stride(-1) != 1:
