@@ -165,13 +165,13 @@ _SIGNATURES = {
     "gw_packed_attn_fwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "gw_packed_attn_fwd": (
         ctypes.c_int,
-        [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _p, _i64p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+        [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _p, _i64p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
          ctypes.c_int, ctypes.c_float, _p, _sz, _p],
     ),
     "gw_packed_attn_bwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "gw_packed_attn_bwd": (
         ctypes.c_int,
-        [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _p, _i64p, _p, _i64p, _p, _p, _i64p, _p, _i64p,
+        [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _p, _i64p, _p, _p, _i64p, _p, _p, _i64p, _p, _i64p,
          _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_float, _p, _sz, _p],
     ),
     "gw_paged_attn_fwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),

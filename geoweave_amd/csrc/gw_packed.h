@@ -248,6 +248,12 @@ constexpr uint32_t kPkExp = __is_same(E, FP16) ? 0x7C00u : 0x7F80u;
 template <typename E>
 __device__ __forceinline__ bool pk_not_finite(uint32_t half) { return (half & kPkExp<E>) == kPkExp<E>; }
 
+// Bits 15 and 31 tell whether the low and the high half are not finite: a full exponent and one more of its
+// units carry into the sign's place.
+template <typename E>
+__device__ __forceinline__ uint32_t pk_not_finite_bits(uint32_t w) {
+  return (w & 0x7FFF7FFFu) + (__is_same(E, FP16) ? 0x04000400u : 0x00800080u);
+}
 template <typename E>
 __device__ __forceinline__ uint32_t pk_finite_word(uint32_t w) {
   return (pk_not_finite<E>(w) ? 0u : w & 0xFFFFu) | (pk_not_finite<E>(w >> 16) ? 0u : w & 0xFFFF0000u);
@@ -258,9 +264,9 @@ __device__ __forceinline__ bool pk_clear_not_finite(uint4 (&q)[N]) {
   uint32_t any = 0u;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    any |= nonfinite2(q[i].x, kPkExp<E>) | nonfinite2(q[i].y, kPkExp<E>) | nonfinite2(q[i].z, kPkExp<E>) |
-           nonfinite2(q[i].w, kPkExp<E>);
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64(any != 0u) == 0ull, 1)) return false;
+    any |= pk_not_finite_bits<E>(q[i].x) | pk_not_finite_bits<E>(q[i].y) | pk_not_finite_bits<E>(q[i].z) |
+           pk_not_finite_bits<E>(q[i].w);
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0u) == 0ull, 1)) return false;
 #pragma unroll
   for (int i = 0; i < N; ++i)
     q[i] = make_uint4(pk_finite_word<E>(q[i].x), pk_finite_word<E>(q[i].y), pk_finite_word<E>(q[i].z),
@@ -283,23 +289,49 @@ __device__ __forceinline__ void pk_add_not_finite(const uint16_t* row, int half,
     }
 }
 
-// Stores a lane's column of a transposed accumulator (32 dims of one row) scaled by f: lanes l and
-// l ^ 32 exchange quads so that each stores eight consecutive dims.
+// What rounding a pair of floats to the 16-bit type leaves, in that type again.
 template <typename E>
-__device__ __forceinline__ void pk_store_col(uint16_t* row, const f32x16& acc, float f, int half, bool on) {
+__device__ __forceinline__ uint32_t pk_pair_rest(float a, float b, uint32_t rounded) {
+  return pack_pair(E{}, a - in_to_float(__is_same(E, FP16), rounded & 0xFFFFu),
+                   b - in_to_float(__is_same(E, FP16), rounded >> 16));
+}
+
+// Stores a lane's column of a transposed accumulator (32 dims of one row) scaled by f: lanes l and
+// l ^ 32 exchange quads so that each stores eight consecutive dims. REST: what the rounding left goes to
+// rest.
+template <typename E, bool REST = false>
+__device__ __forceinline__ void pk_store_col(uint16_t* row, const f32x16& acc, float f, int half, bool on,
+                                             uint16_t* rest = nullptr) {
 #pragma unroll
   for (int gp = 0; gp < 2; ++gp) {
-    uint32_t w[2][2];
+    uint32_t w[2][2], l[2][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int r = 4 * (2 * gp + u);
-      w[u][0] = pack_pair(E{}, acc[r] * f, acc[r + 1] * f);
-      w[u][1] = pack_pair(E{}, acc[r + 2] * f, acc[r + 3] * f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float x = acc[r + 2 * i] * f, y = acc[r + 2 * i + 1] * f;
+        w[u][i] = pack_pair(E{}, x, y);
+        if (REST) l[u][i] = pk_pair_rest<E>(x, y, w[u][i]);
+      }
     }
     const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
     const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
     if (on) *reinterpret_cast<uint4*>(row + 8 * (2 * gp + half)) = make_uint4(x[0], y[0], x[1], y[1]);
+    if constexpr (REST) {
+      const auto z = __builtin_amdgcn_permlane32_swap(l[0][0], l[1][0], false, false);
+      const auto t = __builtin_amdgcn_permlane32_swap(l[0][1], l[1][1], false, false);
+      if (on) *reinterpret_cast<uint4*>(rest + 8 * (2 * gp + half)) = make_uint4(z[0], t[0], z[1], t[1]);
+    }
   }
+}
+
+// Four dims of an output row, and what their rounding left (rest, nullable).
+template <typename E>
+__device__ __forceinline__ void pk_store4(uint16_t* row, uint16_t* rest, float a, float b, float c, float d) {
+  const uint32_t x = pack_pair(E{}, a, b), y = pack_pair(E{}, c, d);
+  *reinterpret_cast<uint2*>(row) = make_uint2(x, y);
+  if (rest) *reinterpret_cast<uint2*>(rest) = make_uint2(pk_pair_rest<E>(a, b, x), pk_pair_rest<E>(c, d, y));
 }
 
 // Waits for this wave's loads and LDS accesses, then for the other waves.

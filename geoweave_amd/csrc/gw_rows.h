@@ -11,6 +11,7 @@ struct RowsParams {
   const uint16_t* k;
   const uint16_t* v;
   uint16_t* o;
+  uint16_t* rest;       // nullable (packed): [Tq][H][D], what the rounding of o left
   float* lse;           // nullable
   float* part;          // parts of cut row tiles: [slot][Hk][16][D] normalised outputs,
   float* part_lse;      // [slot][Hk][16] log2 sums

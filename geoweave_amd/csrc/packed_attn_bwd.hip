@@ -1,7 +1,9 @@
 // Backward of the attention over packed sequences (gfx950): dQ, dK, dV without atomics on the
 // gradients, D = 64 or 128.
 //
-// With P the softmax weights (formed again from the forward's lse) and delta_i = o_i . do_i:
+// With P the softmax weights (formed again from the forward's lse) and delta_i = o_i . do_i, from o as it
+// was before its rounding (the forward keeps what the rounding left: where a row sees few keys, dP - delta
+// nearly cancels, and a delta from the rounded o would double the error of dQ and dK):
 //   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q.
 // Two passes, so that every gradient is summed by one workgroup in a fixed order: the dQ pass has the
 // forward's shape (rows of a key head in registers, K and V tiles through LDS: three products per
@@ -30,6 +32,7 @@ struct PackedBwdParams {
   const uint16_t* k;
   const uint16_t* v;
   const uint16_t* o;
+  const uint16_t* rest;  // [Tq][H][D] what the rounding of o left
   const uint16_t* dout;
   const float* lse;
   uint16_t* dq;
@@ -82,13 +85,14 @@ __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdPa
   const int li = threadIdx.x % LPR;
   for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
     const int t = pt.start + t0 + r / p.H, h = r % p.H;
-    float a[8], b[8];
+    float a[8], b[8], c[8];
     unpack8<E>(*reinterpret_cast<const uint4*>(p.o + (int64_t)t * p.ost + (int64_t)h * p.osh + li * 8), a);
+    unpack8<E>(*reinterpret_cast<const uint4*>(p.rest + ((int64_t)t * p.H + h) * D + li * 8), c);
     unpack8<E>(*reinterpret_cast<const uint4*>(p.dout + (int64_t)t * p.gst + (int64_t)h * p.gsh + li * 8), b);
     float s = 0.f, nn = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      s = fmaf(a[i], b[i], s);
+      s = fmaf(a[i] + c[i], b[i], s);
       nn = fmaf(b[i], b[i], nn);
     }
     s = group_sum<LPR>(s);
@@ -177,14 +181,17 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   if (kFp16) e = pk_scale_exp(sqrtf(pair_sum(nn)) * __uint_as_float(p.max_v[(int64_t)pt.seq * p.Hk + hk]));
   const int64_t srow = (int64_t)head * p.Tq + t;
   const float nlse = p.nlse[srow] * sl2 - kPScale<E> + (float)e;  // p 2^e = 2^(s - lse + e)
-  // dP - delta: delta is where the products start, in a register block of its own; fp16 at D = 64, whose
-  // scale takes the registers, adds it afterwards.
-  constexpr bool kAddDelta = kFp16 && D == 64;
+  // dP - delta: at D = 128 delta is where the products start, in a register block of its own; at D = 64,
+  // where three waves share a SIMD's registers, it is added afterwards (with the block 124 bytes of
+  // scratch a lane and 860 us for 563 on 6 scenes of 2 to 8 views).
+  constexpr bool kAddDelta = D == 64;
   const float ndelta = p.ndelta[srow];
   f32x16 dp0;
 #pragma unroll
   for (int r = 0; r < 16; ++r) dp0[r] = kAddDelta ? 0.f : ndelta;
-  const float unscale = ldexpf(p.scale, -e);
+  // The weight of a row that sees one key is 1 whatever its score: no gradient, where rounding would
+  // leave dP - delta a little off 0.
+  const float unscale = lim == 0 ? 0.f : ldexpf(p.scale, -e);
   auto last_key = [&](int r) { return p.causal ? min(min(r, rows - 1) / p.G + shift, lk - 1) : lk - 1; };
   const int lim_wave = base < rows ? last_key(base + 31) : -1;
   const int keys = last_key(row0 + BM - 1) + 1;
@@ -411,11 +418,11 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
     for (int x = 0; x < 16; ++x) ds[x] = kFp16 ? w[x] * dscale * dp[x] : w[x] * dp[x];
     if constexpr (decltype(masked)::value) {
       const int need = key - shift - i0 - 4 * half;
+      const int need_ds = max(key, 1) - shift - i0 - 4 * half;  // the first key's one-key row has dS = 0
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        const bool sees = 8 * (x / 4) + x % 4 >= need;
-        w[x] = sees ? w[x] : 0.f;
-        ds[x] = sees ? ds[x] : 0.f;
+        w[x] = 8 * (x / 4) + x % 4 >= need ? w[x] : 0.f;
+        ds[x] = 8 * (x / 4) + x % 4 >= need_ds ? ds[x] : 0.f;
       }
     }
 #pragma unroll
@@ -477,7 +484,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
       }
     }
   }
-  const float fk = kFp16 ? ldexpf(p.scale, -e) : p.scale, fv = kFp16 ? ldexpf(1.f, -14) : 1.f;
+  // Rows of a sequence of one key all have dS = 0.
+  const float fk = pt.len == 1 ? 0.f : kFp16 ? ldexpf(p.scale, -e) : p.scale;
+  const float fv = kFp16 ? ldexpf(1.f, -14) : 1.f;
   const int64_t t = pt.start + (on ? key : 0);
   if (p.split_dkv > 1) {
     const int64_t part = (int64_t)p.Tk * p.Hk * D;
@@ -611,7 +620,7 @@ extern "C" size_t gw_packed_attn_bwd_workspace_size(int64_t n, int64_t Tq, int64
 extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
                                   const int64_t* k_strides, const void* v, const int64_t* v_strides,
                                   const int32_t* cu_q, const int32_t* cu_k, const void* o, const int64_t* o_strides,
-                                  const void* dout, const int64_t* do_strides, const float* lse, void* dq,
+                                  const void* o_rest, const void* dout, const int64_t* do_strides, const float* lse, void* dq,
                                   const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                                   const int64_t* dv_strides, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk,
                                   int64_t D, int causal, float softmax_scale, void* workspace, size_t workspace_bytes,
@@ -623,10 +632,10 @@ extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_str
   if (rc != GW_OK) return rc;
   if (Tq == 0 && Tk == 0) return GW_OK;
   GW_CHECK_ARG(cu_q && cu_k && q_strides && k_strides && v_strides && o_strides && do_strides && dq_strides &&
-                   dk_strides && dv_strides && (Tq == 0 || (q && o && dout && lse && dq)) && (Tk == 0 || (k && v && dk && dv)),
+                   dk_strides && dv_strides && (Tq == 0 || (q && o && o_rest && dout && lse && dq)) && (Tk == 0 || (k && v && dk && dv)),
                "a tensor is missing");
   GW_CHECK_ARG(pk_rows_ok(q, q_strides) && pk_rows_ok(k, k_strides) && pk_rows_ok(v, v_strides) &&
-                   pk_rows_ok(o, o_strides) && pk_rows_ok(dout, do_strides) && pk_rows_ok(dq, dq_strides) &&
+                   pk_rows_ok(o, o_strides) && aligned16(o_rest) && pk_rows_ok(dout, do_strides) && pk_rows_ok(dq, dq_strides) &&
                    pk_rows_ok(dk, dk_strides) && pk_rows_ok(dv, dv_strides),
                "q, k, v, o, dO, dq, dk and dv need 16-byte aligned rows, with token strides in [0, 2^24)");
   const size_t need = gw_packed_attn_bwd_workspace_size(n, Tq, Tk, Hq, Hk, D);
@@ -637,6 +646,7 @@ extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_str
   p.k = static_cast<const uint16_t*>(k);
   p.v = static_cast<const uint16_t*>(v);
   p.o = static_cast<const uint16_t*>(o);
+  p.rest = static_cast<const uint16_t*>(o_rest);
   p.dout = static_cast<const uint16_t*>(dout);
   p.lse = lse;
   p.dq = static_cast<uint16_t*>(dq);

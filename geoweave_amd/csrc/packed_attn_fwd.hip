@@ -33,6 +33,7 @@ struct PackedFwdParams {
   const uint16_t* k;
   const uint16_t* v;
   uint16_t* o;
+  uint16_t* rest;  // nullable: [Tq][H][D], what the rounding of o left
   float* lse;
   const int32_t* cu_q;
   const int32_t* cu_k;
@@ -238,7 +239,12 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
     }
     uint16_t* orow = p.o + t * p.ost + (int64_t)head[a] * p.osh;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) pk_store_col<E>(orow + 32 * db, acc[a][db], inv, half, on[a]);
+    for (int db = 0; db < DB; ++db) {
+      if (p.rest)
+        pk_store_col<E, true>(orow + 32 * db, acc[a][db], inv, half, on[a], p.rest + (t * p.H + head[a]) * D + 32 * db);
+      else
+        pk_store_col<E>(orow + 32 * db, acc[a][db], inv, half, on[a]);
+    }
     if (on[a] && half == 0 && p.lse) p.lse[t * p.H + head[a]] = lt == 0.f ? -INFINITY : (m[a] + flog2(lt)) * kDLn2;
   }
 }
@@ -279,8 +285,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackedFwdParams 
     out.w = fmaf(y.w, f, out.w);
   }
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  *reinterpret_cast<uint2*>(p.o + t * p.ost + (int64_t)head * p.osh + 4 * c) =
-      make_uint2(pack_pair(E{}, out.x * inv, out.y * inv), pack_pair(E{}, out.z * inv, out.w * inv));
+  pk_store4<E>(p.o + t * p.ost + (int64_t)head * p.osh + 4 * c, p.rest ? p.rest + row * D + 4 * c : nullptr, out.x * inv,
+               out.y * inv, out.z * inv, out.w * inv);
   if (c == 0 && p.lse) p.lse[row] = lt == 0.f ? -INFINITY : (mx + flog2(lt)) * kDLn2;
 }
 
@@ -349,8 +355,8 @@ extern "C" size_t gw_packed_attn_fwd_workspace_size(int64_t n, int64_t Tq, int64
 extern "C" int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
                                   const int64_t* k_strides, const void* v, const int64_t* v_strides,
                                   const int32_t* cu_q, const int32_t* cu_k, void* o, const int64_t* o_strides,
-                                  float* lse, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
-                                  int causal, float softmax_scale, void* workspace, size_t workspace_bytes,
+                                  void* o_rest, float* lse, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk,
+                                  int64_t D, int causal, float softmax_scale, void* workspace, size_t workspace_bytes,
                                   void* stream) {
   using namespace gw;
   clear_error();
@@ -360,13 +366,15 @@ extern "C" int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_str
   if (Tq == 0) return GW_OK;
   GW_CHECK_ARG(q && o && cu_q && cu_k && q_strides && k_strides && v_strides && o_strides && (Tk == 0 || (k && v)),
                "a tensor is missing");
-  GW_CHECK_ARG(pk_rows_ok(q, q_strides) && pk_rows_ok(k, k_strides) && pk_rows_ok(v, v_strides) && pk_rows_ok(o, o_strides),
+  GW_CHECK_ARG(pk_rows_ok(q, q_strides) && pk_rows_ok(k, k_strides) && pk_rows_ok(v, v_strides) &&
+                   pk_rows_ok(o, o_strides) && aligned16(o_rest),
                "q, k, v and o need 16-byte aligned rows, with token strides in [0, 2^24)");
   PackedFwdParams p = {};
   p.q = static_cast<const uint16_t*>(q);
   p.k = static_cast<const uint16_t*>(k);
   p.v = static_cast<const uint16_t*>(v);
   p.o = static_cast<uint16_t*>(o);
+  p.rest = static_cast<uint16_t*>(o_rest);
   p.lse = lse;
   p.cu_q = cu_q;
   p.cu_k = cu_k;
@@ -397,6 +405,7 @@ extern "C" int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_str
     r.k = p.k;
     r.v = p.v;
     r.o = p.o;
+    r.rest = p.rest;
     r.lse = lse;
     r.cu_q = cu_q;
     r.cu_k = cu_k;

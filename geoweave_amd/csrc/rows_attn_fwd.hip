@@ -304,8 +304,8 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int u = 0; u < DV / 2; ++u) any |= nonfinite2(b.v[j].w[u], kPkExp<E>);
-        if (__builtin_amdgcn_ballot_w64(any != 0u) != 0ull) {
+          for (int u = 0; u < DV / 2; ++u) any |= pk_not_finite_bits<E>(b.v[j].w[u]);
+        if (__builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0u) != 0ull) {
           unclean = true;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -436,9 +436,10 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
   const int tk = rr / p.G, hd = hk * p.G + (rr - tk * p.G);
   const int64_t tg = PAGED ? (int64_t)pt.seq * p.osb + (int64_t)tk * p.ost : (int64_t)(sq.q0 + tk) * p.ost;
   uint16_t* dst = p.o + tg + (int64_t)hd * p.osh + c * DV;
+  uint16_t* rest = !PAGED && p.rest ? p.rest + ((int64_t)(sq.q0 + tk) * p.H + hd) * D + c * DV : nullptr;
 #pragma unroll
   for (int u = 0; u < DV; u += 4)
-    *reinterpret_cast<uint2*>(dst + u) = make_uint2(pack_pair(E{}, out[u], out[u + 1]), pack_pair(E{}, out[u + 2], out[u + 3]));
+    pk_store4<E>(dst + u, rest ? rest + u : nullptr, out[u], out[u + 1], out[u + 2], out[u + 3]);
   if (c == 0 && p.lse) p.lse[(int64_t)(PAGED ? pt.seq * p.Tq + tk : sq.q0 + tk) * p.H + hd] = l2 * kDLn2;
 }
 
@@ -513,8 +514,9 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
   const int tk = rr / p.G, hd = hk * p.G + (rr - tk * p.G);
   const int64_t tg = PAGED ? (int64_t)pt.seq * p.osb + (int64_t)tk * p.ost : (int64_t)(sq.q0 + tk) * p.ost;
-  *reinterpret_cast<uint2*>(p.o + tg + (int64_t)hd * p.osh + c * 4) =
-      make_uint2(pack_pair(E{}, out.x * inv, out.y * inv), pack_pair(E{}, out.z * inv, out.w * inv));
+  pk_store4<E>(p.o + tg + (int64_t)hd * p.osh + c * 4,
+               !PAGED && p.rest ? p.rest + ((int64_t)(sq.q0 + tk) * p.H + hd) * D + c * 4 : nullptr, out.x * inv, out.y * inv,
+               out.z * inv, out.w * inv);
   if (c == 0 && p.lse)
     p.lse[(int64_t)(PAGED ? pt.seq * p.Tq + tk : sq.q0 + tk) * p.H + hd] =
         lt == 0.f ? -INFINITY : (mx + flog2(lt)) * kDLn2;

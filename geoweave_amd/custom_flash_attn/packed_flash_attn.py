@@ -96,26 +96,27 @@ def _rows(x: torch.Tensor):
     return x.data_ptr(), _lib.strides2(st, sh)
 
 
-def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool):
-    """(o, lse | None) for a native head dim."""
+def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool, want_rest: bool = False):
+    """(o, lse | None, what o's rounding left | None) for a native head dim."""
     q, k, v = _prep(q), _prep(k), _prep(v)
     o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if want_lse else None
+    rest = torch.empty_like(o) if want_rest else None
     if q.shape[0] == 0:
-        return o, lse
+        return o, lse, rest
     lib = _lib.load()
     sizes = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
     nbytes = int(lib.gw_packed_attn_fwd_workspace_size(*sizes))
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     with _lib.on_device(q.device):
         rc = lib.gw_packed_attn_fwd(_lib.dtype_code(q.dtype), *_rows(q), *_rows(k), *_rows(v), cu_q.data_ptr(),
-                                    cu_k.data_ptr(), *_rows(o), _lib.ptr(lse), *sizes, int(causal), scale,
+                                    cu_k.data_ptr(), *_rows(o), _lib.ptr(rest), _lib.ptr(lse), *sizes, int(causal), scale,
                                     _lib.ptr(ws), nbytes, _lib.stream_handle(q.device))
     _lib.check(rc, "gw_packed_attn_fwd")
-    return o, lse
+    return o, lse, rest
 
 
-def _backward(do, q, k, v, cu_q, cu_k, o, lse, causal: bool, scale: float):
+def _backward(do, q, k, v, cu_q, cu_k, o, rest, lse, causal: bool, scale: float):
     q, k, v, o, do = (_prep(x) for x in (q, k, v, o, do))
     dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
     if q.shape[0] == 0 and k.shape[0] == 0:
@@ -126,7 +127,7 @@ def _backward(do, q, k, v, cu_q, cu_k, o, lse, causal: bool, scale: float):
     ws = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
     with _lib.on_device(q.device):
         rc = lib.gw_packed_attn_bwd(_lib.dtype_code(q.dtype), *_rows(q), *_rows(k), *_rows(v), cu_q.data_ptr(),
-                                    cu_k.data_ptr(), *_rows(o), *_rows(do), lse.data_ptr(), *_rows(dq), *_rows(dk),
+                                    cu_k.data_ptr(), *_rows(o), rest.data_ptr(), *_rows(do), lse.data_ptr(), *_rows(dq), *_rows(dk),
                                     *_rows(dv), n, tq, tk, hq, hk, d, int(causal), scale, ws.data_ptr(), nbytes,
                                     _lib.stream_handle(q.device))
     _lib.check(rc, "gw_packed_attn_bwd")
@@ -141,22 +142,22 @@ class PackedFlashAttnFunc(torch.autograd.Function):
         d = q.shape[-1]
         dp = d if d in NATIVE_HEAD_DIMS else _padded_head_dim(d)
         qp, kp, vp = (q, k, v) if dp == d else (_pad_head_dim(x, dp) for x in (q, k, v))
-        o, lse = _forward(qp, kp, vp, cu_q, cu_k, causal, scale, True)
+        o, lse, rest = _forward(qp, kp, vp, cu_q, cu_k, causal, scale, True, True)
         if dp != d:
             o = o[..., :d].contiguous()
-        ctx.save_for_backward(q, k, v, cu_q, cu_k, o, lse)
+        ctx.save_for_backward(q, k, v, cu_q, cu_k, o, rest, lse)
         ctx.causal, ctx.scale = causal, scale
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, cu_q, cu_k, o, lse = ctx.saved_tensors
+        q, k, v, cu_q, cu_k, o, rest, lse = ctx.saved_tensors
         d = q.shape[-1]
         dp = d if d in NATIVE_HEAD_DIMS else _padded_head_dim(d)
         args = [do, q, k, v] if dp == d else [_pad_head_dim(x, dp) for x in (do, q, k, v)]
         op = o if dp == d else _pad_head_dim(o, dp)
-        grads = _backward(*args, cu_q, cu_k, op, lse, ctx.causal, ctx.scale)
+        grads = _backward(*args, cu_q, cu_k, op, rest, lse, ctx.causal, ctx.scale)
         if dp != d:
             grads = [g[..., :d].contiguous() for g in grads]
         return (*grads, None, None, None, None)
@@ -180,8 +181,8 @@ def packed_flash_attn_inference_func(q: torch.Tensor, k: torch.Tensor, v: torch.
     cu_q, cu_k, scale = _check_inputs(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale)
     d = q.shape[-1]
     if d in NATIVE_HEAD_DIMS:
-        return _forward(q, k, v, cu_q, cu_k, bool(causal), scale, return_lse)
+        return _forward(q, k, v, cu_q, cu_k, bool(causal), scale, return_lse)[:2]
     dp = _padded_head_dim(d)
-    o, lse = _forward(_pad_head_dim(q, dp), _pad_head_dim(k, dp), _pad_head_dim(v, dp), cu_q, cu_k, bool(causal),
-                      scale, return_lse)
+    o, lse, _ = _forward(_pad_head_dim(q, dp), _pad_head_dim(k, dp), _pad_head_dim(v, dp), cu_q, cu_k, bool(causal),
+                         scale, return_lse)
     return o[..., :d].contiguous(), lse

@@ -664,7 +664,8 @@ int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strides, void* y
  * sequence i has the query tokens [cu_q[i], cu_q[i + 1]) and the keys [cu_k[i], cu_k[i + 1]). A
  * query attends to its sequence's keys, causal != 0: key j <= i + Lk - Lq (i, j within the sequence).
  * A row with no key, and a token in no sequence, gets o = 0, lse = -inf. lse (nullable): fp32
- * [Tq, Hq], natural log. Bounds outside [0, Tq] or [0, Tk] are clamped.
+ * [Tq, Hq], natural log. o_rest (nullable): [Tq, Hq, D] contiguous in o's type, what the rounding of o
+ * left (the backward needs it). Bounds outside [0, Tq] or [0, Tk] are clamped.
  * D in {64, 128}, bf16 or fp16, softmax_scale > 0; 16-byte aligned rows, token strides in [0, 2^24)
  * elements; tokens x Hq below 2^31 - 2^12. workspace: gw_packed_attn_fwd_workspace_size(...) bytes,
  * 16-byte aligned (parts of the keys, where they are split over workgroups). Nothing is read from the device by the host: a captured graph may
@@ -673,22 +674,22 @@ int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strides, void* y
 size_t gw_packed_attn_fwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
 int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                        const void* v, const int64_t* v_strides, const int32_t* cu_q, const int32_t* cu_k,
-                       void* o, const int64_t* o_strides, float* lse, int64_t n, int64_t Tq, int64_t Tk,
-                       int64_t Hq, int64_t Hk, int64_t D, int causal, float softmax_scale, void* workspace,
+                       void* o, const int64_t* o_strides, void* o_rest, float* lse, int64_t n, int64_t Tq,
+                       int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int causal, float softmax_scale, void* workspace,
                        size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------
  * Backward of gw_packed_attn_fwd: dq [Tq, Hq, D], dk and dv [Tk, Hk, D] (each element written once;
- * tokens of no sequence, and rows without keys, get zeros) from the forward's o and lse and the
+ * tokens of no sequence, and rows without keys, get zeros) from the forward's o, o_rest and lse and the
  * gradient dout of o. No float atomics: the same inputs give the same bits. Arguments and limits as
  * there. workspace: gw_packed_attn_bwd_workspace_size(...) bytes, 16-byte aligned.
  * ------------------------------------------------------------------------------------ */
 size_t gw_packed_attn_bwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
 int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                        const void* v, const int64_t* v_strides, const int32_t* cu_q, const int32_t* cu_k,
-                       const void* o, const int64_t* o_strides, const void* dout, const int64_t* do_strides,
-                       const float* lse, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides,
-                       void* dv, const int64_t* dv_strides, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq,
+                       const void* o, const int64_t* o_strides, const void* o_rest, const void* dout,
+                       const int64_t* do_strides, const float* lse, void* dq, const int64_t* dq_strides, void* dk,
+                       const int64_t* dk_strides, void* dv, const int64_t* dv_strides, int64_t n, int64_t Tq, int64_t Tk, int64_t Hq,
                        int64_t Hk, int64_t D, int causal, float softmax_scale, void* workspace,
                        size_t workspace_bytes, void* stream);
 

@@ -141,11 +141,11 @@ def test_view_positions_on_the_cpu():
 
 def _fwd(**over):
     lib, s = _lib.load(), _lib.strides2(256, 64)
-    a = dict(dtype=0, q=256, qs=s, k=256, ks=s, v=256, vs=s, cu=256, o=256, os=s, lse=None, n=1, tq=8, tk=8, hq=4, hk=4,
+    a = dict(dtype=0, q=256, qs=s, k=256, ks=s, v=256, vs=s, cu=256, o=256, os=s, rest=None, lse=None, n=1, tq=8, tk=8, hq=4, hk=4,
              d=64, causal=0, scale=0.125, ws=None, nbytes=0)
     a.update(over)
     rc = lib.gw_packed_attn_fwd(a["dtype"], a["q"], a["qs"], a["k"], a["ks"], a["v"], a["vs"], a["cu"], a["cu"], a["o"],
-                                a["os"], a["lse"], a["n"], a["tq"], a["tk"], a["hq"], a["hk"], a["d"], a["causal"],
+                                a["os"], a["rest"], a["lse"], a["n"], a["tq"], a["tk"], a["hq"], a["hk"], a["d"], a["causal"],
                                 a["scale"], a["ws"], a["nbytes"], None)
     return rc, lib.gw_last_error().decode()
 
@@ -219,14 +219,15 @@ def test_backward_abi():
     need = lib.gw_packed_attn_bwd_workspace_size(1, 8, 8, 4, 4, 64)
     assert need >= 8 * 4 * 8
 
-    def call(ws=256, nbytes=need, d=64, do=256, lse=256):
-        rc = lib.gw_packed_attn_bwd(0, 256, s, 256, s, 256, s, 256, 256, 256, s, do, s, lse, 256, s, 256, s, 256, s, 1, 8, 8, 4,
+    def call(ws=256, nbytes=need, d=64, do=256, lse=256, rest=256):
+        rc = lib.gw_packed_attn_bwd(0, 256, s, 256, s, 256, s, 256, 256, 256, s, rest, do, s, lse, 256, s, 256, s, 256, s, 1, 8, 8, 4,
                                     4, d, 0, 0.125, ws, nbytes, None)
         return rc, lib.gw_last_error().decode()
 
     for kw, code, word in ((dict(nbytes=need - 1), 1, "workspace"), (dict(ws=None), 1, "workspace"),
                            (dict(ws=264), 1, "workspace"), (dict(d=32), 2, "head dim"), (dict(do=None), 1, "missing"),
-                           (dict(lse=None), 1, "missing"), (dict(do=260), 1, "aligned")):
+                           (dict(lse=None), 1, "missing"), (dict(do=260), 1, "aligned"), (dict(rest=None), 1, "missing"),
+                           (dict(rest=8), 1, "aligned")):
         rc, msg = call(**kw)
         assert rc == code and word in msg, (kw, rc, msg)
 
