@@ -15,6 +15,8 @@ struct RowsParams {
   float* lse;           // nullable
   float* part;          // parts of cut row tiles: [slot][Hk][16][D] normalised outputs,
   float* part_lse;      // [slot][Hk][16] log2 sums
+  int2* cut;            // [tile] of a split call: where a row tile's parts are kept, and how many (paged: tile
+                        // sequence * tiles of one + tile; packed: 2 sequence + tile)
   // Paged: table [B][table_width] page numbers (row stride table_stride), lens [B].
   const int32_t* table;
   const int32_t* lens;
@@ -38,9 +40,15 @@ constexpr int kRowsMax = 32;
 
 // Parts per key head to aim at: about four workgroups per CU over all heads.
 inline int rows_want(int64_t Hk) { return (int)(1024 / Hk > 0 ? 1024 / Hk : 1); }
-// Workspace of the parts of a split call. A tile is cut where its keys exceed the part length, so it
-// has fewer than two parts per part length of keys, and all cut tiles fewer than 2 want.
-inline size_t rows_workspace(int64_t Hk, int64_t D) { return (size_t)2 * rows_want(Hk) * Hk * 16 * (D + 1) * sizeof(float); }
+// Row tiles of a call at most: the join's workgroups, and the entries of `cut`.
+inline int64_t rows_tiles(bool paged, int64_t n, int64_t Tq, int64_t G) {
+  return paged ? n * ((Tq * G + 15) / 16) : 2 * (n + 2);
+}
+// Workspace of a split call. A tile is cut where its keys exceed the part length, so it has fewer than
+// two parts per part length of keys, and all cut tiles fewer than 2 want.
+inline size_t rows_workspace(int64_t tiles, int64_t Hk, int64_t D) {
+  return (size_t)2 * rows_want(Hk) * Hk * 16 * (D + 1) * sizeof(float) + (size_t)tiles * sizeof(int2);
+}
 // Launches on checked arguments (dtype bf16 or fp16, D 64 or 128); p.split and p.want are set.
 int rows_attn(int dtype, int D, bool paged, RowsParams p, void* workspace, hipStream_t stream);
 

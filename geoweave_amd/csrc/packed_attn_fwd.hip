@@ -312,11 +312,11 @@ FwdPlan packed_fwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
   // 4 x 1,374 tokens 42.7 and 49.3 us.
   f.qpw = D == 64 && rows / seqs >= 2048 && (rows / 256) * Hk >= 1024 ? 2 : 1;
   const int64_t wgs = (rows / (128 * f.qpw) + (rows / seqs < 128 ? n : n / 2) + 1) * Hk;
-  int64_t split = 512 / (wgs > 0 ? wgs : 1);
+  int64_t split = f.rows && rows / seqs <= 16 ? 1 : 512 / (wgs > 0 ? wgs : 1);
   if (split > keys / 512) split = keys / 512;
   if (split > 16) split = 16;
   f.split = split > 1 ? (int)split : 1;
-  f.rows_bytes = f.rows ? (rows_workspace(Hk, D) + 255) / 256 * 256 : 0;
+  f.rows_bytes = f.rows ? (rows_workspace(rows_tiles(false, n, Tq, G), Hk, D) + 255) / 256 * 256 : 0;
   f.split_bytes = f.tiles && f.split > 1 ? (size_t)f.split * Tq * Hq * (D + 1) * sizeof(float) : 0;
   return f;
 }

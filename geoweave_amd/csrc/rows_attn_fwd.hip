@@ -30,7 +30,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kRows = 16;
-constexpr int kRowsPart = 128;       // a part is a multiple of this many keys (4 waves x 32)
+constexpr int kRowsPart = 256;       // a part is a multiple of this many keys (4 waves x 32, twice)
 constexpr float kRowsSumCap = 32768.f;
 
 __device__ __forceinline__ f32x4 mma16(BF16, uint4 a, uint4 b, f32x4 c) {
@@ -74,18 +74,31 @@ __device__ __forceinline__ RowsSeq rows_seq(const RowsParams& p, int i) {
   return s;
 }
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+// Inclusive sums over the lanes of a wave, by lane exchanges within the vector unit: within 16 lanes, then
+// the last lane of each row on to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int rows_dpp(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x += rows_dpp<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x += rows_dpp<0x112, 0xF>(x);
+  x += rows_dpp<0x114, 0xF>(x);
+  x += rows_dpp<0x118, 0xF>(x);
+  x += rows_dpp<0x142, 0xA>(x);  // row_bcast 15 into rows 1 and 3
+  x += rows_dpp<0x143, 0xC>(x);  // row_bcast 31 into rows 2 and 3
   return x;
 }
-__device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
+__device__ __forceinline__ int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+// Sum over the wave of values below 2^62, 24 bits at a time (64 of those stay below 2^30).
+__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+  int64_t total = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
+  for (int part = 0; part < 3; ++part) {
+    const int piece = (int)((x >> (24 * part)) & 0xFFFFFF);
+    total += (int64_t)lane_of(wave_scan(piece), 63) << (24 * part);
   }
-  return x;
+  return total;
 }
 
 struct RowsPart {
@@ -116,10 +129,10 @@ __device__ __forceinline__ int rows_part_len(const RowsParams& p, int lane) {
   return (int)((max(len, (int64_t)kRowsPart) + kRowsPart - 1) / kRowsPart * kRowsPart);
 }
 
-// The part of slot `slot`, or (tile_index) the row tile of that number.
+// The part of slot `slot`.
 template <bool PAGED>
-__device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, bool tile_index, int lane) {
-  RowsPart r = {-1, 0, 0, 1, 0, 0x7fffff80};
+__device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, int lane) {
+  RowsPart r = {-1, 0, 0, 1, 0, 0x7fffff00};
   if (!p.split) {  // paged only: as many row tiles in each sequence
     const int rt = (p.Tq * p.G + kRows - 1) / kRows;
     r.seq = slot / rt;
@@ -127,7 +140,7 @@ __device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, boo
     if (r.seq >= p.n) r.seq = -1;
     return r;
   }
-  r.len = rows_part_len<PAGED>(p, lane);
+  r.len = __builtin_amdgcn_readfirstlane(rows_part_len<PAGED>(p, lane));
   const int nseq = rows_nseq<PAGED>(p);
   int before = 0, cut_before = 0;
   for (int i0 = 0; i0 < nseq; i0 += 64) {
@@ -138,28 +151,22 @@ __device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, boo
       tiles = rows_tiles_of<PAGED>(p, s);
       parts = max(1, (int)(((int64_t)s.lk + r.len - 1) / r.len));
     }
-    const int mine = tile_index ? tiles : tiles * parts, cut = parts > 1 ? tiles * parts : 0;
-    const int incl = wave_scan(mine, lane), cut_incl = wave_scan(cut, lane);
+    const int mine = tiles * parts, cut = parts > 1 ? mine : 0;
+    const int incl = wave_scan(mine), cut_incl = wave_scan(cut);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(before + incl > slot);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      const int at = slot - before - (__shfl(incl, l) - __shfl(mine, l));
-      r.parts = __shfl(parts, l);
+      const int at = slot - before - lane_of(incl - mine, l);
+      r.parts = lane_of(parts, l);
       r.seq = i0 + l;
-      r.tile = tile_index ? at : at / r.parts;
-      r.part = tile_index ? 0 : at - r.tile * r.parts;
-      r.first = cut_before + (__shfl(cut_incl, l) - __shfl(cut, l)) + r.tile * r.parts;
+      r.tile = at / r.parts;
+      r.part = at - r.tile * r.parts;
+      r.first = cut_before + lane_of(cut_incl - cut, l) + r.tile * r.parts;
       break;
     }
-    before += __shfl(incl, 63);
-    cut_before += __shfl(cut_incl, 63);
+    before += lane_of(incl, 63);
+    cut_before += lane_of(cut_incl, 63);
   }
-  r.seq = __builtin_amdgcn_readfirstlane(r.seq);
-  r.tile = __builtin_amdgcn_readfirstlane(r.tile);
-  r.part = __builtin_amdgcn_readfirstlane(r.part);
-  r.parts = __builtin_amdgcn_readfirstlane(r.parts);
-  r.first = __builtin_amdgcn_readfirstlane(r.first);
-  r.len = __builtin_amdgcn_readfirstlane(r.len);
   return r;
 }
 
@@ -205,8 +212,10 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, i16 = lane & 15;
   const int hk = blockIdx.x % p.Hk, slot = blockIdx.x / p.Hk;
-  const RowsPart pt = rows_find<PAGED>(p, slot, false, lane);
+  const RowsPart pt = rows_find<PAGED>(p, slot, lane);
   if (pt.seq < 0) return;
+  if (p.split && pt.part == 0 && hk == 0 && threadIdx.x == 0)  // for the join
+    p.cut[PAGED ? pt.seq * ((p.Tq * p.G + kRows - 1) / kRows) + pt.tile : 2 * pt.seq + pt.tile] = make_int2(pt.first, pt.parts);
   const RowsSeq sq = rows_seq<PAGED>(p, pt.seq);
   const int lk = __builtin_amdgcn_readfirstlane(sq.lk), k0 = __builtin_amdgcn_readfirstlane(sq.k0);
   const int rows = sq.lq * p.G;
@@ -455,16 +464,20 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
   __shared__ float4 so[GROUPS][LPR];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int hk = blockIdx.x % p.Hk, row = blockIdx.y;
-  const RowsPart pt = rows_find<PAGED>(p, blockIdx.x / p.Hk, true, lane);
-  if (pt.seq < 0 || pt.parts == 1) return;
-  const RowsSeq sq = rows_seq<PAGED>(p, pt.seq);
-  const int rr = pt.tile * kRows + row;
-  if (rr >= sq.lq * p.G) return;
+  const int at_tile = blockIdx.x / p.Hk;
+  const int per = PAGED ? (p.Tq * p.G + kRows - 1) / kRows : 2;
+  const int seq = at_tile / per, tile = at_tile - seq * per;
+  const RowsSeq sq = rows_seq<PAGED>(p, seq);
+  const int rr = tile * kRows + row;
+  if (rr >= sq.lq * p.G || (!PAGED && sq.lq * p.G > kRowsMax)) return;
+  const int2 where = p.cut[at_tile];
+  const int parts = where.y;
+  if (parts == 1) return;
   const int64_t step = (int64_t)p.Hk * kRows;
-  const int64_t at = ((int64_t)pt.first * p.Hk + hk) * kRows + row;
+  const int64_t at = ((int64_t)where.x * p.Hk + hk) * kRows + row;
   // The largest log2 sum (NaN if one is).
   float mx = -INFINITY;
-  for (int i = tid; i < pt.parts; i += 256) {
+  for (int i = tid; i < parts; i += 256) {
     const float x = p.part_lse[at + i * step];
     mx = x > mx || x != x ? x : mx;
     if (mx != mx) break;
@@ -478,8 +491,8 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
   const int c = tid % LPR, grp = tid / LPR;
   float lt = 0.f;
   float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < pt.parts; p0 += kJoinParts) {
-    const int np = min(kJoinParts, pt.parts - p0);
+  for (int p0 = 0; p0 < parts; p0 += kJoinParts) {
+    const int np = min(kJoinParts, parts - p0);
     __syncthreads();
     for (int i = tid; i < np; i += 256) {
       const float x = p.part_lse[at + (p0 + i) * step];
@@ -513,29 +526,29 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
   }
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
   const int tk = rr / p.G, hd = hk * p.G + (rr - tk * p.G);
-  const int64_t tg = PAGED ? (int64_t)pt.seq * p.osb + (int64_t)tk * p.ost : (int64_t)(sq.q0 + tk) * p.ost;
+  const int64_t tg = PAGED ? (int64_t)seq * p.osb + (int64_t)tk * p.ost : (int64_t)(sq.q0 + tk) * p.ost;
   pk_store4<E>(p.o + tg + (int64_t)hd * p.osh + c * 4,
                !PAGED && p.rest ? p.rest + ((int64_t)(sq.q0 + tk) * p.H + hd) * D + c * 4 : nullptr, out.x * inv, out.y * inv,
                out.z * inv, out.w * inv);
   if (c == 0 && p.lse)
-    p.lse[(int64_t)(PAGED ? pt.seq * p.Tq + tk : sq.q0 + tk) * p.H + hd] =
+    p.lse[(int64_t)(PAGED ? seq * p.Tq + tk : sq.q0 + tk) * p.H + hd] =
         lt == 0.f ? -INFINITY : (mx + flog2(lt)) * kDLn2;
 }
 
 template <typename E, int D, bool PAGED>
 int rows_launch(const RowsParams& p, hipStream_t stream) {
-  // Row tiles at most: packed, one or two of each sequence of at most kRowsMax rows (and no more than
-  // the rows in all allow).
-  int64_t tiles = PAGED ? (int64_t)p.n * (((int64_t)p.Tq * p.G + kRows - 1) / kRows)
-                        : (int64_t)p.Tq * p.G / kRows + p.n + 2;
-  if (!PAGED) tiles = tiles < 2ll * (p.n + 2) ? tiles : 2ll * (p.n + 2);
+  // Packed: a sequence of at most kRowsMax rows has one or two tiles, and all have no more than the rows
+  // in all allow.
+  const int64_t joins = rows_tiles(PAGED, p.n, p.Tq, p.G);
+  int64_t tiles = joins;
+  if (!PAGED && (int64_t)p.Tq * p.G / kRows + p.n + 2 < tiles) tiles = (int64_t)p.Tq * p.G / kRows + p.n + 2;
   const int64_t grid = (tiles + (p.split ? p.want : 0)) * p.Hk;
   GW_CHECK_ARG(grid < (1ll << 31), "grid of %lld workgroups is too large", (long long)grid);
   hipLaunchKernelGGL((rows_attn_kernel<E, D, PAGED>), dim3((uint32_t)grid), dim3(256), 0, stream, p);
   GW_HIP_LAUNCH_CHECK("rows attention");
   if (p.split) {
     const int64_t rows = (int64_t)p.Tq * p.G;
-    hipLaunchKernelGGL((rows_join_kernel<E, D, PAGED>), dim3((uint32_t)(tiles * p.Hk), (uint32_t)(rows < kRows ? rows : kRows)),
+    hipLaunchKernelGGL((rows_join_kernel<E, D, PAGED>), dim3((uint32_t)(joins * p.Hk), (uint32_t)(rows < kRows ? rows : kRows)),
                        dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("rows attention (join)");
   }
@@ -554,6 +567,7 @@ int rows_attn(int dtype, int D, bool paged, RowsParams p, void* workspace, hipSt
   if (p.split) {
     p.part = static_cast<float*>(workspace);
     p.part_lse = p.part + (int64_t)2 * p.want * p.Hk * kRows * D;
+    p.cut = reinterpret_cast<int2*>(p.part_lse + (int64_t)2 * p.want * p.Hk * kRows);
   }
   return dtype == GW_DTYPE_BF16 ? rows_dim<BF16>(D, paged, p, stream) : rows_dim<FP16>(D, paged, p, stream);
 }
@@ -568,7 +582,7 @@ static bool paged_split(int64_t B, int64_t N, int64_t Hq, int64_t Hk) {
 extern "C" size_t gw_paged_attn_fwd_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D) {
   using namespace gw;
   if (B < 1 || N < 1 || Hk < 1 || Hq < Hk || D < 1 || !paged_split(B, N, Hq, Hk)) return 0;
-  return rows_workspace(Hk, D);
+  return rows_workspace(rows_tiles(true, B, N, Hq / Hk), Hk, D);
 }
 
 extern "C" int gw_paged_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k,

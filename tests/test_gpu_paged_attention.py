@@ -109,6 +109,7 @@ def test_what_a_new_token_does_not_see(gpu_device, d, hk, value, n):
     """inf and NaN in the newest tokens' keys and values reach the tokens that see them and no other."""
     q, k, v, table, lens = make([n, 20], 6, 4, hk, d, 16, torch.float16, 8)
     clean, lse = run((q, k, v, table, lens), gpu_device)
+    ref = paged_attention(q, k, v, table, lens)
     j = n - 3  # seen by new tokens 3, 4 and 5
     page, slot = int(table[0, j // 16]), j % 16
     v[page, slot, :, 7] = value
@@ -118,8 +119,10 @@ def test_what_a_new_token_does_not_see(gpu_device, d, hk, value, n):
     got = o[0, 3:, :, 7]
     assert (got == value).all() if value == value else got.isnan().all()
     k[page, slot] = value
+    # the rows of a tile raise their running reference together: within the bounds, not the same bits
     o, lse2 = run((q, k, v, table, lens), gpu_device)
-    assert torch.equal(clean[0, :3], o[0, :3]) and torch.equal(lse[0, :3], lse2[0, :3])
+    check(o[:1, :3], lse2[:1, :3], tuple(t[:1, :3] for t in ref), torch.float16, d)
+    check(o[1:], lse2[1:], tuple(t[1:] for t in ref), torch.float16, d)
 
 
 def test_lengths_outside_the_table(gpu_device):
