@@ -13,9 +13,12 @@
 //
 // Bound by memory: each element is read and written once. A workgroup takes TT tokens x all
 // heads of q and k; a thread keeps one pair group (V pairs: V elements of the first half and V of
-// the second) and walks over (token, head) rows, four rows' loads in flight, the first of them
-// issued before the angles are formed. V is the widest of 8, 4, 2, 1 elements that divides every
-// half block and every stride.
+// the second) and walks over (token, head) rows, two rows' loads in flight, the first of them issued
+// before the angles are formed (the angles cost 1 to 2 us of a pass: left out, 48 views took 159 us
+// for 161). Eight tokens and two rows in flight: 65,952 tokens x 20 heads of 128 in bf16 139 us
+// (4.9 TB/s, what a large copy reaches), 16 tokens and four rows 161, four tokens and one row 135;
+// 9,973 tokens x 24 heads of 80 in fp32 53, 70 and 61 us. V is the widest of 8, 4, 2, 1 elements that
+// divides every half block and every stride.
 #include <math.h>
 #include <string.h>
 
@@ -27,8 +30,8 @@ namespace {
 constexpr int kRotMaxAxes = 8;
 constexpr int kRotMaxPairs = 128;  // D <= 256
 constexpr int kRotThreads = 256;
-constexpr int kRotMaxTokens = 16;  // tokens of a workgroup: at most 16 KB of sines and cosines
-constexpr int kRotUnroll = 4;
+constexpr int kRotMaxTokens = 8;  // tokens of a workgroup
+constexpr int kRotUnroll = 2;     // rows of a thread whose loads are in flight together
 
 struct RotTensor {
   const void* x;
@@ -42,7 +45,7 @@ struct RotParams {
   const void* pos;
   int64_t pb, pt, pa;
   int pos_type;
-  int B, T, TT;
+  int B, T, TT, D;
   int pairs;   // rotated pairs
   int groups;  // pair groups of a head, the copied tail's included
   double sign;
@@ -50,6 +53,8 @@ struct RotParams {
   uint8_t axis[kRotMaxPairs];
   // Start of the group's first half, distance to its second, first pair (>= pairs: copied)
   int16_t lo[kRotMaxPairs], half[kRotMaxPairs], pair[kRotMaxPairs];
+  // Per dim (staged form): its pair (-1: copied), distance to its partner
+  int16_t dim_pair[2 * kRotMaxPairs], dim_other[2 * kRotMaxPairs];
 };
 
 template <int BYTES>
@@ -99,6 +104,15 @@ __device__ __forceinline__ float2 rot_cos_sin(double turns, double sign) {
   return make_float2((float)cc, (float)(sign * ss));
 }
 
+// Cosines and sines of nt tokens' pairs into LDS.
+__device__ __forceinline__ void rot_angles(const RotParams& p, int b, int t0, int nt, float2* cs) {
+  for (int i = threadIdx.x; i < nt * p.pairs; i += kRotThreads) {
+    const int tk = i / p.pairs, pr = i - tk * p.pairs;
+    const double pos = rot_position(p.pos, p.pos_type, b * p.pb + (int64_t)(t0 + tk) * p.pt + p.axis[pr] * p.pa);
+    cs[tk * p.pairs + pr] = rot_cos_sin(pos * p.freq[pr], p.sign);
+  }
+}
+
 template <typename E, int V>
 __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(const RotParams p) {
   __shared__ float2 cs[kRotMaxTokens * kRotMaxPairs];
@@ -142,11 +156,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(const RotParam
 #pragma unroll
   for (int u = 0; u < kRotUnroll; ++u) load(u);
 
-  for (int i = threadIdx.x; i < nt * p.pairs; i += kRotThreads) {
-    const int tk = i / p.pairs, pr = i - tk * p.pairs;
-    const double pos = rot_position(p.pos, p.pos_type, b * p.pb + (int64_t)(t0 + tk) * p.pt + p.axis[pr] * p.pa);
-    cs[tk * p.pairs + pr] = rot_cos_sin(pos * p.freq[pr], p.sign);
-  }
+  rot_angles(p, b, t0, nt, cs);
   __syncthreads();
 
   while (true) {
@@ -179,6 +189,103 @@ __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(const RotParam
   }
 }
 
+// ---------------------------------------------------------------------------------------
+// Blocks whose halves are not whole 16-byte (8-byte for the 16-bit types) groups: a wave reads whole
+// rows 16 bytes at a time, keeps them in its own LDS rows, and each thread fetches the partners of its
+// elements from there, wherever they lie. No barrier: a wave's LDS accesses are in order. 9,973 tokens x
+// 24 heads of 80 in fp32 by blocks of 18, 14, 20, 20 (four rows in flight): 70 us, with pairs of single
+// elements 78.
+// ---------------------------------------------------------------------------------------
+template <typename E>
+__global__ __launch_bounds__(kRotThreads) void rotary_staged_kernel(const RotParams p) {
+  constexpr int V = 16 / ElemBytes<E>::value;
+  typedef typename RotRaw<ElemBytes<E>::value>::type Elem;
+  __shared__ float2 cs[kRotMaxTokens * kRotMaxPairs];
+  __shared__ __align__(16) uint8_t rows_s[kRotThreads / 64][kRotUnroll * 64 * 16];
+  const int b = blockIdx.y, t0 = blockIdx.x * p.TT;
+  const int nt = min(p.TT, p.T - t0);
+  const int H0 = p.t[0].H, HT = H0 + p.t[1].H;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int C = p.D / V;       // 16-byte chunks of a row, at most 64
+  const int RW = 64 / C;       // rows of a wave's load
+  const int r0 = lane / C, c = lane - r0 * C;
+  const bool on = r0 < RW;
+  const int rows = nt * HT;
+  const int R = RW * (kRotThreads / 64);
+  const int step_t = R / HT, step_h = R - step_t * HT;
+
+  // This thread's elements: where the partner lies in the row, the pair, and the sign of the partner's term.
+  int16_t partner[V], pair[V];
+  uint32_t minus = 0u;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int d = min(c * V + i, p.D - 1);
+    const int pr = p.dim_pair[d];
+    pair[i] = (int16_t)pr;
+    partner[i] = (int16_t)(pr < 0 ? d : d + p.dim_other[d]);
+    if (pr >= 0 && p.dim_other[d] > 0) minus |= 1u << i;
+  }
+
+  int row = wave * RW + r0, tok = row / HT, head = row - tok * HT;
+  uint4 x[kRotUnroll];
+  int at_tok[kRotUnroll], at_head[kRotUnroll];
+  auto load = [&](int u) __attribute__((always_inline)) {
+    at_tok[u] = on && row < rows ? tok : -1;
+    at_head[u] = head;
+    if (at_tok[u] >= 0) {
+      const bool first = head < H0;
+      const RotTensor& t = first ? p.t[0] : p.t[1];
+      x[u] = *reinterpret_cast<const uint4*>(static_cast<const Elem*>(t.x) + b * t.xb + (int64_t)(t0 + tok) * t.xt +
+                                             (int64_t)(head - (first ? 0 : H0)) * t.xh + c * V);
+    }
+    row += R;
+    tok += step_t;
+    head += step_h;
+    if (head >= HT) {
+      head -= HT;
+      ++tok;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kRotUnroll; ++u) load(u);
+  rot_angles(p, b, t0, nt, cs);
+  __syncthreads();
+
+  const int turns = (rows + R * kRotUnroll - 1) / (R * kRotUnroll);  // the same for every thread
+  for (int n = 0; n < turns; ++n) {
+    uint4 y[kRotUnroll];
+    uint8_t* const mine = rows_s[wave];
+#pragma unroll
+    for (int u = 0; u < kRotUnroll; ++u)
+      if (on) *reinterpret_cast<uint4*>(mine + (u * RW * C + lane) * 16) = x[u];
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < kRotUnroll; ++u) {
+      if (at_tok[u] < 0) continue;
+      const Elem* src = reinterpret_cast<const Elem*>(mine + (u * RW * C + r0 * C) * 16);
+      const float2* tc = cs + at_tok[u] * p.pairs;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float a = ld_f32(E{}, &x[u], i), o = ld_f32(E{}, src, partner[i]);
+        const float2 k = tc[max((int)pair[i], 0)];
+        const float term = o * k.y;
+        const float r = a * k.x + ((minus >> i) & 1u ? -term : term);
+        st_f32(E{}, &y[u], i, r);
+        if (pair[i] < 0) reinterpret_cast<Elem*>(&y[u])[i] = reinterpret_cast<const Elem*>(&x[u])[i];
+      }
+      const bool first = at_head[u] < H0;
+      const RotTensor& t = first ? p.t[0] : p.t[1];
+      *reinterpret_cast<uint4*>(static_cast<Elem*>(t.y) + b * t.yb + (int64_t)(t0 + at_tok[u]) * t.yt +
+                                (int64_t)(at_head[u] - (first ? 0 : H0)) * t.yh + c * V) = y[u];
+    }
+    asm volatile("" ::: "memory");
+    if (n + 1 < turns) {
+#pragma unroll
+      for (int u = 0; u < kRotUnroll; ++u) load(u);
+    }
+  }
+}
+
 // The angles' factors of the calling thread's last axes (64 powers cost more host time than the rest of a
 // call; a layer stack turns by the same axes throughout).
 struct RotFreqs {
@@ -204,8 +311,13 @@ const double* rot_freqs(int n_axes, const int32_t* dims, const double* bases) {
 }
 
 template <typename E>
-int rot_launch(const RotParams& p, int V, hipStream_t stream) {
+int rot_launch(const RotParams& p, int V, bool staged, hipStream_t stream) {
   const dim3 grid((p.T + p.TT - 1) / p.TT, p.B);
+  if (staged) {
+    hipLaunchKernelGGL(rotary_staged_kernel<E>, grid, dim3(kRotThreads), 0, stream, p);
+    GW_HIP_LAUNCH_CHECK("gw_rotary_axes");
+    return GW_OK;
+  }
   switch (V) {
     case 8:
       if constexpr (ElemBytes<E>::value == 2) {
@@ -277,7 +389,16 @@ extern "C" int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strid
     }
     return true;
   };
+  const int wide = V;
   while (V > 1 && !fits(V)) V >>= 1;
+  // Whole rows 16 bytes at a time, whatever the blocks are?
+  bool staged = V < 4 && D % wide == 0 && D / wide <= 64;
+  for (const RotTensor& t : in) {
+    if (t.H == 0) continue;
+    const int64_t all[6] = {t.xb, t.xt, t.xh, t.yb, t.yt, t.yh};
+    for (int64_t x : all) staged = staged && x % wide == 0;
+    staged = staged && aligned16(t.x) && aligned16(t.y);
+  }
   GW_CHECK_ARG(fits(V), "a tensor is not aligned to its element type");
 
   int dim = 0, pair = 0, group = 0;
@@ -288,6 +409,10 @@ extern "C" int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strid
       p.lo[group] = (int16_t)(dim + i);
       p.half[group] = (int16_t)half;
       p.pair[group] = (int16_t)(a < n_axes ? pair + i : kRotMaxPairs);
+    }
+    for (int i = 0; i < n; ++i) {
+      p.dim_pair[dim + i] = (int16_t)(a < n_axes ? pair + (i < half ? i : i - half) : -1);
+      p.dim_other[dim + i] = (int16_t)(i < half ? half : -half);
     }
     if (a < n_axes) {
       for (int i = 0; i < half; ++i) p.axis[pair + i] = (uint8_t)a;
@@ -305,14 +430,15 @@ extern "C" int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strid
   p.pa = pos_strides[2];
   p.B = (int)B;
   p.T = (int)T;
+  p.D = (int)D;
   p.sign = inverse ? -1.0 : 1.0;
   // Few tokens a workgroup until the chip has four workgroups per CU, then up to 16.
   p.TT = kRotMaxTokens;
   while (p.TT > 1 && B * ((T + p.TT - 1) / p.TT) < 1024) p.TT >>= 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case GW_DTYPE_BF16: return rot_launch<BF16>(p, V, s);
-    case GW_DTYPE_FP16: return rot_launch<FP16>(p, V, s);
-    default: return rot_launch<FP32>(p, V, s);
+    case GW_DTYPE_BF16: return rot_launch<BF16>(p, V, staged, s);
+    case GW_DTYPE_FP16: return rot_launch<FP16>(p, V, staged, s);
+    default: return rot_launch<FP32>(p, V, staged, s);
   }
 }
