@@ -70,10 +70,36 @@ __global__ __launch_bounds__(256) void packed_bwd_clear_kernel(uint32_t* a, int6
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) a[i] = 0u;
 }
 
-// stats of 256 / (D / 8) rows at a time: D / 8 lanes per (token, head) row. MAXIMA: also the
+// Statistics of 256 / (D / 8) rows at a time: D / 8 lanes per (token, head) row. MAXIMA: also the
 // sequences' largest row norms (the maximum does not depend on the order of the atomics; rows that
-// are not finite have no part in it, their gradients are not finite whatever the scale).
+// are not finite have no part in it, their gradients are not finite whatever the scale): the largest of
+// the workgroup's rows per key head in LDS, then one atomic where that raises the value (an atomic per
+// row took 1.6 ms for 22,953 tokens x 16 heads).
 constexpr int kStatTokens = 16;
+constexpr int kStatHeads = 128;  // key heads with an LDS word; further ones go to memory at once
+
+struct PkMaxima {
+  uint32_t* lds;
+  uint32_t* out;  // of the sequence
+  int Hk;
+  __device__ __forceinline__ void init() {
+    for (int i = threadIdx.x; i < min(Hk, kStatHeads); i += 256) lds[i] = 0u;
+    __syncthreads();
+  }
+  __device__ __forceinline__ void row(int head, float norm2) {
+    if (!(norm2 < INFINITY)) return;
+    const uint32_t x = __float_as_uint(sqrtf(norm2));
+    if (head < kStatHeads)
+      atomicMax(lds + head, x);
+    else
+      atomicMax(out + head, x);
+  }
+  __device__ __forceinline__ void finish() {
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(Hk, kStatHeads); i += 256)
+      if (lds[i] > __atomic_load_n(out + i, __ATOMIC_RELAXED)) atomicMax(out + i, lds[i]);
+  }
+};
 
 template <typename E, int D, bool MAXIMA>
 __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdParams p) {
@@ -83,6 +109,9 @@ __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdPa
   if (t0 >= pt.len) return;
   const int rows = min(kStatTokens, pt.len - t0) * p.H;
   const int li = threadIdx.x % LPR;
+  __shared__ uint32_t top[kStatHeads];
+  PkMaxima maxima = {top, p.max_do + (int64_t)pt.seq * p.Hk, p.Hk};
+  if (MAXIMA) maxima.init();
   for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
     const int t = pt.start + t0 + r / p.H, h = r % p.H;
     float a[8], b[8], c[8];
@@ -102,9 +131,10 @@ __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdPa
       const int64_t at = (int64_t)h * p.Tq + t;
       p.nlse[at] = l == -INFINITY ? -INFINITY : (kPScale<E> - l * kDLog2e) / p.scale_log2;
       p.ndelta[at] = -s;
-      if (MAXIMA && nn < INFINITY) atomicMax(p.max_do + (int64_t)pt.seq * p.Hk + h / p.G, __float_as_uint(sqrtf(nn)));
+      if (MAXIMA) maxima.row(h / p.G, nn);
     }
   }
+  if (MAXIMA) maxima.finish();
 }
 
 template <typename E, int D>
@@ -115,6 +145,9 @@ __global__ __launch_bounds__(256) void packed_bwd_vmax_kernel(const PackedBwdPar
   if (t0 >= pt.len) return;
   const int rows = min(kStatTokens, pt.len - t0) * p.Hk;
   const int li = threadIdx.x % LPR;
+  __shared__ uint32_t top[kStatHeads];
+  PkMaxima maxima = {top, p.max_v + (int64_t)pt.seq * p.Hk, p.Hk};
+  maxima.init();
   for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
     const int t = pt.start + t0 + r / p.Hk, h = r % p.Hk;
     float a[8], nn = 0.f;
@@ -122,8 +155,9 @@ __global__ __launch_bounds__(256) void packed_bwd_vmax_kernel(const PackedBwdPar
 #pragma unroll
     for (int i = 0; i < 8; ++i) nn = fmaf(a[i], a[i], nn);
     nn = group_sum<LPR>(nn);
-    if (li == 0 && nn < INFINITY) atomicMax(p.max_v + (int64_t)pt.seq * p.Hk + h, __float_as_uint(sqrtf(nn)));
+    if (li == 0) maxima.row(h, nn);
   }
+  maxima.finish();
 }
 
 // The same column in fp32.
@@ -407,10 +441,30 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
       dp[4 * g + 2] = y.z;
       dp[4 * g + 3] = y.w;
     }
+    // Operands of the products in the order of their use, read PRE products ahead; the scheduling barriers
+    // keep the compiler from reading them all at once, for which there are no registers (D = 64: 759 us for
+    // 794 on 6 scenes of 2 to 8 views).
+    constexpr int PRE = D == 64 ? 2 : 4;
+    auto row = [&](int i) __attribute__((always_inline)) { return i < KS ? at.row(qt, st, i) : at.row(gt, st, i - KS); };
+    // Columns for each 16 queries and 32 dims: of dO, then of Q.
+    auto column = [&](int i) __attribute__((always_inline)) {
+      return at.col(i % 2 ? qt : gt, st, i / 2 / DB, i / 2 % DB);
+    };
+    uint4 a[PRE], c[PRE];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mma(E{}, at.row(qt, st, ks), kb[ks], s);
+    for (int i = 0; i < PRE; ++i) a[i] = row(i);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) dp = mma(E{}, at.row(gt, st, ks), vb[ks], dp);
+    for (int i = 0; i < 2 * KS; ++i) {
+      if (i < KS)
+        s = mma(E{}, a[i % PRE], kb[i % KS], s);
+      else
+        dp = mma(E{}, a[i % PRE], vb[i % KS], dp);
+      if (i + PRE < 2 * KS)
+        a[i % PRE] = row(i + PRE);
+      else
+        c[i + PRE - 2 * KS] = column(i + PRE - 2 * KS);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     float w[16], ds[16];
 #pragma unroll
     for (int x = 0; x < 16; ++x) w[x] = fexp2(s[x] * sl2);
@@ -425,24 +479,22 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
         ds[x] = 8 * (x / 4) + x % 4 >= need_ds ? ds[x] : 0.f;
       }
     }
+    const uint4 pb[2] = {pack_quad<E>(w), pack_quad<E>(w + 8)}, sb[2] = {pack_quad<E>(ds), pack_quad<E>(ds + 8)};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const uint4 pb = pack_quad<E>(w + 8 * ks), sb = pack_quad<E>(ds + 8 * ks);
-      uint4 gc[DB], qc[DB];
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        gc[db] = at.col(gt, st, ks, db);
-        qc[db] = at.col(qt, st, ks, db);
-      }
+    for (int i = 0; i < 4 * DB; ++i) {
+      const int ks = i / 2 / DB, db = i / 2 % DB;
+      uint4 q[1] = {c[i % PRE]};
       if constexpr (decltype(masked)::value) {
-        unclean |= pk_clear_not_finite<E>(gc);
-        pk_clear_not_finite<E>(qc);  // keys that such a query sees have a NaN dS
+        const bool any = pk_clear_not_finite<E>(q);
+        if (i % 2 == 0) unclean |= any;  // keys that see a query whose q is not finite have a NaN dS
       }
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        av[db] = mma(E{}, gc[db], pb, av[db]);
-        ak[db] = mma(E{}, qc[db], sb, ak[db]);
-      }
+      if (i % 2 == 0)
+        av[db] = mma(E{}, q[0], pb[ks], av[db]);
+      else
+        ak[db] = mma(E{}, q[0], sb[ks], ak[db]);
+      if (i + PRE < 4 * DB) c[i % PRE] = column(i + PRE);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
