@@ -242,6 +242,11 @@ def strides2(x0: int, x1: int):
     return _I64x2(x0, x1)
 
 
+def row_strides(x: torch.Tensor):
+    """Strides of all dims but the last, 0 for those of one entry (torch leaves them whatever they were)."""
+    return [st if n != 1 else 0 for n, st in zip(x.shape[:-1], x.stride())]
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

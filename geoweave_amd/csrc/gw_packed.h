@@ -130,16 +130,17 @@ struct PkInt {
   static constexpr int value = V;
 };
 
-// A descriptor of `bytes` bytes at a wave-uniform base: loads past them give zeros.
+// A descriptor of `bytes` bytes at a wave-uniform base: loads past them, and at kPkNowhere, give zeros.
+constexpr uint32_t kPkNowhere = 0xFFFF8000u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t pk_rsrc(const char* base, int64_t bytes) {
-  const uint32_t n = (uint32_t)min(max(bytes, (int64_t)0), (int64_t)0xFFFFFFFF);
+  const uint32_t n = (uint32_t)min(max(bytes, (int64_t)0), (int64_t)0xFFFF0000);
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(uniform_ptr(base)), (short)0,
                                            (int)__builtin_amdgcn_readfirstlane(n), 0x00020000);
 }
 
 // Row tiles of one head of one sequence: 64 rows at a time from memory straight to LDS. Lane i of a
 // wave writes 16 bytes at the wave's segment + 16 i, so it reads the chunk that the swizzle keeps there.
-// Rows past the sequence's end arrive as zeros.
+// Rows past the sequence's end arrive as zeros, whatever the strides (a broadcast row has stride 0).
 template <int D, int THREADS>
 struct PkRows {
   static constexpr int kRowBytes = 2 * D;
@@ -148,15 +149,19 @@ struct PkRows {
   static constexpr int kPasses = 64 / kRowsPerPass;
   const char* base;
   int64_t bytes;       // from base to the end of the last row
+  int rows;
+  int row;             // this lane's row in pass 0
   uint32_t stride;     // bytes
   uint32_t off;        // this lane's offset in pass 0
   uint32_t seg;        // this wave's segment of the tile in pass 0
 
-  __device__ __forceinline__ void init(const void* p, int64_t stride_elems, int rows, int tid) {
+  __device__ __forceinline__ void init(const void* p, int64_t stride_elems, int n, int tid) {
     base = uniform_ptr(static_cast<const char*>(p));
+    rows = n;
     stride = (uint32_t)stride_elems * 2u;
     bytes = rows > 0 ? (int64_t)(rows - 1) * stride + kRowBytes : 0;
-    const int row = tid / kChunks, c = tid % kChunks;
+    row = tid / kChunks;
+    const int c = tid % kChunks;
     static_assert(kRowsPerPass % 16 == 0, "the swizzle repeats every 16 rows");
     off = (uint32_t)row * stride + (uint32_t)((c ^ pk_swz<D>(row)) * 16);
     seg = (uint32_t)(tid >> 6) * 1024u;
@@ -169,7 +174,7 @@ struct PkRows {
     for (int i = 0; i < kPasses; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rs, (__attribute__((address_space(3))) void*)(lds + seg + i * kRowsPerPass * kRowBytes), 16,
-          (int)(off + (uint32_t)(i * kRowsPerPass) * stride), 0, 0, 0);
+          (int)(64 * n + row + i * kRowsPerPass < rows ? off + (uint32_t)(i * kRowsPerPass) * stride : kPkNowhere), 0, 0, 0);
   }
 };
 

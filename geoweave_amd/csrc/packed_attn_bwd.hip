@@ -472,11 +472,15 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
     for (int x = 0; x < 16; ++x) ds[x] = kFp16 ? w[x] * dscale * dp[x] : w[x] * dp[x];
     if constexpr (decltype(masked)::value) {
       const int need = key - shift - i0 - 4 * half;
-      const int need_ds = max(key, 1) - shift - i0 - 4 * half;  // the first key's one-key row has dS = 0
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        w[x] = 8 * (x / 4) + x % 4 >= need ? w[x] : 0.f;
-        ds[x] = 8 * (x / 4) + x % 4 >= need_ds ? ds[x] : 0.f;
+        const bool sees = 8 * (x / 4) + x % 4 >= need;
+        w[x] = sees ? w[x] : 0.f;
+        ds[x] = sees ? ds[x] : 0.f;
+      }
+      if (wkey == 0 && i0 <= -shift && -shift < i0 + 32) {  // the row that sees the first key only has dS = 0
+#pragma unroll
+        for (int x = 0; x < 16; ++x) ds[x] = 8 * (x / 4) + x % 4 + 4 * half == -shift - i0 ? 0.f : ds[x];
       }
     }
     const uint4 pb[2] = {pack_quad<E>(w), pack_quad<E>(w + 8)}, sb[2] = {pack_quad<E>(ds), pack_quad<E>(ds + 8)};

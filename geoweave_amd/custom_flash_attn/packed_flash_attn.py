@@ -84,16 +84,16 @@ def _check_inputs(q, k, v, cu_q, cu_k, softmax_scale):
 
 
 def _prep(x: torch.Tensor) -> torch.Tensor:
-    # 16-byte rows, and a token stride within the kernels' offsets.
-    st, sh, sd = x.stride()
-    if sd != 1 or st % 8 or sh % 8 or not 0 <= st < MAX_ROW_STRIDE or x.data_ptr() % 16:
-        x = x.contiguous()
+    # 16-byte rows, and a token stride within the kernels' offsets; a copy where they are not (clone: a
+    # contiguous tensor may start anywhere).
+    st, sh = _lib.row_strides(x)
+    if x.stride(2) != 1 or st % 8 or sh % 8 or st >= MAX_ROW_STRIDE or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
 def _rows(x: torch.Tensor):
-    st, sh, _ = x.stride()
-    return x.data_ptr(), _lib.strides2(st, sh)
+    return x.data_ptr(), _lib.strides2(*_lib.row_strides(x))
 
 
 def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool, want_rest: bool = False):

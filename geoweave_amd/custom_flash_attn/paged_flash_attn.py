@@ -55,7 +55,7 @@ def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale
         raise ValueError("q, the caches, block_table and cache_seqlens must be tensors of one GPU")
     for c in (k_cache, v_cache):
         # Copying a cache to align it would cost more than the call: the caller lays it out.
-        if c.numel() and (c.stride(-1) != 1 or any(s % 8 for s in c.stride()[:-1]) or c.data_ptr() % 16):
+        if c.numel() and (c.stride(-1) != 1 or any(s % 8 for s in _lib.row_strides(c)) or c.data_ptr() % 16):
             raise ValueError("caches need a unit last stride and 16-byte aligned rows")
     return scale
 
@@ -66,8 +66,8 @@ def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_ca
                                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(o in q's shape and dtype, lse fp32 ``q.shape[:-1]`` where asked for); see the module docstring."""
     scale = _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale)
-    if q.stride(-1) != 1 or any(s % 8 for s in q.stride()[:-1]) or q.data_ptr() % 16:
-        q = q.contiguous()
+    if q.stride(-1) != 1 or any(s % 8 for s in _lib.row_strides(q)) or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)  # a contiguous tensor may start anywhere
     if block_table.stride(-1) != 1:
         block_table = block_table.contiguous()
     cache_seqlens = cache_seqlens.contiguous()
@@ -84,10 +84,10 @@ def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_ca
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
     with _lib.on_device(dev):
         rc = lib.gw_paged_attn_fwd(
-            _lib.dtype_code(q.dtype), q4.data_ptr(), _lib.strides3(*q4.stride()[:3]), k_cache.data_ptr(),
-            _lib.strides3(*k_cache.stride()[:3]), v_cache.data_ptr(), _lib.strides3(*v_cache.stride()[:3]),
+            _lib.dtype_code(q.dtype), q4.data_ptr(), _lib.strides3(*_lib.row_strides(q4)), k_cache.data_ptr(),
+            _lib.strides3(*_lib.row_strides(k_cache)), v_cache.data_ptr(), _lib.strides3(*_lib.row_strides(v_cache)),
             block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), o4.data_ptr(),
-            _lib.strides3(*o4.stride()[:3]), _lib.ptr(lse), b, n, hq, hk, d, pages, page, block_table.shape[1],
+            _lib.strides3(*_lib.row_strides(o4)), _lib.ptr(lse), b, n, hq, hk, d, pages, page, block_table.shape[1],
             int(causal), scale, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
     _lib.check(rc, "gw_paged_attn_fwd")
     return o, lse

@@ -234,6 +234,59 @@ def test_strides_layouts_and_broadcast_heads(gpu_device):
     torch.testing.assert_close(g1.float(), g2.float(), atol=0.1, rtol=0.05)  # sums of four rounded terms each
 
 
+def test_broadcast_tokens(gpu_device):
+    """Tensors whose tokens are one row of memory, forward and backward."""
+    dev, t = gpu_device, 150
+    cu = torch.tensor([0, 70, 150], dtype=torch.int32, device=dev)
+    base = [torch.randn(1, 2, 64, device=dev, dtype=torch.bfloat16) for _ in range(4)]
+    full = [torch.randn(t, 2, 64, device=dev, dtype=torch.bfloat16) for _ in range(4)]
+    for i in range(4):  # q, k, v or dO broadcast
+        wide = [x.expand(t, 2, 64) if j == i else full[j] for j, x in enumerate(base)]
+        outs = []
+        for args in (wide, [x.contiguous() for x in wide]):
+            leaves = [x.detach().requires_grad_() for x in args[:3]]
+            o = packed_flash_attn_func(*leaves, cu, None, True)
+            outs.append((o, *torch.autograd.grad(o, leaves, args[3])))
+        assert all(torch.equal(a, b) for a, b in zip(*outs)), i
+
+
+def test_single_tokens_and_tensors_that_start_anywhere(gpu_device):
+    """Dims of one entry keep whatever stride they had, and a contiguous tensor may start at any element."""
+    dev = gpu_device
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    y = torch.randn(128, device=dev, dtype=torch.bfloat16)
+    one = y.as_strided((1, 2, 64), (5, 64, 1))
+    assert one.stride(0) % 8 and one.is_contiguous()
+    o, _ = packed_flash_attn_inference_func(one, one, one, cu)
+    assert torch.equal(o, one)
+    flat = torch.randn(3 + 40 * 2 * 64, device=dev, dtype=torch.bfloat16)
+    off = flat[3:].view(40, 2, 64)
+    cu = torch.tensor([0, 11, 40], dtype=torch.int32, device=dev)
+    want, _ = packed_flash_attn_inference_func(off.clone(), off.clone(), off.clone(), cu, causal=True)
+    got, _ = packed_flash_attn_inference_func(off, off, off, cu, causal=True)
+    assert torch.equal(want, got)
+    leaf = off.detach().requires_grad_()
+    out = packed_flash_attn_func(leaf, leaf, leaf, cu)
+    (g1,) = torch.autograd.grad(out.sum(), leaf)  # a gradient without strides
+    leaf2 = off.clone().requires_grad_()
+    (g2,) = torch.autograd.grad(packed_flash_attn_func(leaf2, leaf2, leaf2, cu).sum(), leaf2)
+    assert torch.equal(g1, g2)
+
+
+def test_no_sequences_and_no_tokens(gpu_device):
+    dev = gpu_device
+    for tq, tk, bounds in ((5, 1000, [0]), (300, 7, [0]), (40, 900, [0, 0, 0]), (0, 9, [0, 0]), (6, 0, [0, 0])):
+        q = torch.full((tq, 2, 64), float("nan"), device=dev, dtype=torch.bfloat16).requires_grad_()
+        k = torch.full((tk, 1, 64), float("nan"), device=dev, dtype=torch.bfloat16).requires_grad_()
+        cu = torch.tensor(bounds, dtype=torch.int32, device=dev)
+        o = packed_flash_attn_func(q, k, k, cu, cu)
+        assert o.shape == q.shape and (o == 0).all()
+        _, lse = packed_flash_attn_inference_func(q, k, k, cu, cu, return_lse=True)
+        assert (lse == -math.inf).all()
+        gq, gk = torch.autograd.grad(o, [q, k], torch.ones_like(o))
+        assert (gq == 0).all() and (gk == 0).all()
+
+
 def test_offsets_past_32_bits(gpu_device):
     """Key rows 2^20 elements apart: the last lie more than 2^32 bytes behind the first."""
     dev, n, d = gpu_device, 2600, 64

@@ -148,6 +148,24 @@ def test_layouts(gpu_device):
     assert torch.equal(want, got)
 
 
+def test_single_entries_and_empty_pools(gpu_device):
+    dev = gpu_device
+    q, k, v, table, lens = (t.to(dev) for t in make([30], 1, 1, 1, 64, 32, torch.float16, 9, spare=0, width=0))
+    want, _ = paged_flash_attn_inference_func(q, k, v, table, lens)
+    y = torch.zeros(2, 67, device=dev, dtype=torch.float16)
+    y[1, 3:] = q.view(-1)
+    odd = y[1:, 3:].as_strided((1, 1, 1, 64), (67, 5, 3, 1), 67 + 3)  # one entry in all dims but the last
+    one = k.as_strided((1, 32, 1, 64), (7, 64, 9, 1))
+    got, _ = paged_flash_attn_inference_func(odd, one, v, table, lens)
+    assert torch.equal(want, got)
+    none = k[:0]
+    for tab in (table, table[:, :0]):
+        o, lse = paged_flash_attn_inference_func(q, none, none, tab, lens, return_lse=True)
+        assert (o == 0).all() and (lse == -math.inf).all()
+    e, _ = paged_flash_attn_inference_func(q[:0], k, v, table[:0], lens[:0])
+    assert e.shape == (0, 1, 1, 64)
+
+
 def test_offsets_past_32_bits(gpu_device):
     """Pages 2^26 elements apart: the last begins more than 2^32 bytes behind the first."""
     dev, pages, page, d = gpu_device, 40, 64, 64
