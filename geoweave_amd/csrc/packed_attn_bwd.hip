@@ -101,15 +101,42 @@ struct PkMaxima {
   }
 };
 
-template <typename E, int D, bool MAXIMA>
-__global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdParams p) {
+template <typename E, int D>
+__device__ __forceinline__ void pk_largest_v(const PackedBwdParams& p, int slot, uint32_t* top) {
   constexpr int LPR = D / 8;
+  const PackedTile pt = pk_find_tile(p.cu_k, p.n, p.Tk, 1, kStatTokens, slot);
+  const int t0 = pt.tile * kStatTokens;
+  if (t0 >= pt.len) return;
+  const int rows = min(kStatTokens, pt.len - t0) * p.Hk;
+  const int li = threadIdx.x % LPR;
+  PkMaxima maxima = {top, p.max_v + (int64_t)pt.seq * p.Hk, p.Hk};
+  maxima.init();
+  for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
+    const int t = pt.start + t0 + r / p.Hk, h = r % p.Hk;
+    float a[8], nn = 0.f;
+    unpack8<E>(*reinterpret_cast<const uint4*>(p.v + (int64_t)t * p.vst + (int64_t)h * p.vsh + li * 8), a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nn = fmaf(a[i], a[i], nn);
+    nn = group_sum<LPR>(nn);
+    if (li == 0) maxima.row(h, nn);
+  }
+  maxima.finish();
+}
+
+// The first qslots workgroups take query rows, the others (MAXIMA) rows of V.
+template <typename E, int D, bool MAXIMA>
+__global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdParams p, int qslots) {
+  constexpr int LPR = D / 8;
+  __shared__ uint32_t top[kStatHeads];
+  if (MAXIMA && (int)blockIdx.x >= qslots) {
+    pk_largest_v<E, D>(p, blockIdx.x - qslots, top);
+    return;
+  }
   const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, 1, kStatTokens, blockIdx.x);
   const int t0 = pt.tile * kStatTokens;
   if (t0 >= pt.len) return;
   const int rows = min(kStatTokens, pt.len - t0) * p.H;
   const int li = threadIdx.x % LPR;
-  __shared__ uint32_t top[kStatHeads];
   PkMaxima maxima = {top, p.max_do + (int64_t)pt.seq * p.Hk, p.Hk};
   if (MAXIMA) maxima.init();
   for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
@@ -135,29 +162,6 @@ __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdPa
     }
   }
   if (MAXIMA) maxima.finish();
-}
-
-template <typename E, int D>
-__global__ __launch_bounds__(256) void packed_bwd_vmax_kernel(const PackedBwdParams p) {
-  constexpr int LPR = D / 8;
-  const PackedTile pt = pk_find_tile(p.cu_k, p.n, p.Tk, 1, kStatTokens, blockIdx.x);
-  const int t0 = pt.tile * kStatTokens;
-  if (t0 >= pt.len) return;
-  const int rows = min(kStatTokens, pt.len - t0) * p.Hk;
-  const int li = threadIdx.x % LPR;
-  __shared__ uint32_t top[kStatHeads];
-  PkMaxima maxima = {top, p.max_v + (int64_t)pt.seq * p.Hk, p.Hk};
-  maxima.init();
-  for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
-    const int t = pt.start + t0 + r / p.Hk, h = r % p.Hk;
-    float a[8], nn = 0.f;
-    unpack8<E>(*reinterpret_cast<const uint4*>(p.v + (int64_t)t * p.vst + (int64_t)h * p.vsh + li * 8), a);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) nn = fmaf(a[i], a[i], nn);
-    nn = group_sum<LPR>(nn);
-    if (li == 0) maxima.row(h, nn);
-  }
-  maxima.finish();
 }
 
 // The same column in fp32.
@@ -621,14 +625,10 @@ int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(packed_bwd_clear_kernel, dim3((uint32_t)((words + 255) / 256 > 1024 ? 1024 : (words + 255) / 256)),
                        dim3(256), 0, stream, p.max_do, words);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (clear)");
-    if (p.Tk > 0) {
-      hipLaunchKernelGGL((packed_bwd_vmax_kernel<E, D>), dim3((uint32_t)(p.Tk / kStatTokens + p.n + 2)), dim3(256), 0, stream, p);
-      GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (v)");
-    }
   }
   if (p.Tq > 0) {
-    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D, kFp16>), dim3((uint32_t)(p.Tq / kStatTokens + p.n + 2)), dim3(256), 0,
-                       stream, p);
+    const int stat_q = p.Tq / kStatTokens + p.n + 2, stat_k = kFp16 && p.Tk > 0 ? p.Tk / kStatTokens + p.n + 2 : 0;
+    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D, kFp16>), dim3((uint32_t)stat_q + stat_k), dim3(256), 0, stream, p, stat_q);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (rows)");
     hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)(qslots * p.Hk), p.split_dq), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq)");
