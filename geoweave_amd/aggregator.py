@@ -378,7 +378,7 @@ class Aggregator(nn.Module):
         V, C_in, H, W = images.shape
         if C_in != 3:
             raise ValueError(f"expected 3 input channels, got {C_in}")
-        if sum(views) != V or any(n < 1 for n in views):
+        if not views or sum(views) != V or any(n < 1 for n in views):
             raise ValueError(f"scenes of {views} views do not make up {V} images")
         dtype = self.frame_blocks[0].norm1.weight.dtype
         x = ((images - self._resnet_mean[0]) / self._resnet_std[0]).to(dtype)

@@ -14,8 +14,7 @@
 // Bound by memory: each element is read and written once. A workgroup takes TT tokens x all
 // heads of q and k; a thread keeps one pair group (V pairs: V elements of the first half and V of
 // the second) and walks over (token, head) rows, two rows' loads in flight, the first of them issued
-// before the angles are formed (the angles cost 1 to 2 us of a pass: left out, 48 views took 159 us
-// for 161). Eight tokens and two rows in flight: 65,952 tokens x 20 heads of 128 in bf16 139 us
+// before the angles are formed (the angles cost 1 to 2 us of a pass of 48 views). Eight tokens and two rows in flight: 65,952 tokens x 20 heads of 128 in bf16 139 us
 // (4.9 TB/s, what a large copy reaches), 16 tokens and four rows 161, four tokens and one row 135;
 // 9,973 tokens x 24 heads of 80 in fp32 53, 70 and 61 us. V is the widest of 8, 4, 2, 1 elements that
 // divides every half block and every stride.
@@ -432,7 +431,7 @@ extern "C" int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strid
   p.T = (int)T;
   p.D = (int)D;
   p.sign = inverse ? -1.0 : 1.0;
-  // Few tokens a workgroup until the chip has four workgroups per CU, then up to 16.
+  // Few tokens a workgroup until the chip has four workgroups per CU, then up to 8.
   p.TT = kRotMaxTokens;
   while (p.TT > 1 && B * ((T + p.TT - 1) / p.TT) < 1024) p.TT >>= 1;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -472,7 +472,9 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
   if (rr >= sq.lq * p.G || (!PAGED && sq.lq * p.G > kRowsMax)) return;
   const int2 where = p.cut[at_tile];
   const int parts = where.y;
-  if (parts == 1) return;
+  // One part, or (packed bounds out of order, which may name more rows than there are) a tile that no
+  // workgroup took and whose entry may hold anything.
+  if (parts <= 1 || parts > 2 * p.want || (uint32_t)where.x > (uint32_t)(2 * p.want - parts)) return;
   const int64_t step = (int64_t)p.Hk * kRows;
   const int64_t at = ((int64_t)where.x * p.Hk + hk) * kRows + row;
   // The largest log2 sum (NaN if one is).

@@ -136,7 +136,7 @@ def rotary_axes_func(x: torch.Tensor, positions: torch.Tensor, axis_dims: Sequen
     (``[T, A]`` or ``[B, T, A]``; int32, int64 or float32): axis ``a`` turns dims ``i`` and ``i + d/2``
     of its block of ``d = axis_dims[a]`` dims by ``positions[..., a] * bases[a] ** (-2 i / d)``. The
     blocks lie one behind the other; dims behind the last are copied. The result is contiguous.
-    Differentiable in ``x``."""
+    Differentiable in ``x`` (positions get no gradient)."""
     axis_dims, bases = _check(x, None, positions, axis_dims, bases)
     return RotaryAxesFunc.apply(positions, axis_dims, bases, x)[0]
 

@@ -361,6 +361,28 @@ def test_bounds_that_are_not_in_order_stay_in_the_tensors(gpu_device):
         assert o.shape == q.shape
 
 
+def test_bounds_out_of_order_over_few_rows(gpu_device):
+    """Bounds that run back name more tiles of few rows than the call has workgroups: every access stays in the
+    workspace."""
+    dev, t, n, h = gpu_device, 400, 900, 16
+    back = torch.tensor([0] + [17 * (i % 21) for i in range(n - 1)] + [t], dtype=torch.int32, device=dev)
+    q = torch.randn(t, h, 64, device=dev, dtype=torch.bfloat16)
+    k, v = (torch.randn(n * 512 + 600, 1, 64, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    cu_k = torch.arange(n + 1, dtype=torch.int32, device=dev) * 512
+    cu_k[-1] += 600
+    heads = [x.expand(-1, h, -1) for x in (k, v)]
+    for _ in range(2):
+        o, lse = packed_flash_attn_inference_func(q, *heads, back, cu_k, return_lse=True)
+        torch.cuda.synchronize(dev)
+        assert o.shape == q.shape and lse.shape == (t, h)
+    # in order again: the values of an ordinary call
+    ordered = torch.arange(n + 1, device=dev).clamp(max=t).to(torch.int32)
+    o, _ = packed_flash_attn_inference_func(q, *heads, ordered, cu_k)
+    for i in (0, h - 1):
+        ref = packed_attention(q[:, i:i + 1].cpu(), k.cpu(), v.cpu(), ordered.cpu(), cu_k.cpu(), False)
+        check(o[:, i:i + 1], ref, "o", torch.bfloat16, 64)
+
+
 def test_gradients_against_differences(gpu_device):
     """The directional derivative of sum(o w) by central differences of the 64-bit oracle."""
     args = make([20, 45], [33, 45], 4, 2, 64, torch.bfloat16, 8)
