@@ -85,6 +85,84 @@ __device__ __forceinline__ PackedTile pk_find_tile(const int32_t* cu, int n, int
   return r;
 }
 
+// Longest first. In the order of the slots the workgroups of a long sequence may start last, and the chip
+// waits for them. A list of the tiles by falling work (64-row tiles of the other side that a tile meets), in
+// classes of an eighth of a power of two, is formed by one workgroup; empty slots come last. Only when a
+// tile is computed depends on it, no result does.
+constexpr int kPkOrderMax = 4096;  // slots of a list; longer calls have rounds of workgroups enough
+constexpr int kPkClasses = 128;
+
+// KEYS: tiles of bm keys that meet queries; else tiles of bm rows (token, head of g) that meet keys, the causal
+// ones counted from the sequence's end. order: [slots]; count: LDS, kPkClasses + 1 words. A wave takes 64
+// sequences at a time.
+template <bool KEYS>
+__device__ __forceinline__ void pk_order(const int32_t* cu, int T, const int32_t* cu_other, int T_other, int n, int g,
+                                         int bm, int causal, int slots, int2* order, uint32_t* count) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto tiles = [&](auto&& take) {
+    auto one = [&](int seq, int len, int other, int ntile, int t) {
+      int work;
+      if (KEYS) {
+        work = ((other + 63) >> 6) - (causal ? max(0, t * bm - (len - other)) >> 6 : 0);
+      } else {
+        const int last = (min((ntile - t) * bm, len * g) - 1) / g;
+        work = ((causal ? min(last + other - len, other - 1) + 1 : other) + 63) >> 6;
+      }
+      take(seq, t, work > 0 ? max(0, kPkClasses - 2 - (int)(8.f * flog2((float)work))) : kPkClasses - 1);
+    };
+    for (int i0 = 64 * wave; i0 < n + 2; i0 += 256) {
+      const int i = i0 + lane;
+      int len = 0, other = 0;
+      if (i < n + 2) len = max(0, pk_bound(cu, n, T, i + 1) - pk_bound(cu, n, T, i));
+      if (i >= 1 && i <= n) other = max(0, pk_bound(cu_other, n, T_other, i + 1) - pk_bound(cu_other, n, T_other, i));
+      const int ntile = (len * g + bm - 1) / bm;
+      // Sequences of a few tiles: a sequence per lane. The longer ones one by one, a tile per lane.
+      const bool few = ntile <= 16;
+      for (int t = 0; t < 16 && __builtin_amdgcn_ballot_w64(few && t < ntile); ++t)
+        if (few && t < ntile) one(i, len, other, ntile, t);
+      for (uint64_t left = __builtin_amdgcn_ballot_w64(!few); left; left &= left - 1) {
+        const int l = __builtin_ctzll(left);
+        const int ln = __builtin_amdgcn_readlane(len, l), lo = __builtin_amdgcn_readlane(other, l);
+        const int nt = __builtin_amdgcn_readlane(ntile, l);
+        for (int t = lane; t < nt; t += 64) one(i0 + l, ln, lo, nt, t);
+      }
+    }
+  };
+  if (tid < kPkClasses) count[tid] = 0u;
+  __syncthreads();
+  tiles([&](int, int, int cls) { atomicAdd(count + cls, 1u); });
+  __syncthreads();
+  if (tid < 64) {  // where each class starts
+    const uint32_t a = count[2 * tid], b = count[2 * tid + 1];
+    uint32_t x = a + b;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t y = __shfl_up(x, d);
+      if (tid >= d) x += y;
+    }
+    count[2 * tid] = x - a - b;
+    count[2 * tid + 1] = x - b;
+    if (tid == 63) count[kPkClasses] = x;
+  }
+  __syncthreads();
+  tiles([&](int seq, int t, int cls) {
+    const uint32_t at = atomicAdd(count + cls, 1u);
+    if (at < (uint32_t)slots) order[at] = make_int2(seq, t);  // bounds out of order may name more tiles
+  });
+  for (int s = (int)min(count[kPkClasses], (uint32_t)slots) + tid; s < slots; s += 256) order[s] = make_int2(0, -1);
+}
+
+// The tile of workgroup slot `slot`, by the list where there is one (tile -1: nothing to do).
+__device__ __forceinline__ PackedTile pk_tile(const int2* order, const int32_t* cu, int n, int T, int g, int bm, int slot) {
+  if (!order) return pk_find_tile(cu, n, T, g, bm, slot);
+  PackedTile r;
+  r.seq = __builtin_amdgcn_readfirstlane(order[slot].x);
+  r.tile = __builtin_amdgcn_readfirstlane(order[slot].y);
+  r.start = __builtin_amdgcn_readfirstlane(pk_bound(cu, n, T, r.seq));
+  r.len = max(0, __builtin_amdgcn_readfirstlane(pk_bound(cu, n, T, r.seq + 1)) - r.start);
+  return r;
+}
+
 // The sequence of token t (a search per lane).
 __device__ __forceinline__ PackedTile pk_token(const int32_t* cu, int n, int T, int t) {
   int lo = 0, hi = n + 2;  // the sequence lies in [lo, hi)

@@ -43,6 +43,8 @@ struct PackedBwdParams {
   float* ndelta;      // [H][Tq] -delta
   uint32_t* max_do;   // [n + 2][Hk] largest |do_i| of a sequence's rows, as float bits (fp16 only)
   uint32_t* max_v;    // [n + 2][Hk] largest |v_j|
+  int2* order_q;      // tiles of the dQ and of the dK/dV pass by falling work, or null
+  int2* order_k;
   int split_dq, split_dkv;  // parts that the passes' inner loops are cut into
   float* part_dq;     // split_dq > 1: [part][Tq][H][D]
   float* part_dkv;    // split_dkv > 1: [part][dk, dv][Tk][Hk][D]
@@ -53,6 +55,12 @@ struct PackedBwdParams {
   int64_t dqst, dqsh, dkst, dksh, dvst, dvsh;
   float scale, scale_log2;
 };
+
+constexpr int kBwdTile = 128;  // rows of a dQ workgroup, keys of a dK/dV workgroup
+
+// Workgroup slots per key head of the two passes.
+__host__ __device__ inline int dq_slots(const PackedBwdParams& p) { return (int)((int64_t)p.Tq * p.G / kBwdTile) + p.n + 2; }
+__host__ __device__ inline int dkv_slots(const PackedBwdParams& p) { return p.Tk / kBwdTile + p.n + 2; }
 
 // fp16: P enters its product times 2^14.
 template <typename E>
@@ -123,16 +131,26 @@ __device__ __forceinline__ void pk_largest_v(const PackedBwdParams& p, int slot,
   maxima.finish();
 }
 
-// The first qslots workgroups take query rows, the others (MAXIMA) rows of V.
+// Workgroups 0 and 1 form the lists of the two passes' tiles, the next qslots take query rows, the others
+// (MAXIMA) rows of V.
 template <typename E, int D, bool MAXIMA>
 __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdParams p, int qslots) {
   constexpr int LPR = D / 8;
-  __shared__ uint32_t top[kStatHeads];
-  if (MAXIMA && (int)blockIdx.x >= qslots) {
-    pk_largest_v<E, D>(p, blockIdx.x - qslots, top);
+  __shared__ uint32_t top[kStatHeads > kPkClasses ? kStatHeads : kPkClasses + 1];
+  if (blockIdx.x == 0) {
+    if (p.order_q) pk_order<false>(p.cu_q, p.Tq, p.cu_k, p.Tk, p.n, p.G, kBwdTile, p.causal, dq_slots(p), p.order_q, top);
     return;
   }
-  const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, 1, kStatTokens, blockIdx.x);
+  if (blockIdx.x == 1) {
+    if (p.order_k) pk_order<true>(p.cu_k, p.Tk, p.cu_q, p.Tq, p.n, 1, kBwdTile, p.causal, dkv_slots(p), p.order_k, top);
+    return;
+  }
+  const int block = blockIdx.x - 2;
+  if (MAXIMA && block >= qslots) {
+    pk_largest_v<E, D>(p, block - qslots, top);
+    return;
+  }
+  const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, 1, kStatTokens, block);
   const int t0 = pt.tile * kStatTokens;
   if (t0 >= pt.len) return;
   const int rows = min(kStatTokens, pt.len - t0) * p.H;
@@ -178,7 +196,7 @@ __device__ __forceinline__ void pk_store_part(float* row, const f32x16& acc, flo
 // ---------------------------------------------------------------------------------------
 template <typename E, int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(const PackedBwdParams p) {
-  constexpr int KS = D / 16, DB = D / 32, BM = 128;
+  constexpr int KS = D / 16, DB = D / 32, BM = kBwdTile;
   constexpr int kTileBytes = 64 * 2 * D;
   constexpr bool kFp16 = __is_same(E, FP16);
   __shared__ __align__(16) uint8_t kt0[kTileBytes], kt1[kTileBytes], vt0[kTileBytes], vt1[kTileBytes];
@@ -187,10 +205,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int hk = blockIdx.x % p.Hk;
-  const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, p.G, BM, blockIdx.x / p.Hk);
+  const PackedTile pt = pk_tile(p.order_q, p.cu_q, p.n, p.Tq, p.G, BM, blockIdx.x / p.Hk);
   const int rows = pt.len * p.G;
   const int ntile = (rows + BM - 1) / BM;
-  if (pt.tile >= ntile) return;
+  if (pt.tile < 0 || pt.tile >= ntile) return;
   const int row0 = (p.causal ? ntile - 1 - pt.tile : pt.tile) * BM;
   int k0, lk;
   pk_other(p.cu_k, p.n, p.Tk, pt.seq, k0, lk);
@@ -339,7 +357,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
 // ---------------------------------------------------------------------------------------
 template <typename E, int D>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedBwdParams p) {
-  constexpr int KS = D / 16, DB = D / 32, BN = 128;
+  constexpr int KS = D / 16, DB = D / 32, BN = kBwdTile;
   constexpr int kTileBytes = 64 * 2 * D;
   constexpr bool kFp16 = __is_same(E, FP16);
   __shared__ __align__(16) uint8_t qt0[kTileBytes], qt1[kTileBytes], gt0[kTileBytes], gt1[kTileBytes];
@@ -349,9 +367,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int hk = blockIdx.x % p.Hk;
-  const PackedTile pt = pk_find_tile(p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk);
+  const PackedTile pt = pk_tile(p.order_k, p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk);
   const int key0 = pt.tile * BN;
-  if (key0 >= pt.len) return;
+  if (key0 < 0 || key0 >= pt.len) return;
   int q0, lq;
   pk_other(p.cu_q, p.n, p.Tq, pt.seq, q0, lq);
   const int shift = pt.len - lq;  // causal: key j is seen by tokens i >= j - shift
@@ -595,6 +613,7 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(const float* __res
 // least 512 keys or queries on average. The parts' fp32 sums are joined in order by another launch.
 struct BwdPlan {
   int dq, dkv;
+  int64_t slots_q, slots_k;  // entries of the lists of tiles (0: no list)
   size_t dq_bytes, dkv_bytes;
 };
 
@@ -608,6 +627,11 @@ BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
     return (int)(s > 16 ? 16 : s > 1 ? s : 1);
   };
   BwdPlan b = {};
+  // A single sequence's tiles are in falling order as they are.
+  b.slots_q = Tq * G / kBwdTile + n + 2;
+  b.slots_k = Tk / kBwdTile + n + 2;
+  if (n < 2 || Tq == 0 || b.slots_q > kPkOrderMax) b.slots_q = 0;
+  if (n < 2 || Tq == 0 || b.slots_k > kPkOrderMax) b.slots_k = 0;
   b.dq = parts(Tq * G, Tk);
   b.dkv = parts(Tk, Tq * G);
   b.dq_bytes = b.dq > 1 ? (size_t)b.dq * Tq * Hq * D * sizeof(float) : 0;
@@ -618,7 +642,7 @@ BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
 template <typename E, int D>
 int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
   constexpr bool kFp16 = __is_same(E, FP16);
-  const int64_t qslots = (int64_t)p.Tq * p.G / 128 + p.n + 2, kslots = (int64_t)p.Tk / 128 + p.n + 2;
+  const int64_t qslots = dq_slots(p), kslots = dkv_slots(p);
   GW_CHECK_ARG(qslots * p.Hk < (1ll << 31) && kslots * p.Hk < (1ll << 31), "the grid is too large");
   if (kFp16) {
     const int64_t words = 2 * (int64_t)(p.n + 2) * p.Hk;  // max_do and max_v, one behind the other
@@ -628,7 +652,8 @@ int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
   }
   if (p.Tq > 0) {
     const int stat_q = p.Tq / kStatTokens + p.n + 2, stat_k = kFp16 && p.Tk > 0 ? p.Tk / kStatTokens + p.n + 2 : 0;
-    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D, kFp16>), dim3((uint32_t)stat_q + stat_k), dim3(256), 0, stream, p, stat_q);
+    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D, kFp16>), dim3(2u + stat_q + stat_k), dim3(256), 0, stream, p,
+                       stat_q);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (rows)");
     hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)(qslots * p.Hk), p.split_dq), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq)");
@@ -670,7 +695,7 @@ extern "C" size_t gw_packed_attn_bwd_workspace_size(int64_t n, int64_t Tq, int64
   if (n < 0 || Tq < 0 || Tk < 0 || Hk < 1 || Hq < Hk || D < 1) return 0;
   const gw::BwdPlan b = gw::packed_bwd_plan(n, Tq, Tk, Hq, Hk, D);
   return gw::pk_align((size_t)Tq * Hq * 8) + gw::pk_align((size_t)(n + 2) * Hk * 8) + gw::pk_align(b.dq_bytes) +
-         gw::pk_align(b.dkv_bytes);
+         gw::pk_align(b.dkv_bytes) + 8 * (size_t)(b.slots_q + b.slots_k);
 }
 
 extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
@@ -718,6 +743,9 @@ extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_str
   p.split_dkv = b.dkv;
   p.part_dq = reinterpret_cast<float*>(ws + pk_align((size_t)Tq * Hq * 8) + pk_align((size_t)(n + 2) * Hk * 8));
   p.part_dkv = p.part_dq + pk_align(b.dq_bytes) / sizeof(float);
+  int2* lists = reinterpret_cast<int2*>(p.part_dkv + pk_align(b.dkv_bytes) / sizeof(float));
+  if (b.slots_q) p.order_q = lists;
+  if (b.slots_k) p.order_k = lists + b.slots_q;
   p.cu_q = cu_q;
   p.cu_k = cu_k;
   p.n = (int)n;
