@@ -6,7 +6,7 @@
 // One pass over the keys with a running reference maximum m and sum l (held in fp32, in the exp2
 // domain): o = (sum_j 2^(s_j - m) v_j) / l. m is raised only when a lane's weights of 32 keys sum past
 // 2^15, so P fits fp16 and no maximum is taken per tile otherwise; the result does not depend on which m
-// was used. P is rounded to the inputs' 16-bit type for the second product (half a step, 2^-9 or 2^-12
+// was used. P is rounded to the inputs' 16-bit type for the second product (half a step, 2^-8 or 2^-11
 // of a weight, with errors that average out over the keys); sums add the fp32 weights.
 //
 // The rows of a key head are (token, head of the group), token-major, so a group's heads share the
