@@ -16,6 +16,12 @@
 // packed weights are the second product's operand as they are; V is read from its row-major tile by
 // transposing LDS reads. The next 32 keys' scores are issued before the current weights are formed.
 //
+// Bound by the matrix cores and the vector unit together (one exp2, half a pack and an add per score): 43,968
+// tokens x 16 heads of 64 in bf16 7.4 to 7.7 ms, 1.02 to 1.07 PFLOP/s with the matrix cores busy 55 % of the
+// time; 12 causal sequences of up to 8,844 tokens, 16 heads over 4 of 128 in fp16, 1.46 ms, 1.0 PFLOP/s (61 %).
+// Tiles by falling work, as in the backward, need a launch of their own here (7 to 14 us) and
+// saved 4 us of 57 on 96 short sequences, 20 of 428 on six long ones.
+//
 // Rows of K and V behind a sequence's end arrive as zeros (the loads' descriptor ends there), so
 // what lies in memory behind it, inf and NaN included, cannot reach a result.
 #include <math.h>

@@ -20,7 +20,8 @@
  *    caller casts fp32 to 16 bits first, dsa_attention.py:5296-5300). The indexer top-k,
  *    its backward and its view-bias gradient also take GW_DTYPE_FP32 (the reference's
  *    indexer computes in q.dtype, any float type: sparse_topk_indexer.py:1293, and its
- *    caller may cast to score_dtype float32: indexer.py:321-326).
+ *    caller may cast to score_dtype float32: indexer.py:321-326), and so does the rotation
+ *    of gw_rotary_axes.
  */
 #ifndef GEOWEAVE_HIP_H
 #define GEOWEAVE_HIP_H
@@ -39,7 +40,7 @@ extern "C" {
 
 #define GW_DTYPE_BF16 0
 #define GW_DTYPE_FP16 1
-#define GW_DTYPE_FP32 2 /* the indexer entry points and gw_indexer_kl_* only */
+#define GW_DTYPE_FP32 2 /* the indexer entry points, gw_indexer_kl_* and gw_rotary_axes only */
 
 /* Message for the last failed call on this thread ("" if none). */
 const char* gw_last_error(void);
@@ -668,8 +669,9 @@ int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strides, void* y
  * left (the backward needs it). Bounds outside [0, Tq] or [0, Tk] are clamped.
  * D in {64, 128}, bf16 or fp16, softmax_scale > 0; 16-byte aligned rows, token strides in [0, 2^24)
  * elements; tokens x Hq below 2^31 - 2^12. workspace: gw_packed_attn_fwd_workspace_size(...) bytes,
- * 16-byte aligned (parts of the keys, where they are split over workgroups). Nothing is read from the device by the host: a captured graph may
- * be replayed with other bounds of the same n.
+ * 16-byte aligned (parts of the keys, where they are split over workgroups). Nothing is read from the
+ * device by the host: a captured graph may be replayed with other bounds of the same n. Bounds out of
+ * order give unspecified values, and no access outside the tensors and the workspace.
  * ------------------------------------------------------------------------------------ */
 size_t gw_packed_attn_fwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
 int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
