@@ -244,7 +244,14 @@ def strides2(x0: int, x1: int):
 
 def row_strides(x: torch.Tensor):
     """Strides of all dims but the last, 0 for those of one entry (torch leaves them whatever they were)."""
+    if 1 not in x.shape:
+        return x.stride()[:-1]
     return [st if n != 1 else 0 for n, st in zip(x.shape[:-1], x.stride())]
+
+
+def empty_rows(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape, type and device (half the host time of ``torch.empty``)."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -87,7 +87,7 @@ def _prep(x: torch.Tensor) -> torch.Tensor:
     # 16-byte rows, and a token stride within the kernels' offsets; a copy where they are not (clone: a
     # contiguous tensor may start anywhere).
     st, sh = _lib.row_strides(x)
-    if x.stride(2) != 1 or st % 8 or sh % 8 or st >= MAX_ROW_STRIDE or x.data_ptr() % 16:
+    if x.stride(2) != 1 or (st | sh) & 7 or st >= MAX_ROW_STRIDE or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -99,9 +99,9 @@ def _rows(x: torch.Tensor):
 def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool, want_rest: bool = False):
     """(o, lse | None, what o's rounding left | None) for a native head dim."""
     q, k, v = _prep(q), _prep(k), _prep(v)
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    o = _lib.empty_rows(q)
     lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if want_lse else None
-    rest = torch.empty_like(o) if want_rest else None
+    rest = _lib.empty_rows(q) if want_rest else None
     if q.shape[0] == 0:
         return o, lse, rest
     lib = _lib.load()
@@ -118,7 +118,7 @@ def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool, wa
 
 def _backward(do, q, k, v, cu_q, cu_k, o, rest, lse, causal: bool, scale: float):
     q, k, v, o, do = (_prep(x) for x in (q, k, v, o, do))
-    dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
+    dq, dk, dv = (_lib.empty_rows(x) for x in (q, k, v))
     if q.shape[0] == 0 and k.shape[0] == 0:
         return dq, dk, dv
     n, tq, tk, hq, hk, d = cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]

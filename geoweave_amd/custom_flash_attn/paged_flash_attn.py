@@ -32,7 +32,8 @@ __all__ = ["paged_flash_attn_inference_func"]
 MAX_KEYS = 0x7FFFF000
 
 
-def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale) -> float:
+def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale):
+    """(scale, strides of k_cache, of v_cache), checked."""
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, Hq, D] or [B, N, Hq, D], got {tuple(q.shape)}")
     if k_cache.dim() != 4:
@@ -53,11 +54,14 @@ def _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale
     scale = _check_scale(softmax_scale, d)
     if not (q.is_cuda and all(t.device == q.device for t in (k_cache, v_cache, block_table, cache_seqlens))):
         raise ValueError("q, the caches, block_table and cache_seqlens must be tensors of one GPU")
+    strides = []
     for c in (k_cache, v_cache):
         # Copying a cache to align it would cost more than the call: the caller lays it out.
-        if c.numel() and (c.stride(-1) != 1 or any(s % 8 for s in _lib.row_strides(c)) or c.data_ptr() % 16):
+        page, slot, head = _lib.row_strides(c)
+        if c.numel() and (c.stride(3) != 1 or (page | slot | head) & 7 or c.data_ptr() % 16):
             raise ValueError("caches need a unit last stride and 16-byte aligned rows")
-    return scale
+        strides.append(_lib.strides3(page, slot, head))
+    return scale, *strides
 
 
 def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -65,17 +69,23 @@ def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_ca
                                     softmax_scale: Optional[float] = None, return_lse: bool = False,
                                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(o in q's shape and dtype, lse fp32 ``q.shape[:-1]`` where asked for); see the module docstring."""
-    scale = _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale)
-    if q.stride(-1) != 1 or any(s % 8 for s in _lib.row_strides(q)) or q.data_ptr() % 16:
+    scale, k_strides, v_strides = _check_inputs(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale)
+    new = _lib.row_strides(q)
+    if q.stride(-1) != 1 or any(s & 7 for s in new) or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)  # a contiguous tensor may start anywhere
+        new = _lib.row_strides(q)
     if block_table.stride(-1) != 1:
         block_table = block_table.contiguous()
     cache_seqlens = cache_seqlens.contiguous()
     dev = q.device
-    o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    o = _lib.empty_rows(q)
     lse = torch.empty(q.shape[:-1], device=dev, dtype=torch.float32) if return_lse else None
-    q4, o4 = (q.unsqueeze(1), o.unsqueeze(1)) if q.dim() == 3 else (q, o)
-    b, n, hq, d = q4.shape
+    if q.dim() == 4:
+        b, n, hq, d = q.shape
+        q_strides, o_strides = _lib.strides3(*new), _lib.strides3(n * hq * d, hq * d, d)
+    else:
+        (b, hq, d), n = q.shape, 1
+        q_strides, o_strides = _lib.strides3(new[0], 0, new[1]), _lib.strides3(hq * d, 0, d)
     if b == 0 or n == 0:
         return o, lse
     pages, page, hk, _ = k_cache.shape
@@ -84,10 +94,9 @@ def paged_flash_attn_inference_func(q: torch.Tensor, k_cache: torch.Tensor, v_ca
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
     with _lib.on_device(dev):
         rc = lib.gw_paged_attn_fwd(
-            _lib.dtype_code(q.dtype), q4.data_ptr(), _lib.strides3(*_lib.row_strides(q4)), k_cache.data_ptr(),
-            _lib.strides3(*_lib.row_strides(k_cache)), v_cache.data_ptr(), _lib.strides3(*_lib.row_strides(v_cache)),
-            block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), o4.data_ptr(),
-            _lib.strides3(*_lib.row_strides(o4)), _lib.ptr(lse), b, n, hq, hk, d, pages, page, block_table.shape[1],
-            int(causal), scale, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+            _lib.dtype_code(q.dtype), q.data_ptr(), q_strides, k_cache.data_ptr(), k_strides, v_cache.data_ptr(), v_strides,
+            block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), o.data_ptr(), o_strides,
+            _lib.ptr(lse), b, n, hq, hk, d, pages, page, block_table.shape[1], int(causal), scale, _lib.ptr(ws), nbytes,
+            _lib.stream_handle(dev))
     _lib.check(rc, "gw_paged_attn_fwd")
     return o, lse

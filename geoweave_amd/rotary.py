@@ -90,7 +90,7 @@ def _check(q, k, positions, axis_dims, bases):
 def _rotate(xs, positions, axis_dims, bases, inverse: bool):
     """Turned copies (contiguous) of one or two tensors."""
     xs = [x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous() for x in xs]
-    ys = [torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in xs]
+    ys = [_lib.empty_rows(x) for x in xs]
     B = xs[0].shape[0] if xs[0].dim() == 4 else 1
     T, D = xs[0].shape[-3], xs[0].shape[-1]
     if B == 0 or T == 0 or all(x.shape[-2] == 0 for x in xs):

@@ -83,6 +83,17 @@ def test_more_sequences_than_one_scan_round(gpu_device):
     check(o, lse, paged_attention(*args), torch.float16, 128)
 
 
+def test_pages_that_several_sequences_share(gpu_device):
+    """A prefix that sequences have in common, and a page that one sequence names twice."""
+    args = list(make([200, 330, 96, 2000], 2, 4, 2, 64, 16, torch.bfloat16, 5))
+    table = args[3]
+    table[1, :6] = table[0, :6]
+    table[2, :6] = table[0, :6]
+    table[3, 40:80] = table[3, 0:40]
+    o, lse = run(args, gpu_device)
+    check(o, lse, paged_attention(*args), torch.bfloat16, 64)
+
+
 def test_unused_slots_and_pages_outside_the_pool(gpu_device):
     """inf and NaN wherever no key lies, page numbers outside the pool in the middle and at the end."""
     args = list(make([300, 77, 500, 40], 4, 4, 2, 64, 24, torch.bfloat16, 3))
