@@ -264,7 +264,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one (a launch goes to the current device, and
     a caller's tensors may lie on another)."""
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _SAME_DEVICE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def stream_handle(device: torch.device) -> int:

@@ -83,52 +83,51 @@ def _check_inputs(q, k, v, cu_q, cu_k, softmax_scale):
     return cu_q.contiguous(), cu_k.contiguous(), scale
 
 
-def _prep(x: torch.Tensor) -> torch.Tensor:
-    # 16-byte rows, and a token stride within the kernels' offsets; a copy where they are not (clone: a
-    # contiguous tensor may start anywhere).
+def _rows(x: torch.Tensor):
+    """(x, (its address, its strides)) with 16-byte rows, and a token stride within the kernels' offsets; of a copy
+    where they are not (clone: a contiguous tensor may start anywhere)."""
     st, sh = _lib.row_strides(x)
     if x.stride(2) != 1 or (st | sh) & 7 or st >= MAX_ROW_STRIDE or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _rows(x: torch.Tensor):
-    return x.data_ptr(), _lib.strides2(*_lib.row_strides(x))
+        st, sh = _lib.row_strides(x)
+    return x, (x.data_ptr(), _lib.strides2(st, sh))
 
 
 def _forward(q, k, v, cu_q, cu_k, causal: bool, scale: float, want_lse: bool, want_rest: bool = False):
     """(o, lse | None, what o's rounding left | None) for a native head dim."""
-    q, k, v = _prep(q), _prep(k), _prep(v)
+    tq, hq, d = q.shape
     o = _lib.empty_rows(q)
-    lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if want_lse else None
+    lse = torch.empty((tq, hq), device=q.device, dtype=torch.float32) if want_lse else None
     rest = _lib.empty_rows(q) if want_rest else None
-    if q.shape[0] == 0:
+    if tq == 0:
         return o, lse, rest
+    (q, qr), (k, kr), (v, vr) = _rows(q), _rows(k), _rows(v)
     lib = _lib.load()
-    sizes = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+    sizes = (cu_q.numel() - 1, tq, k.shape[0], hq, k.shape[1], d)
     nbytes = int(lib.gw_packed_attn_fwd_workspace_size(*sizes))
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     with _lib.on_device(q.device):
-        rc = lib.gw_packed_attn_fwd(_lib.dtype_code(q.dtype), *_rows(q), *_rows(k), *_rows(v), cu_q.data_ptr(),
-                                    cu_k.data_ptr(), *_rows(o), _lib.ptr(rest), _lib.ptr(lse), *sizes, int(causal), scale,
-                                    _lib.ptr(ws), nbytes, _lib.stream_handle(q.device))
+        rc = lib.gw_packed_attn_fwd(_lib.dtype_code(q.dtype), *qr, *kr, *vr, cu_q.data_ptr(), cu_k.data_ptr(),
+                                    o.data_ptr(), _lib.strides2(hq * d, d), _lib.ptr(rest), _lib.ptr(lse), *sizes,
+                                    int(causal), scale, _lib.ptr(ws), nbytes, _lib.stream_handle(q.device))
     _lib.check(rc, "gw_packed_attn_fwd")
     return o, lse, rest
 
 
 def _backward(do, q, k, v, cu_q, cu_k, o, rest, lse, causal: bool, scale: float):
-    q, k, v, o, do = (_prep(x) for x in (q, k, v, o, do))
-    dq, dk, dv = (_lib.empty_rows(x) for x in (q, k, v))
-    if q.shape[0] == 0 and k.shape[0] == 0:
+    dq, dk, dv = _lib.empty_rows(q), _lib.empty_rows(k), _lib.empty_rows(v)
+    (tq, hq, d), (tk, hk, _) = q.shape, k.shape
+    if tq == 0 and tk == 0:
         return dq, dk, dv
-    n, tq, tk, hq, hk, d = cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
+    (q, qr), (k, kr), (v, vr), (o, orow), (do, dor) = _rows(q), _rows(k), _rows(v), _rows(o), _rows(do)
+    n, q_out, k_out = cu_q.numel() - 1, _lib.strides2(hq * d, d), _lib.strides2(hk * d, d)
     lib = _lib.load()
     nbytes = int(lib.gw_packed_attn_bwd_workspace_size(n, tq, tk, hq, hk, d))
     ws = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
     with _lib.on_device(q.device):
-        rc = lib.gw_packed_attn_bwd(_lib.dtype_code(q.dtype), *_rows(q), *_rows(k), *_rows(v), cu_q.data_ptr(),
-                                    cu_k.data_ptr(), *_rows(o), rest.data_ptr(), *_rows(do), lse.data_ptr(), *_rows(dq), *_rows(dk),
-                                    *_rows(dv), n, tq, tk, hq, hk, d, int(causal), scale, ws.data_ptr(), nbytes,
+        rc = lib.gw_packed_attn_bwd(_lib.dtype_code(q.dtype), *qr, *kr, *vr, cu_q.data_ptr(), cu_k.data_ptr(), *orow,
+                                    rest.data_ptr(), *dor, lse.data_ptr(), dq.data_ptr(), q_out, dk.data_ptr(), k_out,
+                                    dv.data_ptr(), k_out, n, tq, tk, hq, hk, d, int(causal), scale, ws.data_ptr(), nbytes,
                                     _lib.stream_handle(q.device))
     _lib.check(rc, "gw_packed_attn_bwd")
     return dq, dk, dv

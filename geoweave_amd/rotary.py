@@ -97,7 +97,8 @@ def _rotate(xs, positions, axis_dims, bases, inverse: bool):
         return ys
     args = []
     for x, y in zip(xs, ys):
-        args += [x.data_ptr(), _strides(x), y.data_ptr(), _strides(y), x.shape[-2]]
+        h = x.shape[-2]
+        args += [x.data_ptr(), _strides(x), y.data_ptr(), _lib.strides3(T * h * D, h * D, D), h]
     if len(xs) == 1:
         args += [None, None, None, None, 0]
     pos_strides = _lib.strides3(*positions.stride()) if positions.dim() == 3 else _lib.strides3(0, *positions.stride())
