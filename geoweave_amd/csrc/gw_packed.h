@@ -417,6 +417,14 @@ __device__ __forceinline__ void pk_store4(uint16_t* row, uint16_t* rest, float a
   if (rest) *reinterpret_cast<uint2*>(rest) = make_uint2(pk_pair_rest<E>(a, b, x), pk_pair_rest<E>(c, d, y));
 }
 
+// Waits for this wave's LDS accesses only (loads stay in flight), then for the other waves.
+__device__ __forceinline__ void pk_lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Waits for this wave's loads and LDS accesses, then for the other waves.
 __device__ __forceinline__ void pk_tile_barrier() {
   __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)

@@ -21,8 +21,7 @@
 //
 // Bound as the forward is, by the matrix cores and the vector unit: six sequences of 3,013 to 4,795 tokens,
 // 16 heads of 64 in bf16, dQ 552 us (1.01 PFLOP/s, matrix cores busy 60 % of the time), dK/dV 790 us (0.95, 54 %),
-// the statistics 28 us. D = 128 holds dK/dV to one wave per SIMD (690 TFLOP/s); dV and dK
-// in a pass each were slower. 96 causal sequences of 17 to 697 tokens, 16 heads over 8: 27 + 54 + 79 us;
+// the statistics 28 us; the same with heads of 128 dQ 1,016 us (1.1 PFLOP/s), dK/dV 1,660 (0.90). 96 causal sequences of 17 to 697 tokens, 16 heads over 8: 27 + 54 + 79 us;
 // without the lists of tiles by falling work 24 + 61 + 103.
 //
 // Rows behind a sequence's end arrive as zeros, and rows that see no key have P = 0.
@@ -356,14 +355,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
 }
 
 // ---------------------------------------------------------------------------------------
-// dK and dV: 4 waves x 32 keys of one key head; tiles of 64 query tokens of each head of the group. A
+// dK and dV, D = 64: 4 waves x 32 keys of one key head; tiles of 64 query tokens of each head of the group. A
 // lane holds one key and 16 queries of S = Q K^T and dP = dO V^T, whose products start at -lse / scale
 // and -delta. (64 keys per wave, one wave per SIMD, read half as much from LDS and took 20 % longer: the
 // products and the weights of one wave do not overlap enough.)
 // ---------------------------------------------------------------------------------------
-template <typename E, int D>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedBwdParams p) {
-  constexpr int KS = D / 16, DB = D / 32, BN = kBwdTile;
+template <typename E>
+__global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdParams p) {
+  constexpr int D = 64, KS = D / 16, DB = D / 32, BN = kBwdTile;
   constexpr int kTileBytes = 64 * 2 * D;
   constexpr bool kFp16 = __is_same(E, FP16);
   __shared__ __align__(16) uint8_t qt0[kTileBytes], qt1[kTileBytes], gt0[kTileBytes], gt1[kTileBytes];
@@ -470,9 +469,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
       dp[4 * g + 3] = y.w;
     }
     // Operands of the products in the order of their use, read PRE products ahead; the scheduling barriers
-    // keep the compiler from reading them all at once, for which there are no registers (D = 64: 759 us for
-    // 794 on 6 scenes of 2 to 8 views).
-    constexpr int PRE = D == 64 ? 2 : 4;
+    // keep the compiler from reading them all at once, for which there are no registers (759 us for 794
+    // on 6 scenes of 2 to 8 views).
+    constexpr int PRE = 2;
     auto row = [&](int i) __attribute__((always_inline)) { return i < KS ? at.row(qt, st, i) : at.row(gt, st, i - KS); };
     // Columns for each 16 queries and 32 dims: of dO, then of Q.
     auto column = [&](int i) __attribute__((always_inline)) {
@@ -591,6 +590,238 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(co
   }
 }
 
+// The same for D = 128, where one wave cannot hold K, V, dK and dV and leave room for another on its SIMD: waves
+// w and w + 4 share 32 keys. The first holds K and dV: S, P and P^T dO. The second holds V and dK: dP, dS
+// and dS^T Q, with P from the first through LDS in fp32. A barrier in the middle of a tile hands P over; the
+// two meet on one SIMD, where the products of one run beside the weights of the other. Six sequences of 3,013 to
+// 4,795 tokens, 16 heads, bf16: 1,660 us, 2,062 with one wave per SIMD that holds all four, and longer still with dV
+// and dK in a pass each.
+template <typename E>
+__global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const PackedBwdParams p) {
+  constexpr int D = 128, KS = D / 16, DB = D / 32, BN = kBwdTile;
+  constexpr int kTileBytes = 64 * 2 * D;
+  constexpr bool kFp16 = __is_same(E, FP16);
+  __shared__ __align__(16) uint8_t qt0[kTileBytes], qt1[kTileBytes], gt0[kTileBytes], gt1[kTileBytes];
+  __shared__ __align__(16) float nl0[64], nl1[64], nd0[64], nd1[64];
+  __shared__ __align__(16) float4 weights[4][2][4][64];  // [keys][sub-tile][quad][lane]
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave & 3;
+  const int col = lane & 31, half = lane >> 5;
+  const int hk = blockIdx.x % p.Hk;
+  const PackedTile pt = pk_tile(p.order_k, p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk);
+  const int key0 = pt.tile * BN;
+  if (key0 < 0 || key0 >= pt.len) return;
+  int q0, lq;
+  pk_other(p.cu_q, p.n, p.Tq, pt.seq, q0, lq);
+  const int shift = pt.len - lq;  // causal: key j is seen by tokens i >= j - shift
+  const float sl2 = p.scale_log2;
+  const int wkey = key0 + kw * 32;
+  const int key = wkey + col;
+  const bool on = key < pt.len;
+
+  int e = 0;
+  if (kFp16) {
+    const int64_t at = (int64_t)pt.seq * p.Hk + hk;
+    e = pk_scale_exp(__uint_as_float(p.max_do[at]) * __uint_as_float(p.max_v[at]));
+  }
+  const float dscale = kFp16 ? ldexpf(1.f, e - 14) : 1.f;
+
+  const int first = p.causal ? max(0, key0 - shift) >> 6 : 0;  // first tile with a query that sees a key
+  const int ntq = (lq + 63) >> 6;
+  const int per = ntq > first ? ntq - first : 0;
+  const int64_t all = (int64_t)per * p.G;
+  const int64_t share = p.split_dkv > 1 ? (all + p.split_dkv - 1) / p.split_dkv : all;
+  const int64_t t0 = min((int64_t)blockIdx.y * share, all);
+  const int total = (int)min(share, all - t0);
+
+  PkRows<D, 512> qrows, grows;
+  const uint16_t* qbase = p.q + (int64_t)q0 * p.qst + (int64_t)hk * p.G * p.qsh;
+  const uint16_t* gbase = p.dout + (int64_t)q0 * p.gst + (int64_t)hk * p.G * p.gsh;
+  const int64_t sbase = (int64_t)hk * p.G * p.Tq + q0;
+  qrows.init(qbase, p.qst, lq, tid);
+  grows.init(gbase, p.gst, lq, tid);
+  int ld_h = per > 0 ? (int)(t0 / per) : 0;
+  int ld_t = first + (int)(t0 - (int64_t)ld_h * per);
+  auto load = [&](uint8_t* qd, uint8_t* gd, float* ld, float* dd) __attribute__((always_inline)) {
+    qrows.base = uniform_ptr(reinterpret_cast<const char*>(qbase + (int64_t)ld_h * p.qsh));
+    grows.base = uniform_ptr(reinterpret_cast<const char*>(gbase + (int64_t)ld_h * p.gsh));
+    qrows.load(ld_t, qd);
+    grows.load(ld_t, gd);
+    const int64_t sat = sbase + (int64_t)ld_h * p.Tq + ld_t * 64;
+    const int64_t left = (int64_t)(lq - ld_t * 64) * 4;
+    if (wave == 0)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.nlse + sat), left),
+                                               (__attribute__((address_space(3))) void*)ld, 4, lane * 4, 0, 0, 0);
+    if (wave == 4)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.ndelta + sat), left),
+                                               (__attribute__((address_space(3))) void*)dd, 4, lane * 4, 0, 0, 0);
+    if (++ld_t == ntq) {
+      ld_t = first;
+      if (++ld_h == p.G) ld_h = p.G - 1;
+    }
+  };
+  const PkLane<D> at(lane);
+
+  auto role = [&](auto second) __attribute__((always_inline)) {
+    constexpr bool B = decltype(second)::value;
+    uint4 st[KS];  // K or V rows of this lane's key
+    {
+      const int64_t t = pt.start + min(key, pt.len - 1);
+      const uint16_t* r = (B ? p.v + t * p.vst + (int64_t)hk * p.vsh : p.k + t * p.kst + (int64_t)hk * p.ksh) + half * 8;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) st[ks] = *reinterpret_cast<const uint4*>(r + ks * 16);
+    }
+    f32x16 acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+    bool unclean = false;
+
+    // A tile of 64 queries: rows of rt against the stationary rows, columns of ct into acc.
+    auto whole = [&](auto masked, const uint8_t* rt, const uint8_t* ct, const float* start, int i0)
+                     __attribute__((always_inline)) {
+      constexpr int PRE = 3;
+      f32x16 x[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 y = *reinterpret_cast<const float4*>(start + 32 * u + 8 * g + 4 * half);
+          x[u][4 * g] = y.x;
+          x[u][4 * g + 1] = y.y;
+          x[u][4 * g + 2] = y.z;
+          x[u][4 * g + 3] = y.w;
+        }
+      uint4 a[PRE], c[PRE];
+      auto column = [&](int i) __attribute__((always_inline)) {  // sub-tile, 16 queries, 32 dims
+        return at.col(ct, i / (2 * DB), i / DB % 2, i % DB);
+      };
+#pragma unroll
+      for (int i = 0; i < PRE; ++i) a[i] = at.row(rt, 0, i);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        x[i / KS] = mma(E{}, a[i % PRE], st[i % KS], x[i / KS]);
+        if (i + PRE < 2 * KS)
+          a[i % PRE] = at.row(rt, (i + PRE) / KS, (i + PRE) % KS);
+        else
+          c[i + PRE - 2 * KS] = column(i + PRE - 2 * KS);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      uint4 b[2][2];
+      auto sees = [&](int u, int i, float y) __attribute__((always_inline)) {
+        if constexpr (decltype(masked)::value) return 8 * (i / 4) + i % 4 >= key - shift - i0 - 32 * u - 4 * half ? y : 0.f;
+        return y;
+      };
+      if constexpr (!B) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = sees(u, i, fexp2(x[u][i] * sl2));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) weights[kw][u][g][lane] = make_float4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+          b[u][0] = pack_quad<E>(w);
+          b[u][1] = pack_quad<E>(w + 8);
+        }
+      }
+      pk_lds_barrier();
+      if constexpr (B) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float ds[16];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 w = weights[kw][u][g][lane];
+            ds[4 * g] = w.x;
+            ds[4 * g + 1] = w.y;
+            ds[4 * g + 2] = w.z;
+            ds[4 * g + 3] = w.w;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ds[i] = sees(u, i, kFp16 ? ds[i] * dscale * x[u][i] : ds[i] * x[u][i]);
+          if constexpr (decltype(masked)::value) {
+            const int j0 = i0 + 32 * u;
+            if (wkey == 0 && j0 <= -shift && -shift < j0 + 32) {  // the row that sees the first key only has dS = 0
+#pragma unroll
+              for (int i = 0; i < 16; ++i) ds[i] = 8 * (i / 4) + i % 4 + 4 * half == -shift - j0 ? 0.f : ds[i];
+            }
+          }
+          b[u][0] = pack_quad<E>(ds);
+          b[u][1] = pack_quad<E>(ds + 8);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4 * DB; ++i) {
+        uint4 q[1] = {c[i % PRE]};
+        if constexpr (decltype(masked)::value) {
+          const bool any = pk_clear_not_finite<E>(q);
+          if (!B) unclean |= any;  // keys that see a query whose q is not finite have a NaN dS
+        }
+        acc[i % DB] = mma(E{}, q[0], b[i / (2 * DB)][i / DB % 2], acc[i % DB]);
+        if (i + PRE < 4 * DB) c[i % PRE] = column(i + PRE);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+
+    int cur = per > 0 ? first + (int)(t0 % per) : 0;  // the tile that is computed
+    // Queries of tiles from `full` on see every key of the workgroup's block.
+    const int full = p.causal ? (key0 + BN - 1 - shift + 63) >> 6 : first;
+    auto tile = [&](auto buf) __attribute__((always_inline)) {
+      constexpr int N = decltype(buf)::value;
+      const uint8_t *rc = N ? (B ? gt1 : qt1) : (B ? gt0 : qt0), *cc = N ? (B ? qt1 : gt1) : (B ? qt0 : gt0);
+      const float* sc = N ? (B ? nd1 : nl1) : (B ? nd0 : nl0);
+      load(N ? qt0 : qt1, N ? gt0 : gt1, N ? nl0 : nl1, N ? nd0 : nd1);
+      if (wkey < pt.len && cur >= full)
+        whole(PkInt<0>{}, rc, cc, sc, 64 * cur);
+      else if (wkey < pt.len && 64 * cur + 63 + shift >= wkey)
+        whole(PkInt<1>{}, rc, cc, sc, 64 * cur);
+      else
+        pk_lds_barrier();
+      if (++cur == ntq) cur = first;
+      pk_tile_barrier();
+    };
+    int n = 0;
+#pragma unroll 1
+    for (; n + 1 < total; n += 2) {
+      tile(PkInt<0>{});
+      tile(PkInt<1>{});
+    }
+    if (n < total) tile(PkInt<0>{});
+    if (__builtin_expect(unclean, 0)) {
+      for (int64_t x = t0; x < t0 + total; ++x) {
+        const int h = (int)(x / per), i0 = 64 * (first + (int)(x % per));
+        for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i)
+          pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, acc);
+      }
+    }
+    // Rows of a sequence of one key all have dS = 0.
+    const float f = B ? (pt.len == 1 ? 0.f : kFp16 ? ldexpf(p.scale, -e) : p.scale) : kFp16 ? ldexpf(1.f, -14) : 1.f;
+    const int64_t t = pt.start + (on ? key : 0);
+    if (p.split_dkv > 1) {
+      const int64_t part = (int64_t)p.Tk * p.Hk * D;
+      float* dst = p.part_dkv + (2 * blockIdx.y + (B ? 0 : 1)) * part + (t * p.Hk + hk) * D;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) pk_store_part(dst + 32 * db, acc[db], f, half, on);
+      return;
+    }
+    uint16_t* dst = B ? p.dk + t * p.dkst + (int64_t)hk * p.dksh : p.dv + t * p.dvst + (int64_t)hk * p.dvsh;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) pk_store_col<E>(dst + 32 * db, acc[db], f, half, on);
+  };
+
+  if (total > 0) {
+    load(qt0, gt0, nl0, nd0);
+    pk_tile_barrier();
+  }
+  if (wave < 4)
+    role(PkInt<0>{});
+  else
+    role(PkInt<1>{});
+}
+
 // Sums the parts of a gradient [T, H, D], in order: part i at src + i * step.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void packed_bwd_join_kernel(const float* __restrict__ src, int64_t step, int parts,
@@ -671,7 +902,12 @@ int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
     }
   }
   if (p.Tk > 0) {
-    hipLaunchKernelGGL((packed_bwd_dkv_kernel<E, D>), dim3((uint32_t)(kslots * p.Hk), p.split_dkv), dim3(256), 0, stream, p);
+    const dim3 tiles((uint32_t)(kslots * p.Hk), p.split_dkv);
+    if constexpr (D == 64) {
+      hipLaunchKernelGGL(packed_bwd_dkv_kernel<E>, tiles, dim3(256), 0, stream, p);
+    } else {
+      hipLaunchKernelGGL(packed_bwd_dkv_pair_kernel<E>, tiles, dim3(512), 0, stream, p);
+    }
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk, dv)");
     if (p.split_dkv > 1) {
       const int64_t rows = (int64_t)p.Tk * p.Hk;
