@@ -93,11 +93,12 @@ constexpr int kPkOrderMax = 4096;  // slots of a list; longer calls have rounds 
 constexpr int kPkClasses = 128;
 
 // KEYS: tiles of bm keys that meet queries; else tiles of bm rows (token, head of g) that meet keys, the causal
-// ones counted from the sequence's end. order: [slots]; count: LDS, kPkClasses + 1 words. A wave takes 64
+// ones counted from the sequence's end. order: [slots]; count: LDS, kPkClasses + 1 words;
+// parts: how many workgroups share such a tile. A wave takes 64
 // sequences at a time.
-template <bool KEYS>
+template <bool KEYS, typename Parts>
 __device__ __forceinline__ void pk_order(const int32_t* cu, int T, const int32_t* cu_other, int T_other, int n, int g,
-                                         int bm, int causal, int slots, int2* order, uint32_t* count) {
+                                         int bm, int causal, int slots, int2* order, uint32_t* count, Parts&& parts) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto tiles = [&](auto&& take) {
     auto one = [&](int seq, int len, int other, int ntile, int t) {
@@ -108,7 +109,8 @@ __device__ __forceinline__ void pk_order(const int32_t* cu, int T, const int32_t
         const int last = (min((ntile - t) * bm, len * g) - 1) / g;
         work = ((causal ? min(last + other - len, other - 1) + 1 : other) + 63) >> 6;
       }
-      take(seq, t, work > 0 ? max(0, kPkClasses - 2 - (int)(8.f * flog2((float)work))) : kPkClasses - 1);
+      const float share = (float)work / (float)parts(work);
+      take(seq, t, work > 0 ? max(0, kPkClasses - 2 - (int)(8.f * flog2(fmaxf(share, 1.f)))) : kPkClasses - 1);
     };
     for (int i0 = 64 * wave; i0 < n + 2; i0 += 256) {
       const int i = i0 + lane;

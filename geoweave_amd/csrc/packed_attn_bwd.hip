@@ -50,9 +50,10 @@ struct PackedBwdParams {
   uint32_t* max_v;    // [n + 2][Hk] largest |v_j|
   int2* order_q;      // tiles of the dQ and of the dK/dV pass by falling work, or null
   int2* order_k;
-  int split_dq, split_dkv;  // parts that the passes' inner loops are cut into
-  float* part_dq;     // split_dq > 1: [part][Tq][H][D]
-  float* part_dkv;    // split_dkv > 1: [part][dk, dv][Tk][Hk][D]
+  int split_dq, split_dkv;  // parts at most that a workgroup's inner loop is cut into,
+  int per_dq, per_dkv;      // one for each so many tiles of 64
+  float* part_dq;     // cut rows: [part][Tq][H][D]
+  float* part_dkv;    // cut rows: [part][dk, dv][Tk][Hk][D]
   const int32_t* cu_q;
   const int32_t* cu_k;
   int n, Tq, Tk, H, Hk, G, causal;
@@ -66,6 +67,25 @@ constexpr int kBwdTile = 128;  // rows of a dQ workgroup, keys of a dK/dV workgr
 // Workgroup slots per key head of the two passes.
 __host__ __device__ inline int dq_slots(const PackedBwdParams& p) { return (int)((int64_t)p.Tq * p.G / kBwdTile) + p.n + 2; }
 __host__ __device__ inline int dkv_slots(const PackedBwdParams& p) { return p.Tk / kBwdTile + p.n + 2; }
+
+// Parts of a loop over `work` tiles of 64.
+__device__ __forceinline__ int pk_parts(int work, int split, int per) {
+  return split > 1 ? min(split, max(1, (work + per - 1) / per)) : 1;
+}
+// Tiles of 64 keys that block x (kBwdTile rows) of a sequence of len queries and lk keys meets.
+__device__ __forceinline__ int dq_work(const PackedBwdParams& p, int len, int lk, int x) {
+  const int last = (min((x + 1) * kBwdTile, len * p.G) - 1) / p.G;
+  const int keys = p.causal ? min(last + lk - len, lk - 1) + 1 : lk;
+  return keys > 0 ? (keys + 63) >> 6 : 0;
+}
+// First tile of 64 queries that meets block x (kBwdTile keys) of a sequence of len keys and lq queries, and how
+// many tiles do, those of all heads of the group.
+__device__ __forceinline__ int dkv_first(const PackedBwdParams& p, int len, int lq, int x) {
+  return p.causal ? max(0, x * kBwdTile - (len - lq)) >> 6 : 0;
+}
+__device__ __forceinline__ int dkv_work(const PackedBwdParams& p, int len, int lq, int x) {
+  return max(0, ((lq + 63) >> 6) - dkv_first(p, len, lq, x)) * p.G;  // fits: the host bounds Tq * H
+}
 
 // fp16: P enters its product times 2^14.
 template <typename E>
@@ -143,11 +163,13 @@ __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdPa
   constexpr int LPR = D / 8;
   __shared__ uint32_t top[kStatHeads > kPkClasses ? kStatHeads : kPkClasses + 1];
   if (blockIdx.x == 0) {
-    if (p.order_q) pk_order<false>(p.cu_q, p.Tq, p.cu_k, p.Tk, p.n, p.G, kBwdTile, p.causal, dq_slots(p), p.order_q, top);
+    if (p.order_q) pk_order<false>(p.cu_q, p.Tq, p.cu_k, p.Tk, p.n, p.G, kBwdTile, p.causal, dq_slots(p), p.order_q, top,
+                                   [&](int work) { return pk_parts(work, p.split_dq, p.per_dq); });
     return;
   }
   if (blockIdx.x == 1) {
-    if (p.order_k) pk_order<true>(p.cu_k, p.Tk, p.cu_q, p.Tq, p.n, 1, kBwdTile, p.causal, dkv_slots(p), p.order_k, top);
+    if (p.order_k) pk_order<true>(p.cu_k, p.Tk, p.cu_q, p.Tq, p.n, 1, kBwdTile, p.causal, dkv_slots(p), p.order_k, top,
+                                  [&](int work) { return pk_parts(work * p.G, p.split_dkv, p.per_dkv); });
     return;
   }
   const int block = blockIdx.x - 2;
@@ -209,14 +231,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int hk = blockIdx.x % p.Hk;
-  const PackedTile pt = pk_tile(p.order_q, p.cu_q, p.n, p.Tq, p.G, BM, blockIdx.x / p.Hk);
+  const int hk = blockIdx.x % p.Hk, part = blockIdx.x / p.Hk % p.split_dq;
+  const PackedTile pt = pk_tile(p.order_q, p.cu_q, p.n, p.Tq, p.G, BM, blockIdx.x / p.Hk / p.split_dq);
   const int rows = pt.len * p.G;
   const int ntile = (rows + BM - 1) / BM;
   if (pt.tile < 0 || pt.tile >= ntile) return;
   const int row0 = (p.causal ? ntile - 1 - pt.tile : pt.tile) * BM;
   int k0, lk;
   pk_other(p.cu_k, p.n, p.Tk, pt.seq, k0, lk);
+  const int all = dq_work(p, pt.len, lk, row0 / BM), parts = pk_parts(all, p.split_dq, p.per_dq);
+  if (part >= parts) return;
   const int shift = lk - pt.len;
   const float sl2 = p.scale_log2;
 
@@ -255,11 +279,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   const float unscale = lim == 0 ? 0.f : ldexpf(p.scale, -e);
   auto last_key = [&](int r) { return p.causal ? min(min(r, rows - 1) / p.G + shift, lk - 1) : lk - 1; };
   const int lim_wave = base < rows ? last_key(base + 31) : -1;
-  const int keys = last_key(row0 + BM - 1) + 1;
   // This part's tiles of 64 keys.
-  const int all = keys > 0 ? (keys + 63) >> 6 : 0;
-  const int per = p.split_dq > 1 ? (all + p.split_dq - 1) / p.split_dq : all;
-  const int tk0 = min((int)blockIdx.y * per, all), ntk = min(per, all - tk0);
+  const int per = (all + parts - 1) / parts;
+  const int tk0 = min(part * per, all), ntk = min(per, all - tk0);
 
   f32x16 acc[DB];
 #pragma unroll
@@ -343,8 +365,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
       pk_tile_barrier();
     });
   }
-  if (p.split_dq > 1) {
-    float* dst = p.part_dq + (((int64_t)blockIdx.y * p.Tq + t) * p.H + head) * D;
+  if (parts > 1) {
+    float* dst = p.part_dq + (((int64_t)part * p.Tq + t) * p.H + head) * D;
 #pragma unroll
     for (int db = 0; db < DB; ++db) pk_store_part(dst + 32 * db, acc[db], unscale, half, on);
     return;
@@ -371,12 +393,14 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int hk = blockIdx.x % p.Hk;
-  const PackedTile pt = pk_tile(p.order_k, p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk);
+  const int hk = blockIdx.x % p.Hk, part = blockIdx.x / p.Hk % p.split_dkv;
+  const PackedTile pt = pk_tile(p.order_k, p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk / p.split_dkv);
   const int key0 = pt.tile * BN;
   if (key0 < 0 || key0 >= pt.len) return;
   int q0, lq;
   pk_other(p.cu_q, p.n, p.Tq, pt.seq, q0, lq);
+  const int all = dkv_work(p, pt.len, lq, pt.tile), parts = pk_parts(all, p.split_dkv, p.per_dkv);
+  if (part >= parts) return;
   const int shift = pt.len - lq;  // causal: key j is seen by tokens i >= j - shift
   const float sl2 = p.scale_log2;
   const int wkey = key0 + wave * 32;
@@ -410,14 +434,11 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
 #pragma unroll
     for (int r = 0; r < 16; ++r) ak[db][r] = av[db][r] = 0.f;
 
-  const int first = p.causal ? max(0, key0 - shift) >> 6 : 0;  // first tile with a query that sees a key
+  const int first = dkv_first(p, pt.len, lq, pt.tile);  // first tile with a query that sees a key
   const int ntq = (lq + 63) >> 6;
   const int per = ntq > first ? ntq - first : 0;
   // This part's tiles, head by head of the group.
-  const int64_t all = (int64_t)per * p.G;
-  const int64_t share = p.split_dkv > 1 ? (all + p.split_dkv - 1) / p.split_dkv : all;
-  const int64_t t0 = min((int64_t)blockIdx.y * share, all);
-  const int total = (int)min(share, all - t0);
+  const int share = (all + parts - 1) / parts, t0 = min(part * share, all), total = min(share, all - t0);
 
   PkRows<D, 256> qrows, grows;
   const uint16_t* qbase = p.q + (int64_t)q0 * p.qst + (int64_t)hk * p.G * p.qsh;
@@ -426,8 +447,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
   qrows.init(qbase, p.qst, lq, tid);
   grows.init(gbase, p.gst, lq, tid);
   // The tile that is loaded next: head of the group and tile of its queries.
-  int ld_h = per > 0 ? (int)(t0 / per) : 0;
-  int ld_t = first + (int)(t0 - (int64_t)ld_h * per);
+  int ld_h = per > 0 ? t0 / per : 0;
+  int ld_t = first + t0 - ld_h * per;
   auto load = [&](uint8_t* qd, uint8_t* gd, float* ld, float* dd) __attribute__((always_inline)) {
     qrows.base = uniform_ptr(reinterpret_cast<const char*>(qbase + (int64_t)ld_h * p.qsh));
     grows.base = uniform_ptr(reinterpret_cast<const char*>(gbase + (int64_t)ld_h * p.gsh));
@@ -532,7 +553,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
   if (total > 0) {
     load(qt0, gt0, nl0, nd0);
     pk_tile_barrier();
-    int cur = first + (int)(t0 % per);  // the tile that is computed
+    int cur = first + t0 % per;  // the tile that is computed
     // Queries of tiles from `full` on see every key of the workgroup's block.
     const int full = p.causal ? (key0 + BN - 1 - shift + 63) >> 6 : first;
     auto tile = [&](auto buf) __attribute__((always_inline)) {
@@ -560,8 +581,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
     }
     if (n < total) tile(PkInt<0>{});
     if (__builtin_expect(unclean, 0)) {
-      for (int64_t x = t0; x < t0 + total; ++x) {
-        const int h = (int)(x / per), i0 = 64 * (first + (int)(x % per));
+      for (int x = t0; x < t0 + total; ++x) {
+        const int h = x / per, i0 = 64 * (first + x % per);
         for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i)
           pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, av);
       }
@@ -571,13 +592,13 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
   const float fk = pt.len == 1 ? 0.f : kFp16 ? ldexpf(p.scale, -e) : p.scale;
   const float fv = kFp16 ? ldexpf(1.f, -14) : 1.f;
   const int64_t t = pt.start + (on ? key : 0);
-  if (p.split_dkv > 1) {
-    const int64_t part = (int64_t)p.Tk * p.Hk * D;
-    float* dst = p.part_dkv + 2 * blockIdx.y * part + (t * p.Hk + hk) * D;
+  if (parts > 1) {
+    const int64_t step = (int64_t)p.Tk * p.Hk * D;
+    float* dst = p.part_dkv + 2 * part * step + (t * p.Hk + hk) * D;
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
       pk_store_part(dst + 32 * db, ak[db], fk, half, on);
-      pk_store_part(dst + part + 32 * db, av[db], fv, half, on);
+      pk_store_part(dst + step + 32 * db, av[db], fv, half, on);
     }
     return;
   }
@@ -608,12 +629,14 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave & 3;
   const int col = lane & 31, half = lane >> 5;
-  const int hk = blockIdx.x % p.Hk;
-  const PackedTile pt = pk_tile(p.order_k, p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk);
+  const int hk = blockIdx.x % p.Hk, part = blockIdx.x / p.Hk % p.split_dkv;
+  const PackedTile pt = pk_tile(p.order_k, p.cu_k, p.n, p.Tk, 1, BN, blockIdx.x / p.Hk / p.split_dkv);
   const int key0 = pt.tile * BN;
   if (key0 < 0 || key0 >= pt.len) return;
   int q0, lq;
   pk_other(p.cu_q, p.n, p.Tq, pt.seq, q0, lq);
+  const int all = dkv_work(p, pt.len, lq, pt.tile), parts = pk_parts(all, p.split_dkv, p.per_dkv);
+  if (part >= parts) return;
   const int shift = pt.len - lq;  // causal: key j is seen by tokens i >= j - shift
   const float sl2 = p.scale_log2;
   const int wkey = key0 + kw * 32;
@@ -627,13 +650,11 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
   }
   const float dscale = kFp16 ? ldexpf(1.f, e - 14) : 1.f;
 
-  const int first = p.causal ? max(0, key0 - shift) >> 6 : 0;  // first tile with a query that sees a key
+  const int first = dkv_first(p, pt.len, lq, pt.tile);  // first tile with a query that sees a key
   const int ntq = (lq + 63) >> 6;
   const int per = ntq > first ? ntq - first : 0;
-  const int64_t all = (int64_t)per * p.G;
-  const int64_t share = p.split_dkv > 1 ? (all + p.split_dkv - 1) / p.split_dkv : all;
-  const int64_t t0 = min((int64_t)blockIdx.y * share, all);
-  const int total = (int)min(share, all - t0);
+  // This part's tiles, head by head of the group.
+  const int share = (all + parts - 1) / parts, t0 = min(part * share, all), total = min(share, all - t0);
 
   PkRows<D, 512> qrows, grows;
   const uint16_t* qbase = p.q + (int64_t)q0 * p.qst + (int64_t)hk * p.G * p.qsh;
@@ -641,8 +662,8 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
   const int64_t sbase = (int64_t)hk * p.G * p.Tq + q0;
   qrows.init(qbase, p.qst, lq, tid);
   grows.init(gbase, p.gst, lq, tid);
-  int ld_h = per > 0 ? (int)(t0 / per) : 0;
-  int ld_t = first + (int)(t0 - (int64_t)ld_h * per);
+  int ld_h = per > 0 ? t0 / per : 0;
+  int ld_t = first + t0 - ld_h * per;
   auto load = [&](uint8_t* qd, uint8_t* gd, float* ld, float* dd) __attribute__((always_inline)) {
     qrows.base = uniform_ptr(reinterpret_cast<const char*>(qbase + (int64_t)ld_h * p.qsh));
     grows.base = uniform_ptr(reinterpret_cast<const char*>(gbase + (int64_t)ld_h * p.gsh));
@@ -766,7 +787,7 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
       }
     };
 
-    int cur = per > 0 ? first + (int)(t0 % per) : 0;  // the tile that is computed
+    int cur = per > 0 ? first + t0 % per : 0;  // the tile that is computed
     // Queries of tiles from `full` on see every key of the workgroup's block.
     const int full = p.causal ? (key0 + BN - 1 - shift + 63) >> 6 : first;
     auto tile = [&](auto buf) __attribute__((always_inline)) {
@@ -791,8 +812,8 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
     }
     if (n < total) tile(PkInt<0>{});
     if (__builtin_expect(unclean, 0)) {
-      for (int64_t x = t0; x < t0 + total; ++x) {
-        const int h = (int)(x / per), i0 = 64 * (first + (int)(x % per));
+      for (int x = t0; x < t0 + total; ++x) {
+        const int h = x / per, i0 = 64 * (first + x % per);
         for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i)
           pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, acc);
       }
@@ -800,9 +821,8 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
     // Rows of a sequence of one key all have dS = 0.
     const float f = B ? (pt.len == 1 ? 0.f : kFp16 ? ldexpf(p.scale, -e) : p.scale) : kFp16 ? ldexpf(1.f, -14) : 1.f;
     const int64_t t = pt.start + (on ? key : 0);
-    if (p.split_dkv > 1) {
-      const int64_t part = (int64_t)p.Tk * p.Hk * D;
-      float* dst = p.part_dkv + (2 * blockIdx.y + (B ? 0 : 1)) * part + (t * p.Hk + hk) * D;
+    if (parts > 1) {
+      float* dst = p.part_dkv + ((2 * part + (B ? 0 : 1)) * (int64_t)p.Tk + t) * p.Hk * D + (int64_t)hk * D;
 #pragma unroll
       for (int db = 0; db < DB; ++db) pk_store_part(dst + 32 * db, acc[db], f, half, on);
       return;
@@ -822,15 +842,28 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
     role(PkInt<1>{});
 }
 
-// Sums the parts of a gradient [T, H, D], in order: part i at src + i * step.
-template <typename E, int D>
-__global__ __launch_bounds__(256) void packed_bwd_join_kernel(const float* __restrict__ src, int64_t step, int parts,
-                                                              int64_t rows, int H, uint16_t* __restrict__ dst,
-                                                              int64_t st, int64_t sh) {
+// Sums the parts of the rows that were cut, in order. KEYS: dk (blockIdx.y = 0) and dv; else dq.
+template <typename E, int D, bool KEYS>
+__global__ __launch_bounds__(256) void packed_bwd_join_kernel(const PackedBwdParams p) {
   constexpr int LPR = D / 4;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int H = KEYS ? p.Hk : p.H, T = KEYS ? p.Tk : p.Tq;
+  const int64_t rows = (int64_t)T * H, row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int c = threadIdx.x % LPR;
   if (row >= rows) return;
+  const int t = (int)(row / H), h = (int)(row - (int64_t)t * H);
+  const PackedTile pt = pk_token(KEYS ? p.cu_k : p.cu_q, p.n, T, t);
+  int other = 0;
+  if (pt.seq >= 1 && pt.seq <= p.n) {
+    const int32_t* cu = KEYS ? p.cu_q : p.cu_k;
+    const int To = KEYS ? p.Tq : p.Tk;
+    other = max(0, pk_bound(cu, p.n, To, pt.seq + 1) - pk_bound(cu, p.n, To, pt.seq));
+  }
+  const int at = t - pt.start;
+  const int parts = KEYS ? pk_parts(dkv_work(p, pt.len, other, at / kBwdTile), p.split_dkv, p.per_dkv)
+                         : pk_parts(dq_work(p, pt.len, other, (at * p.G + h % p.G) / kBwdTile), p.split_dq, p.per_dq);
+  if (parts == 1) return;
+  const float* src = KEYS ? p.part_dkv + blockIdx.y * rows * D : p.part_dq;
+  const int64_t step = (KEYS ? 2 : 1) * rows * D;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int i = 0; i < parts; ++i) {
@@ -840,27 +873,35 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(const float* __res
     s.z += x.z;
     s.w += x.w;
   }
-  const int64_t t = row / H;
-  *reinterpret_cast<uint2*>(dst + t * st + (row - t * H) * sh + 4 * c) =
-      make_uint2(pack_pair(E{}, s.x, s.y), pack_pair(E{}, s.z, s.w));
+  uint16_t* dst = !KEYS            ? p.dq + (int64_t)t * p.dqst + (int64_t)h * p.dqsh
+                  : blockIdx.y == 0 ? p.dk + (int64_t)t * p.dkst + (int64_t)h * p.dksh
+                                    : p.dv + (int64_t)t * p.dvst + (int64_t)h * p.dvsh;
+  *reinterpret_cast<uint2*>(dst + 4 * c) = make_uint2(pack_pair(E{}, s.x, s.y), pack_pair(E{}, s.z, s.w));
 }
 
-// Parts that the keys of the dQ pass and the queries of the dK/dV pass are cut into, where the tiles
-// alone leave workgroup slots empty (two per CU), from the sizes that the host knows; a part has at
-// least 512 keys or queries on average. The parts' fp32 sums are joined in order by another launch.
+// Parts that the keys of a dQ workgroup and the queries of a dK/dV workgroup are cut into, where the tiles
+// alone leave workgroup slots empty, or where one long sequence among short ones would run on by itself: at
+// most `dq`, one for every `per_dq` tiles of 64, which the kernels find from the lengths. The fewer workgroups there
+// are, the shorter the parts: 8 to 64 tiles. The parts' fp32 sums are joined in order by another launch; their
+// workspace stays below 512 MiB a pass. 37 causal sequences of 1 to 3,151 tokens, 8 heads over 2: forward and
+// backward 381 us with as many parts for every sequence, 249 so; 4 heads, 2 sequences of 3,000 to 6,000: 298, 282.
 struct BwdPlan {
-  int dq, dkv;
+  int dq, dkv, per_dq, per_dkv;
   int64_t slots_q, slots_k;  // entries of the lists of tiles (0: no list)
   size_t dq_bytes, dkv_bytes;
 };
 
 BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
-  const int64_t G = Hq / Hk, seqs = n > 0 ? n : 1;
-  auto parts = [&](int64_t rows, int64_t other) {
+  const int64_t G = Hq / Hk;
+  // rows: of the workgroups' own side; other: of the loops'; bytes: of a part; slots: workgroups at once.
+  auto parts = [&](int64_t rows, int64_t other, int64_t bytes, int64_t slots, int& per) {
     // Tiles: at least one per sequence that has rows, and the last one of a sequence half full.
     const int64_t wgs = (rows / 128 + (rows < 128 * n ? n : n / 2) + 1) * Hk;
-    int64_t s = 512 / (wgs > 0 ? wgs : 1);
-    if (s > other / seqs / 512) s = other / seqs / 512;
+    per = (int)(wgs * 64 / slots < 8 ? 8 : wgs * 64 / slots > 64 ? 64 : wgs * 64 / slots);
+    if (other / (n > 0 ? n : 1) / 16 < per) return 1;  // four times the average is no part
+    int64_t s = 2 * slots / wgs;
+    if (s > (other / 64 + per) / per) s = (other / 64 + per) / per;
+    if (s > (512ll << 20) / bytes) s = (512ll << 20) / bytes;
     return (int)(s > 16 ? 16 : s > 1 ? s : 1);
   };
   BwdPlan b = {};
@@ -869,10 +910,11 @@ BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
   b.slots_k = Tk / kBwdTile + n + 2;
   if (n < 2 || Tq == 0 || b.slots_q > kPkOrderMax) b.slots_q = 0;
   if (n < 2 || Tq == 0 || b.slots_k > kPkOrderMax) b.slots_k = 0;
-  b.dq = parts(Tq * G, Tk);
-  b.dkv = parts(Tk, Tq * G);
-  b.dq_bytes = b.dq > 1 ? (size_t)b.dq * Tq * Hq * D * sizeof(float) : 0;
-  b.dkv_bytes = b.dkv > 1 ? (size_t)b.dkv * 2 * Tk * Hk * D * sizeof(float) : 0;
+  const int64_t dq_part = Tq * Hq * D * 4, dkv_part = 2 * Tk * Hk * D * 4;
+  b.dq = parts(Tq * G, Tk, dq_part > 0 ? dq_part : 1, D == 64 ? 768 : 512, b.per_dq);
+  b.dkv = parts(Tk, Tq * G, dkv_part > 0 ? dkv_part : 1, D == 64 ? 512 : 256, b.per_dkv);
+  b.dq_bytes = b.dq > 1 ? (size_t)b.dq * dq_part : 0;
+  b.dkv_bytes = b.dkv > 1 ? (size_t)b.dkv * dkv_part : 0;
   return b;
 }
 
@@ -880,7 +922,7 @@ template <typename E, int D>
 int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
   constexpr bool kFp16 = __is_same(E, FP16);
   const int64_t qslots = dq_slots(p), kslots = dkv_slots(p);
-  GW_CHECK_ARG(qslots * p.Hk < (1ll << 31) && kslots * p.Hk < (1ll << 31), "the grid is too large");
+  GW_CHECK_ARG(qslots * p.Hk * p.split_dq < (1ll << 31) && kslots * p.Hk * p.split_dkv < (1ll << 31), "the grid is too large");
   if (kFp16) {
     const int64_t words = 2 * (int64_t)(p.n + 2) * p.Hk;  // max_do and max_v, one behind the other
     hipLaunchKernelGGL(packed_bwd_clear_kernel, dim3((uint32_t)((words + 255) / 256 > 1024 ? 1024 : (words + 255) / 256)),
@@ -892,17 +934,16 @@ int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D, kFp16>), dim3(2u + stat_q + stat_k), dim3(256), 0, stream, p,
                        stat_q);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (rows)");
-    hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)(qslots * p.Hk), p.split_dq), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)(qslots * p.Hk * p.split_dq)), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq)");
     if (p.split_dq > 1) {
-      const int64_t rows = (int64_t)p.Tq * p.H;
-      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D>), dim3((uint32_t)((rows * (D / 4) + 255) / 256)), dim3(256), 0, stream,
-                         p.part_dq, rows * D, p.split_dq, rows, p.H, p.dq, p.dqst, p.dqsh);
+      const int64_t threads = (int64_t)p.Tq * p.H * (D / 4);
+      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D, false>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, stream, p);
       GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq join)");
     }
   }
   if (p.Tk > 0) {
-    const dim3 tiles((uint32_t)(kslots * p.Hk), p.split_dkv);
+    const dim3 tiles((uint32_t)(kslots * p.Hk * p.split_dkv));
     if constexpr (D == 64) {
       hipLaunchKernelGGL(packed_bwd_dkv_kernel<E>, tiles, dim3(256), 0, stream, p);
     } else {
@@ -910,14 +951,9 @@ int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
     }
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk, dv)");
     if (p.split_dkv > 1) {
-      const int64_t rows = (int64_t)p.Tk * p.Hk;
-      const dim3 grid((uint32_t)((rows * (D / 4) + 255) / 256));
-      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D>), grid, dim3(256), 0, stream, p.part_dkv, 2 * rows * D, p.split_dkv,
-                         rows, p.Hk, p.dk, p.dkst, p.dksh);
-      GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk join)");
-      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D>), grid, dim3(256), 0, stream, p.part_dkv + rows * D, 2 * rows * D,
-                         p.split_dkv, rows, p.Hk, p.dv, p.dvst, p.dvsh);
-      GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dv join)");
+      const int64_t threads = (int64_t)p.Tk * p.Hk * (D / 4);
+      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D, true>), dim3((uint32_t)((threads + 255) / 256), 2), dim3(256), 0, stream, p);
+      GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk, dv join)");
     }
   }
   return GW_OK;
@@ -983,6 +1019,8 @@ extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_str
   const BwdPlan b = packed_bwd_plan(n, Tq, Tk, Hq, Hk, D);
   p.split_dq = b.dq;
   p.split_dkv = b.dkv;
+  p.per_dq = b.per_dq;
+  p.per_dkv = b.per_dkv;
   p.part_dq = reinterpret_cast<float*>(ws + pk_align((size_t)Tq * Hq * 8) + pk_align((size_t)(n + 2) * Hk * 8));
   p.part_dkv = p.part_dq + pk_align(b.dq_bytes) / sizeof(float);
   int2* lists = reinterpret_cast<int2*>(p.part_dkv + pk_align(b.dkv_bytes) / sizeof(float));
