@@ -103,6 +103,20 @@ def test_forward_and_gradients(gpu_device, dtype, d, hq, hk, causal, lens):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_one_long_sequence_among_short_ones(gpu_device, dtype, d, causal):
+    """The long one's loops are cut into parts, the others' are not."""
+    args = make([3, 1500, 40, 0, 17, 1], None, 6, 1, d, dtype, seed=4)
+    q, k, v, do, cu_q, cu_k = args
+    got = step(args, gpu_device, causal)
+    ref = packed_attention(q, k, v, cu_q, cu_k, causal, do=do)
+    for name, x in zip(("o", "dq", "dk", "dv"), got):
+        check(x, ref, name, dtype, d)
+    assert all(torch.equal(a, b) for a, b in zip(got, step(args, gpu_device, causal))), "the same bits again"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_long_rows_with_rising_scores(gpu_device, dtype):
     """Scores that grow along the keys move the running reference many times."""
     args = list(make([40, 7], [2100, 3], 2, 1, 64, dtype, 3))

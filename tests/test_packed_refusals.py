@@ -242,3 +242,13 @@ def test_workspaces_are_bounded_by_the_sizes():
             assert fwd <= 1 << 29, (n, tq, tk, hq, hk, d, fwd)
     assert lib.gw_paged_attn_fwd_workspace_size(64, 1, 32, 8, 128) <= 1 << 26
     assert lib.gw_paged_attn_fwd_workspace_size(8192, 1, 32, 8, 128) == 0  # no split
+
+
+def test_backward_workspaces_are_bounded_by_the_sizes():
+    """Beside 8 bytes per (token, head) and per (sequence, key head), the parts stay below 512 MiB a pass."""
+    lib = _lib.load()
+    for n, tq, tk in ((1, 1, 1 << 24), (1, 40, 1 << 24), (1, 1374, 1 << 20), (8, 200000, 40), (1, 1 << 22, 1 << 22),
+                      (200, 30000, 30000), (1, 8000, 8000)):
+        for hq, hk, d in ((16, 16, 64), (32, 1, 128), (2, 1, 64)):
+            got = lib.gw_packed_attn_bwd_workspace_size(n, tq, tk, hq, hk, d)
+            assert got <= 8 * tq * hq + 8 * (n + 2) * hk + (1 << 30) + (1 << 17), (n, tq, tk, hq, hk, d, got)
