@@ -323,6 +323,17 @@ __device__ __forceinline__ void pk_tiles(int ntk, int nfull, F&& tile) {
   if (n < ntk) tile(PkInt<1>{}, PkInt<0>{}, n);
 }
 
+// A running reference m of the softmax: weights are 2^(s - m), rounded to the 16-bit type for the second
+// product. fp16's smallest step is 2^-24, so with the largest score as the reference what lies 25 octaves below it
+// would be 0 in the product while the sum keeps it (43,968 keys that far below one with v = 0: o = 0 for
+// 1.2e-3). Its reference lies 10 octaves below the largest score: a weight keeps all its bits down to 2^-24 of the
+// largest, and a smaller one is off by at most 2^-35 of the largest. bf16 has the exponents of fp32. A lane whose
+// weights of a step (8 or 16) sum past the cap raises m, so no weight leaves fp16's range.
+template <typename E>
+constexpr float kPkBelow = __is_same(E, FP16) ? 10.f : 0.f;
+template <typename E>
+constexpr float kPkSumCap = __is_same(E, FP16) ? 60000.f : 32768.f;
+
 // inf and NaN in places that a row does not see. A masked weight is 0, but 0 * inf is NaN: in tiles
 // that some rows see only in part, inf and NaN among the second operand's entries are cleared before the
 // product, and once it is known that there were any (never, in healthy data), a pass over those tiles

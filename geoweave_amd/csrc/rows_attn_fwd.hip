@@ -33,7 +33,6 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kRows = 16;
 constexpr int kRowsPart = 256;       // a part is a multiple of this many keys (4 waves x 32, twice)
-constexpr float kRowsSumCap = 32768.f;
 
 __device__ __forceinline__ f32x4 mma16(BF16, uint4 a, uint4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -334,10 +333,10 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
       return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     };
     float ls = weights(-m);
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= kRowsSumCap)) != 0ull, 0)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= kPkSumCap<E>)) != 0ull, 0)) {
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      const float mn = fmaxf(m, rows_max(mx) * p.scale_log2);
+      const float mn = fmaxf(m, rows_max(mx) * p.scale_log2 - kPkBelow<E>);
       const float alpha = fexp2(m - mn);
       m = mn;
       l *= alpha;
