@@ -14,10 +14,11 @@
 // reads of the same LDS tiles.
 //
 // P and dS enter their products in the inputs' 16-bit type (half a step of each entry). fp16 has few
-// exponents for them: P is scaled by 2^14; dS in the dQ pass by a power of two per row, from the row's
-// |do| and the sequence's largest |v| (|dP - delta| <= 2 |do_i| max_j |v_j|), in the dK/dV pass by one per
-// sequence and key head, so that |dS| stays below 2^15. The powers are exact and taken out of the fp32
-// sums again.
+// exponents for them: P is scaled by 2^14, dS by a power of two of the lane's row (dQ) or key (dK) that follows the
+// largest entry as it comes (PkFit), so that an entry keeps all its bits down to 2^-23 of the largest and no
+// row or key depends on what it does not meet. (One power per sequence from the largest |do| and |v|: a row with 2^12
+// times the others' dO beside a key with 2^6 times the others' v left the dK of the keys behind it 5 times their bound
+// off.) The powers are exact and taken out of the fp32 sums again.
 //
 // Bound as the forward is, by the matrix cores and the vector unit: six sequences of 3,013 to 4,795 tokens,
 // 16 heads of 64 in bf16, dQ 552 us (1.01 PFLOP/s, matrix cores busy 60 % of the time), dK/dV 790 us (0.95, 54 %),
@@ -46,8 +47,6 @@ struct PackedBwdParams {
   float* nlse;        // [H][Tq] -lse / scale (fp16: + 14 / (scale log2 e)), -inf for a row without keys: the
                       // products' start of S - lse / scale
   float* ndelta;      // [H][Tq] -delta
-  uint32_t* max_do;   // [n + 2][Hk] largest |do_i| of a sequence's rows, as float bits (fp16 only)
-  uint32_t* max_v;    // [n + 2][Hk] largest |v_j|
   int2* order_q;      // tiles of the dQ and of the dK/dV pass by falling work, or null
   int2* order_k;
   int split_dq, split_dkv;  // parts at most that a workgroup's inner loop is cut into,
@@ -91,77 +90,48 @@ __device__ __forceinline__ int dkv_work(const PackedBwdParams& p, int len, int l
 template <typename E>
 constexpr float kPScale = __is_same(E, FP16) ? 14.f : 0.f;
 
-// Exponent e with 2 bound 2^e <= 2^15 (0 where there is no bound to speak of).
-__device__ __forceinline__ int pk_scale_exp(float bound) {
-  if (!(bound > 0.f) || !(bound < INFINITY)) return 0;
-  int x;
-  (void)frexpf(bound, &x);  // bound < 2^x
-  return min(max(14 - x, -100), 100);
-}
-
-__global__ __launch_bounds__(256) void packed_bwd_clear_kernel(uint32_t* a, int64_t n) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) a[i] = 0u;
-}
-
-// Statistics of 256 / (D / 8) rows at a time: D / 8 lanes per (token, head) row. MAXIMA: also the
-// sequences' largest row norms (the maximum does not depend on the order of the atomics; rows that
-// are not finite have no part in it, their gradients are not finite whatever the scale): the largest of
-// the workgroup's rows per key head in LDS, then one atomic where that raises the value (an atomic per
-// row took 1.6 ms for 22,953 tokens x 16 heads).
-constexpr int kStatTokens = 16;
-constexpr int kStatHeads = 128;  // key heads with an LDS word; further ones go to memory at once
-
-struct PkMaxima {
-  uint32_t* lds;
-  uint32_t* out;  // of the sequence
-  int Hk;
-  __device__ __forceinline__ void init() {
-    for (int i = threadIdx.x; i < min(Hk, kStatHeads); i += 256) lds[i] = 0u;
-    __syncthreads();
-  }
-  __device__ __forceinline__ void row(int head, float norm2) {
-    if (!(norm2 < INFINITY)) return;
-    const uint32_t x = __float_as_uint(sqrtf(norm2));
-    if (head < kStatHeads)
-      atomicMax(lds + head, x);
-    else
-      atomicMax(out + head, x);
-  }
-  __device__ __forceinline__ void finish() {
-    __syncthreads();
-    for (int i = threadIdx.x; i < min(Hk, kStatHeads); i += 256)
-      if (lds[i] > __atomic_load_n(out + i, __ATOMIC_RELAXED)) atomicMax(out + i, lds[i]);
+// fp16: dS of a lane's row or key enters its product times 2^e. An entry that would pass 2^15 lowers e to where the
+// largest of the step lies in [2^9, 2^10), and the lane's sums follow (lanes l and l ^ 32 hold the same row or
+// key and sum into each other's accumulators: e is the same in both). The start is above what any entry but 0 allows
+// (2^60 times the smallest product of two fp16 values, 2^-48), and within fp32 for the largest, 2^40. inf and
+// NaN leave e as it is.
+constexpr int kFitStart = 60;
+struct PkFit {
+  int e = kFitStart;
+  // ds: all entries times 2^e of which none has entered its product yet. The power that was taken out, 2^-x
+  // (x = 0 nearly always).
+  template <int N, int DB>
+  __device__ __forceinline__ int fit(float (&ds)[N], f32x16 (&acc)[DB]) {
+    float mx = fabsf(ds[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, fabsf(ds[i]));
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > 32768.f) == 0ull, 1)) return 0;
+    mx = pair_max(mx);
+    int x = 0;
+    if (mx > 32768.f && mx < INFINITY) {
+      (void)frexpf(mx, &x);  // mx < 2^x
+      x -= 10;
+    }
+    const float f = ldexpf(1.f, -x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) ds[i] *= f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] *= f;
+    e -= x;
+    return x;
   }
 };
 
-template <typename E, int D>
-__device__ __forceinline__ void pk_largest_v(const PackedBwdParams& p, int slot, uint32_t* top) {
-  constexpr int LPR = D / 8;
-  const PackedTile pt = pk_find_tile(p.cu_k, p.n, p.Tk, 1, kStatTokens, slot);
-  const int t0 = pt.tile * kStatTokens;
-  if (t0 >= pt.len) return;
-  const int rows = min(kStatTokens, pt.len - t0) * p.Hk;
-  const int li = threadIdx.x % LPR;
-  PkMaxima maxima = {top, p.max_v + (int64_t)pt.seq * p.Hk, p.Hk};
-  maxima.init();
-  for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
-    const int t = pt.start + t0 + r / p.Hk, h = r % p.Hk;
-    float a[8], nn = 0.f;
-    unpack8<E>(*reinterpret_cast<const uint4*>(p.v + (int64_t)t * p.vst + (int64_t)h * p.vsh + li * 8), a);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) nn = fmaf(a[i], a[i], nn);
-    nn = group_sum<LPR>(nn);
-    if (li == 0) maxima.row(h, nn);
-  }
-  maxima.finish();
-}
+// Statistics of 256 / (D / 8) rows at a time: D / 8 lanes per (token, head) row.
+constexpr int kStatTokens = 16;
 
-// Workgroups 0 and 1 form the lists of the two passes' tiles, the next qslots take query rows, the others
-// (MAXIMA) rows of V.
-template <typename E, int D, bool MAXIMA>
-__global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdParams p, int qslots) {
+// Workgroups 0 and 1 form the lists of the two passes' tiles, the others take query rows.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdParams p) {
   constexpr int LPR = D / 8;
-  __shared__ uint32_t top[kStatHeads > kPkClasses ? kStatHeads : kPkClasses + 1];
+  __shared__ uint32_t top[kPkClasses + 1];
   if (blockIdx.x == 0) {
     if (p.order_q) pk_order<false>(p.cu_q, p.Tq, p.cu_k, p.Tk, p.n, p.G, kBwdTile, p.causal, dq_slots(p), p.order_q, top,
                                    [&](int work) { return pk_parts(work, p.split_dq, p.per_dq); });
@@ -172,41 +142,28 @@ __global__ __launch_bounds__(256) void packed_bwd_stats_kernel(const PackedBwdPa
                                   [&](int work) { return pk_parts(work * p.G, p.split_dkv, p.per_dkv); });
     return;
   }
-  const int block = blockIdx.x - 2;
-  if (MAXIMA && block >= qslots) {
-    pk_largest_v<E, D>(p, block - qslots, top);
-    return;
-  }
-  const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, 1, kStatTokens, block);
+  const PackedTile pt = pk_find_tile(p.cu_q, p.n, p.Tq, 1, kStatTokens, blockIdx.x - 2);
   const int t0 = pt.tile * kStatTokens;
   if (t0 >= pt.len) return;
   const int rows = min(kStatTokens, pt.len - t0) * p.H;
   const int li = threadIdx.x % LPR;
-  PkMaxima maxima = {top, p.max_do + (int64_t)pt.seq * p.Hk, p.Hk};
-  if (MAXIMA) maxima.init();
   for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
     const int t = pt.start + t0 + r / p.H, h = r % p.H;
     float a[8], b[8], c[8];
     unpack8<E>(*reinterpret_cast<const uint4*>(p.o + (int64_t)t * p.ost + (int64_t)h * p.osh + li * 8), a);
     unpack8<E>(*reinterpret_cast<const uint4*>(p.rest + ((int64_t)t * p.H + h) * D + li * 8), c);
     unpack8<E>(*reinterpret_cast<const uint4*>(p.dout + (int64_t)t * p.gst + (int64_t)h * p.gsh + li * 8), b);
-    float s = 0.f, nn = 0.f;
+    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s = fmaf(a[i] + c[i], b[i], s);
-      nn = fmaf(b[i], b[i], nn);
-    }
+    for (int i = 0; i < 8; ++i) s = fmaf(a[i] + c[i], b[i], s);
     s = group_sum<LPR>(s);
-    if (MAXIMA) nn = group_sum<LPR>(nn);
     if (li == 0) {
       const float l = p.lse[(int64_t)t * p.H + h];
       const int64_t at = (int64_t)h * p.Tq + t;
       p.nlse[at] = l == -INFINITY ? -INFINITY : (kPScale<E> - l * kDLog2e) / p.scale_log2;
       p.ndelta[at] = -s;
-      if (MAXIMA) maxima.row(h / p.G, nn);
     }
   }
-  if (MAXIMA) maxima.finish();
 }
 
 // The same column in fp32.
@@ -251,7 +208,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   const int lim = p.causal ? min(tok + shift, lk - 1) : lk - 1;
   const int64_t t = pt.start + tok;
   uint4 qa[KS], ga[KS];
-  float nn = 0.f;
   {
     const uint16_t* qr = p.q + t * p.qst + (int64_t)head * p.qsh + half * 8;
     const uint16_t* gr = p.dout + t * p.gst + (int64_t)head * p.gsh + half * 8;
@@ -259,13 +215,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
     for (int ks = 0; ks < KS; ++ks) {
       qa[ks] = *reinterpret_cast<const uint4*>(qr + ks * 16);
       ga[ks] = *reinterpret_cast<const uint4*>(gr + ks * 16);
-      if (kFp16) nn += dot8<E>(ga[ks], ga[ks]);
     }
   }
-  int e = 0;
-  if (kFp16) e = pk_scale_exp(sqrtf(pair_sum(nn)) * __uint_as_float(p.max_v[(int64_t)pt.seq * p.Hk + hk]));
+  PkFit fit;
   const int64_t srow = (int64_t)head * p.Tq + t;
-  const float nlse = p.nlse[srow] * sl2 - kPScale<E> + (float)e;  // p 2^e = 2^(s - lse + e)
+  float nlse = p.nlse[srow] * sl2;  // fp16: p 2^e = 2^(s - lse + e)
+  if (kFp16) nlse += (float)kFitStart - kPScale<E>;
   // dP - delta: at D = 128 delta is where the products start, in a register block of its own; at D = 64,
   // where three waves share a SIMD's registers, it is added afterwards (with the block 124 bytes of
   // scratch a lane and 860 us for 563 on 6 scenes of 2 to 8 views).
@@ -274,9 +229,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   f32x16 dp0;
 #pragma unroll
   for (int r = 0; r < 16; ++r) dp0[r] = kAddDelta ? 0.f : ndelta;
-  // The weight of a row that sees one key is 1 whatever its score: no gradient, where rounding would
-  // leave dP - delta a little off 0.
-  const float unscale = lim == 0 ? 0.f : ldexpf(p.scale, -e);
   auto last_key = [&](int r) { return p.causal ? min(min(r, rows - 1) / p.G + shift, lk - 1) : lk - 1; };
   const int lim_wave = base < rows ? last_key(base + 31) : -1;
   // This part's tiles of 64 keys.
@@ -311,11 +263,21 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
     if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
   };
   auto sub = [&](auto masked, const uint8_t* kt, int st, int j0, Rows& r, auto&& next) __attribute__((always_inline)) {
+    // fp16 at D = 128: read behind the fit, whose branch they would have to outlive (100 bytes of scratch a lane and
+    // 657 us for 548 on the 6 scenes in causal order, 16 heads over 4).
+    constexpr bool kLate = kFp16 && D == 128;
     uint4 kc[2 * DB];
+    auto columns = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) kc[2 * db + ks] = at.col(kt, st, ks, db);
+        for (int ks = 0; ks < 2; ++ks) kc[2 * db + ks] = at.col(kt, st, ks, db);
+    };
+    // Rows that see a key that is not finite have a NaN score and so a NaN dS.
+    auto clear = [&]() __attribute__((always_inline)) {
+      if (decltype(masked)::value && p.causal) pk_clear_not_finite<E>(kc);
+    };
+    if constexpr (!kLate) columns();
     f32x16 s, dp = dp0;
 #pragma unroll
     for (int x = 0; x < 16; ++x) s[x] = 0.f;
@@ -332,10 +294,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
       const int room = lim - j0 - 4 * half;
 #pragma unroll
       for (int x = 0; x < 16; ++x) ds[x] = 8 * (x / 4) + x % 4 <= room ? ds[x] : 0.f;
-      // Rows that see such a key have a NaN score and so a NaN dS.
-      if (p.causal) pk_clear_not_finite<E>(kc);
     }
+    if constexpr (!kLate) clear();
+    if constexpr (kFp16) nlse -= (float)fit.fit(ds, acc);
     const uint4 b[2] = {pack_quad<E>(ds), pack_quad<E>(ds + 8)};
+    if constexpr (kLate) {
+      columns();
+      clear();
+    }
     step();
     next();
 #pragma unroll
@@ -365,6 +331,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
       pk_tile_barrier();
     });
   }
+  // The weight of a row that sees one key is 1 whatever its score: no gradient, where rounding would
+  // leave dP - delta a little off 0.
+  const float unscale = lim == 0 ? 0.f : kFp16 ? fminf(ldexpf(p.scale, -fit.e), 3e38f) : p.scale;
   if (parts > 1) {
     float* dst = p.part_dq + (((int64_t)part * p.Tq + t) * p.H + head) * D;
 #pragma unroll
@@ -421,12 +390,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
     }
   }
   // fp16: dS = P (dP - delta) 2^e, P 2^14.
-  int e = 0;
-  if (kFp16) {
-    const int64_t at = (int64_t)pt.seq * p.Hk + hk;
-    e = pk_scale_exp(__uint_as_float(p.max_do[at]) * __uint_as_float(p.max_v[at]));
-  }
-  const float dscale = kFp16 ? ldexpf(1.f, e - 14) : 1.f;
+  PkFit fit;
+  float dscale = ldexpf(1.f, kFitStart - 14);
 
   f32x16 ak[DB], av[DB];
 #pragma unroll
@@ -531,6 +496,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
         for (int x = 0; x < 16; ++x) ds[x] = 8 * (x / 4) + x % 4 + 4 * half == -shift - i0 ? 0.f : ds[x];
       }
     }
+    if constexpr (kFp16) dscale = ldexpf(dscale, -fit.fit(ds, ak));
     const uint4 pb[2] = {pack_quad<E>(w), pack_quad<E>(w + 8)}, sb[2] = {pack_quad<E>(ds), pack_quad<E>(ds + 8)};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -589,7 +555,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
     }
   }
   // Rows of a sequence of one key all have dS = 0.
-  const float fk = pt.len == 1 ? 0.f : kFp16 ? ldexpf(p.scale, -e) : p.scale;
+  const float fk = pt.len == 1 ? 0.f : kFp16 ? fminf(ldexpf(p.scale, -fit.e), 3e38f) : p.scale;
   const float fv = kFp16 ? ldexpf(1.f, -14) : 1.f;
   const int64_t t = pt.start + (on ? key : 0);
   if (parts > 1) {
@@ -643,13 +609,6 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
   const int key = wkey + col;
   const bool on = key < pt.len;
 
-  int e = 0;
-  if (kFp16) {
-    const int64_t at = (int64_t)pt.seq * p.Hk + hk;
-    e = pk_scale_exp(__uint_as_float(p.max_do[at]) * __uint_as_float(p.max_v[at]));
-  }
-  const float dscale = kFp16 ? ldexpf(1.f, e - 14) : 1.f;
-
   const int first = dkv_first(p, pt.len, lq, pt.tile);  // first tile with a query that sees a key
   const int ntq = (lq + 63) >> 6;
   const int per = ntq > first ? ntq - first : 0;
@@ -699,6 +658,8 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
     bool unclean = false;
+    PkFit fit;  // fp16: dS = P (dP - delta) 2^e, P 2^14
+    float dscale = ldexpf(1.f, kFitStart - 14);
 
     // A tile of 64 queries: rows of rt against the stationary rows, columns of ct into acc.
     auto whole = [&](auto masked, const uint8_t* rt, const uint8_t* ct, const float* start, int i0)
@@ -749,28 +710,35 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
       }
       pk_lds_barrier();
       if constexpr (B) {
+        float ds[32];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          float ds[16];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float4 w = weights[kw][u][g][lane];
-            ds[4 * g] = w.x;
-            ds[4 * g + 1] = w.y;
-            ds[4 * g + 2] = w.z;
-            ds[4 * g + 3] = w.w;
+            ds[16 * u + 4 * g] = w.x;
+            ds[16 * u + 4 * g + 1] = w.y;
+            ds[16 * u + 4 * g + 2] = w.z;
+            ds[16 * u + 4 * g + 3] = w.w;
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) ds[i] = sees(u, i, kFp16 ? ds[i] * dscale * x[u][i] : ds[i] * x[u][i]);
+          for (int i = 0; i < 16; ++i) {
+            const float w = ds[16 * u + i];
+            ds[16 * u + i] = sees(u, i, kFp16 ? w * dscale * x[u][i] : w * x[u][i]);
+          }
           if constexpr (decltype(masked)::value) {
             const int j0 = i0 + 32 * u;
             if (wkey == 0 && j0 <= -shift && -shift < j0 + 32) {  // the row that sees the first key only has dS = 0
 #pragma unroll
-              for (int i = 0; i < 16; ++i) ds[i] = 8 * (i / 4) + i % 4 + 4 * half == -shift - j0 ? 0.f : ds[i];
+              for (int i = 0; i < 16; ++i) ds[16 * u + i] = 8 * (i / 4) + i % 4 + 4 * half == -shift - j0 ? 0.f : ds[16 * u + i];
             }
           }
-          b[u][0] = pack_quad<E>(ds);
-          b[u][1] = pack_quad<E>(ds + 8);
+        }
+        if constexpr (kFp16) dscale = ldexpf(dscale, -fit.fit(ds, acc));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          b[u][0] = pack_quad<E>(ds + 16 * u);
+          b[u][1] = pack_quad<E>(ds + 16 * u + 8);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -819,7 +787,7 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
       }
     }
     // Rows of a sequence of one key all have dS = 0.
-    const float f = B ? (pt.len == 1 ? 0.f : kFp16 ? ldexpf(p.scale, -e) : p.scale) : kFp16 ? ldexpf(1.f, -14) : 1.f;
+    const float f = B ? (pt.len == 1 ? 0.f : kFp16 ? fminf(ldexpf(p.scale, -fit.e), 3e38f) : p.scale) : kFp16 ? ldexpf(1.f, -14) : 1.f;
     const int64_t t = pt.start + (on ? key : 0);
     if (parts > 1) {
       float* dst = p.part_dkv + ((2 * part + (B ? 0 : 1)) * (int64_t)p.Tk + t) * p.Hk * D + (int64_t)hk * D;
@@ -921,19 +889,11 @@ BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
 
 template <typename E, int D>
 int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
-  constexpr bool kFp16 = __is_same(E, FP16);
   const int64_t qslots = dq_slots(p), kslots = dkv_slots(p);
   GW_CHECK_ARG(qslots * p.Hk * p.split_dq < (1ll << 31) && kslots * p.Hk * p.split_dkv < (1ll << 31), "the grid is too large");
-  if (kFp16) {
-    const int64_t words = 2 * (int64_t)(p.n + 2) * p.Hk;  // max_do and max_v, one behind the other
-    hipLaunchKernelGGL(packed_bwd_clear_kernel, dim3((uint32_t)((words + 255) / 256 > 1024 ? 1024 : (words + 255) / 256)),
-                       dim3(256), 0, stream, p.max_do, words);
-    GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (clear)");
-  }
   if (p.Tq > 0) {
-    const int stat_q = p.Tq / kStatTokens + p.n + 2, stat_k = kFp16 && p.Tk > 0 ? p.Tk / kStatTokens + p.n + 2 : 0;
-    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D, kFp16>), dim3(2u + stat_q + stat_k), dim3(256), 0, stream, p,
-                       stat_q);
+    const int stat_q = p.Tq / kStatTokens + p.n + 2;
+    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D>), dim3(2u + stat_q), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (rows)");
     hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)(qslots * p.Hk * p.split_dq)), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq)");
@@ -973,8 +933,7 @@ inline size_t pk_align(size_t n) { return (n + 255) & ~(size_t)255; }
 extern "C" size_t gw_packed_attn_bwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
   if (n < 0 || Tq < 0 || Tk < 0 || Hk < 1 || Hq < Hk || D < 1) return 0;
   const gw::BwdPlan b = gw::packed_bwd_plan(n, Tq, Tk, Hq, Hk, D);
-  return gw::pk_align((size_t)Tq * Hq * 8) + gw::pk_align((size_t)(n + 2) * Hk * 8) + gw::pk_align(b.dq_bytes) +
-         gw::pk_align(b.dkv_bytes) + 8 * (size_t)(b.slots_q + b.slots_k);
+  return gw::pk_align((size_t)Tq * Hq * 8) + gw::pk_align(b.dq_bytes) + gw::pk_align(b.dkv_bytes) + 8 * (size_t)(b.slots_q + b.slots_k);
 }
 
 extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const void* k,
@@ -1015,14 +974,12 @@ extern "C" int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_str
   char* ws = static_cast<char*>(workspace);
   p.nlse = reinterpret_cast<float*>(ws);
   p.ndelta = p.nlse + Tq * Hq;
-  p.max_do = reinterpret_cast<uint32_t*>(ws + pk_align((size_t)Tq * Hq * 8));
-  p.max_v = p.max_do + (n + 2) * Hk;
   const BwdPlan b = packed_bwd_plan(n, Tq, Tk, Hq, Hk, D);
   p.split_dq = b.dq;
   p.split_dkv = b.dkv;
   p.per_dq = b.per_dq;
   p.per_dkv = b.per_dkv;
-  p.part_dq = reinterpret_cast<float*>(ws + pk_align((size_t)Tq * Hq * 8) + pk_align((size_t)(n + 2) * Hk * 8));
+  p.part_dq = reinterpret_cast<float*>(ws + pk_align((size_t)Tq * Hq * 8));
   p.part_dkv = p.part_dq + pk_align(b.dq_bytes) / sizeof(float);
   int2* lists = reinterpret_cast<int2*>(p.part_dkv + pk_align(b.dkv_bytes) / sizeof(float));
   if (b.slots_q) p.order_q = lists;
