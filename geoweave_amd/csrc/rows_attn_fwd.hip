@@ -26,13 +26,13 @@
 
 #include "gw_packed.h"
 #include "gw_rows.h"
+#include "gw_rows_parts.h"
 
 namespace gw {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kRows = 16;
-constexpr int kRowsPart = 256;       // a part is a multiple of this many keys (4 waves x 32, twice)
 
 __device__ __forceinline__ f32x4 mma16(BF16, uint4 a, uint4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -125,9 +125,7 @@ __device__ __forceinline__ int rows_part_len(const RowsParams& p, int lane) {
     const RowsSeq s = rows_seq<PAGED>(p, i);
     total += (int64_t)rows_tiles_of<PAGED>(p, s) * s.lk;
   }
-  total = wave_sum64(total);
-  const int64_t len = (total + p.want - 1) / p.want;
-  return (int)((max(len, (int64_t)kRowsPart) + kRowsPart - 1) / kRowsPart * kRowsPart);
+  return rows_part_keys(wave_sum64(total), p.want);
 }
 
 // The part of slot `slot`.
@@ -150,7 +148,7 @@ __device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, int
     if (i < nseq) {
       const RowsSeq s = rows_seq<PAGED>(p, i);
       tiles = rows_tiles_of<PAGED>(p, s);
-      parts = max(1, (int)(((int64_t)s.lk + r.len - 1) / r.len));
+      parts = rows_parts(s.lk, r.len);
     }
     const int mine = tiles * parts, cut = parts > 1 ? mine : 0;
     const int incl = wave_scan(mine), cut_incl = wave_scan(cut);
