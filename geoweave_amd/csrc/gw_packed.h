@@ -337,7 +337,9 @@ constexpr float kPkSumCap = __is_same(E, FP16) ? 60000.f : 32768.f;
 // inf and NaN in places that a row does not see. A masked weight is 0, but 0 * inf is NaN: in tiles
 // that some rows see only in part, inf and NaN among the second operand's entries are cleared before the
 // product, and once it is known that there were any (never, in healthy data), a pass over those tiles
-// adds them to the rows that do see them.
+// adds them to the rows that do see them. Entries of V and dO meet weights (ZERO false: the entries are added); K
+// and Q meet dS, where a row or key that sees such an entry has a NaN dS or, its score -inf, a dS of 0, and 0 * inf
+// is NaN (ZERO true: NaN is added).
 template <typename E>
 constexpr uint32_t kPkExp = __is_same(E, FP16) ? 0x7C00u : 0x7F80u;
 
@@ -371,7 +373,7 @@ __device__ __forceinline__ bool pk_clear_not_finite(uint4 (&q)[N]) {
 }
 // Adds the entries of a memory row that are not finite to a lane's accumulator entries (dims 32 db + 8 g + 4 half
 // + 0..3), where `seen`.
-template <typename E, int DB>
+template <typename E, bool ZERO = false, int DB>
 __device__ __forceinline__ void pk_add_not_finite(const uint16_t* row, int half, bool seen, f32x16 (&acc)[DB]) {
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -381,7 +383,7 @@ __device__ __forceinline__ void pk_add_not_finite(const uint16_t* row, int half,
       const uint32_t h[4] = {w.x & 0xFFFFu, w.x >> 16, w.y & 0xFFFFu, w.y >> 16};
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (seen && pk_not_finite<E>(h[i])) acc[db][4 * g + i] += in_to_float(__is_same(E, FP16), h[i]);
+        if (seen && pk_not_finite<E>(h[i])) acc[db][4 * g + i] += ZERO ? NAN : in_to_float(__is_same(E, FP16), h[i]);
     }
 }
 

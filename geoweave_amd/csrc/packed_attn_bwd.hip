@@ -221,10 +221,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   const int64_t srow = (int64_t)head * p.Tq + t;
   float nlse = p.nlse[srow] * sl2;  // fp16: p 2^e = 2^(s - lse + e)
   if (kFp16) nlse += (float)kFitStart - kPScale<E>;
-  // dP - delta: at D = 128 delta is where the products start, in a register block of its own; at D = 64,
+  // dP - delta: in bf16 at D = 128 delta is where the products start, in a register block of its own; at D = 64,
   // where three waves share a SIMD's registers, it is added afterwards (with the block 124 bytes of
-  // scratch a lane and 860 us for 563 on 6 scenes of 2 to 8 views).
-  constexpr bool kAddDelta = D == 64;
+  // scratch a lane and 860 us for 563 on 6 scenes of 2 to 8 views), and so it is in fp16 (581 us with the block,
+  // 560 without).
+  constexpr bool kAddDelta = D == 64 || kFp16;
   const float ndelta = p.ndelta[srow];
   f32x16 dp0;
 #pragma unroll
@@ -262,9 +263,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   auto step = []() __attribute__((always_inline)) {
     if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
   };
+  bool unclean = false;  // K holds inf or NaN in tiles that some rows see only in part
   auto sub = [&](auto masked, const uint8_t* kt, int st, int j0, Rows& r, auto&& next) __attribute__((always_inline)) {
     // fp16 at D = 128: read behind the fit, whose branch they would have to outlive (100 bytes of scratch a lane and
-    // 657 us for 548 on the 6 scenes in causal order, 16 heads over 4).
+    // 657 us for 548 on 6 causal sequences of 3,013 to 4,795 tokens, 16 heads over 4).
     constexpr bool kLate = kFp16 && D == 128;
     uint4 kc[2 * DB];
     auto columns = [&]() __attribute__((always_inline)) {
@@ -273,9 +275,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) kc[2 * db + ks] = at.col(kt, st, ks, db);
     };
-    // Rows that see a key that is not finite have a NaN score and so a NaN dS.
     auto clear = [&]() __attribute__((always_inline)) {
-      if (decltype(masked)::value && p.causal) pk_clear_not_finite<E>(kc);
+      if (decltype(masked)::value && p.causal) unclean |= pk_clear_not_finite<E>(kc);
     };
     if constexpr (!kLate) columns();
     f32x16 s, dp = dp0;
@@ -330,6 +331,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
       }
       pk_tile_barrier();
     });
+    if (__builtin_expect(unclean, 0)) {
+      const int end = min(64 * (tk0 + ntk), min(lk, lim_wave + 1));
+      for (int j = 64 * (tk0 + (full & ~1)); j < end; ++j)  // pk_tiles masks from an even tile on
+        pk_add_not_finite<E, true>(p.k + (int64_t)(k0 + j) * p.kst + (int64_t)hk * p.ksh, half, j <= lim, acc);
+    }
   }
   // The weight of a row that sees one key is 1 whatever its score: no gradient, where rounding would
   // leave dP - delta a little off 0.
@@ -436,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
   };
 
   const PkLane<D> at(lane);
-  bool unclean = false;  // dO holds inf or NaN in tiles that see some keys only in part
+  bool unclean = false, unclean_q = false;  // dO, Q hold inf or NaN in tiles that see some keys only in part
   // A sub-tile of 32 queries. Entry x of this lane is query i0 + 8 (x / 4) + 4 half + x % 4.
   auto sub = [&](auto masked, const uint8_t* qt, const uint8_t* gt, const float* nl, const float* nd, int st, int i0)
                  __attribute__((always_inline)) {
@@ -505,7 +511,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
       uint4 q[1] = {c[i % PRE]};
       if constexpr (decltype(masked)::value) {
         const bool any = pk_clear_not_finite<E>(q);
-        if (i % 2 == 0) unclean |= any;  // keys that see a query whose q is not finite have a NaN dS
+        (i % 2 == 0 ? unclean : unclean_q) |= any;
       }
       if (i % 2 == 0)
         av[db] = mma(E{}, q[0], pb[ks], av[db]);
@@ -546,11 +552,14 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
       tile(PkInt<1>{});
     }
     if (n < total) tile(PkInt<0>{});
-    if (__builtin_expect(unclean, 0)) {
+    if (__builtin_expect(unclean | unclean_q, 0)) {
       for (int x = t0; x < t0 + total; ++x) {
         const int h = x / per, i0 = 64 * (first + x % per);
-        for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i)
-          pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, av);
+        for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i) {
+          if (unclean) pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, av);
+          if (unclean_q)
+            pk_add_not_finite<E, true>(qbase + (int64_t)i * p.qst + (int64_t)h * p.qsh, half, key <= i + shift, ak);
+        }
       }
     }
   }
@@ -657,7 +666,7 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
-    bool unclean = false;
+    bool unclean = false;  // the columns (dO, Q) hold inf or NaN in tiles that see some keys only in part
     PkFit fit;  // fp16: dS = P (dP - delta) 2^e, P 2^14
     float dscale = ldexpf(1.f, kFitStart - 14);
 
@@ -745,10 +754,7 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
 #pragma unroll
       for (int i = 0; i < 4 * DB; ++i) {
         uint4 q[1] = {c[i % PRE]};
-        if constexpr (decltype(masked)::value) {
-          const bool any = pk_clear_not_finite<E>(q);
-          if (!B) unclean |= any;  // keys that see a query whose q is not finite have a NaN dS
-        }
+        if constexpr (decltype(masked)::value) unclean |= pk_clear_not_finite<E>(q);
         acc[i % DB] = mma(E{}, q[0], b[i / (2 * DB)][i / DB % 2], acc[i % DB]);
         if (i + PRE < 4 * DB) c[i % PRE] = column(i + PRE);
         __builtin_amdgcn_sched_barrier(0);
@@ -782,8 +788,10 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
     if (__builtin_expect(unclean, 0)) {
       for (int x = t0; x < t0 + total; ++x) {
         const int h = x / per, i0 = 64 * (first + x % per);
-        for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i)
-          pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, acc);
+        for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i) {
+          const uint16_t* row = B ? qbase + (int64_t)i * p.qst + (int64_t)h * p.qsh : gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh;
+          pk_add_not_finite<E, B>(row, half, key <= i + shift, acc);
+        }
       }
     }
     // Rows of a sequence of one key all have dS = 0.
