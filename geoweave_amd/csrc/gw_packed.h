@@ -220,7 +220,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t pk_rsrc(const char* base, int6
 
 // Row tiles of one head of one sequence: 64 rows at a time from memory straight to LDS. Lane i of a
 // wave writes 16 bytes at the wave's segment + 16 i, so it reads the chunk that the swizzle keeps there.
-// Rows past the sequence's end arrive as zeros, whatever the strides (a broadcast row has stride 0).
+// Rows past the sequence's end arrive as zeros, whatever the strides (a broadcast row has stride 0), or as the last
+// row again (LAST; 64 n < rows).
 template <int D, int THREADS>
 struct PkRows {
   static constexpr int kRowBytes = 2 * D;
@@ -247,14 +248,16 @@ struct PkRows {
     seg = (uint32_t)(tid >> 6) * 1024u;
   }
   // Rows [64 n, 64 n + 64) to lds.
+  template <bool LAST = false>
   __device__ __forceinline__ void load(int n, uint8_t* lds) const {
     const int64_t at = (int64_t)n * 64 * stride;
     const __amdgpu_buffer_rsrc_t rs = pk_rsrc(base + at, bytes - at);
+    const uint32_t end = LAST ? off - (uint32_t)row * stride + (uint32_t)(rows - 1 - 64 * n) * stride : kPkNowhere;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rs, (__attribute__((address_space(3))) void*)(lds + seg + i * kRowsPerPass * kRowBytes), 16,
-          (int)(64 * n + row + i * kRowsPerPass < rows ? off + (uint32_t)(i * kRowsPerPass) * stride : kPkNowhere), 0, 0, 0);
+          (int)(64 * n + row + i * kRowsPerPass < rows ? off + (uint32_t)(i * kRowsPerPass) * stride : end), 0, 0, 0);
   }
 };
 

@@ -25,7 +25,7 @@
 // the statistics 28 us; the same with heads of 128 dQ 1,016 us (1.1 PFLOP/s), dK/dV 1,660 (0.90). 96 causal sequences of 17 to 697 tokens, 16 heads over 8: 27 + 54 + 79 us;
 // without the lists of tiles by falling work 24 + 61 + 103.
 //
-// Rows behind a sequence's end arrive as zeros, and rows that see no key have P = 0.
+// Rows behind a sequence's end add 0 to every gradient, and rows that see no key have P = 0.
 #include <math.h>
 
 #include "gw_packed.h"
@@ -423,15 +423,18 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
   auto load = [&](uint8_t* qd, uint8_t* gd, float* ld, float* dd) __attribute__((always_inline)) {
     qrows.base = uniform_ptr(reinterpret_cast<const char*>(qbase + (int64_t)ld_h * p.qsh));
     grows.base = uniform_ptr(reinterpret_cast<const char*>(gbase + (int64_t)ld_h * p.gsh));
-    qrows.load(ld_t, qd);
+    qrows.template load<true>(ld_t, qd);
     grows.load(ld_t, gd);
-    // 64 lse and 64 delta, 4 bytes a lane (their start is only 4-byte aligned): waves 0 and 1. Zeros behind
-    // the last query, whose Q and dO are zero as well.
+    // 64 lse and 64 delta, 4 bytes a lane (their start is only 4-byte aligned): waves 0 and 1. A tile's rows behind
+    // the last query repeat its Q and lse, and have dO = 0 and delta = 0: they add 0 to every key, and their
+    // weights are finite where the last query's are (zeros of Q would make NaN with a key's inf, whose weights are 0
+    // where it scores -inf).
     const int64_t sat = sbase + (int64_t)ld_h * p.Tq + ld_t * 64;
     const int64_t left = (int64_t)(lq - ld_t * 64) * 4;
+    const int last = (int)min(left, (int64_t)256) - 4;
     if (wave == 0)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.nlse + sat), left),
-                                               (__attribute__((address_space(3))) void*)ld, 4, lane * 4, 0, 0, 0);
+                                               (__attribute__((address_space(3))) void*)ld, 4, min(lane * 4, last), 0, 0, 0);
     if (wave == 1)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.ndelta + sat), left),
                                                (__attribute__((address_space(3))) void*)dd, 4, lane * 4, 0, 0, 0);
@@ -635,13 +638,14 @@ __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const Packe
   auto load = [&](uint8_t* qd, uint8_t* gd, float* ld, float* dd) __attribute__((always_inline)) {
     qrows.base = uniform_ptr(reinterpret_cast<const char*>(qbase + (int64_t)ld_h * p.qsh));
     grows.base = uniform_ptr(reinterpret_cast<const char*>(gbase + (int64_t)ld_h * p.gsh));
-    qrows.load(ld_t, qd);
+    qrows.template load<true>(ld_t, qd);
     grows.load(ld_t, gd);
     const int64_t sat = sbase + (int64_t)ld_h * p.Tq + ld_t * 64;
     const int64_t left = (int64_t)(lq - ld_t * 64) * 4;
+    const int last = (int)min(left, (int64_t)256) - 4;
     if (wave == 0)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.nlse + sat), left),
-                                               (__attribute__((address_space(3))) void*)ld, 4, lane * 4, 0, 0, 0);
+                                               (__attribute__((address_space(3))) void*)ld, 4, min(lane * 4, last), 0, 0, 0);
     if (wave == 4)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(pk_rsrc(reinterpret_cast<const char*>(p.ndelta + sat), left),
                                                (__attribute__((address_space(3))) void*)dd, 4, lane * 4, 0, 0, 0);

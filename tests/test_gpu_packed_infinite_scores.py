@@ -73,3 +73,25 @@ def test_a_query_that_scores_minus_infinity(gpu_device, dtype, d, hq, hk, lens_q
         keys = torch.arange(cu_k[-1])
         seen = (keys < n_k) & (keys <= i + n_k - n_q if causal else True)
         check_but(dk, ref, "dk", dtype, d, seen)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hq,hk", [(64, 2, 2), (128, 4, 2), (64, 1, 1)])
+@pytest.mark.parametrize("lens_q,lens_k", CASES + [([65], [65]), ([129, 3], [1, 700]), ([1], [64])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_a_key_that_scores_minus_infinity(gpu_device, dtype, d, hq, hk, lens_q, lens_k, causal):
+    """Its weights are 0, so its dk and dv are 0; queries behind the sequence's end, which a tile holds as zeros, are
+    no queries (0 times its inf would be NaN)."""
+    q, k, v, do, cu_q, cu_k = positive(make(lens_q, lens_k, hq, hk, d, dtype, 22))
+    n_k = cu_k[1]
+    s_mag = packed_attention(q, k, v, cu_q, cu_k, causal)["s_mag"]
+    for j in {n_k // 2, n_k - 1}:
+        kj, far = k.clone(), k.double()
+        kj[j, :, DIM], far[j, :, DIM] = -math.inf, -1e30
+        ref = packed_attention(q, far, v, cu_q, cu_k, causal, do=do)
+        ref["s_mag"] = s_mag
+        _, _, dk, dv = step((q, kj, v, do, cu_q, cu_k), gpu_device, causal)
+        if n_k > 1:
+            assert (dk[j] == 0).all() and (dv[j] == 0).all()
+            check(dv, ref, "dv", dtype, d)
+            check(dk, ref, "dk", dtype, d)
