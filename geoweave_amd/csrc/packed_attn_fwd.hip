@@ -4,11 +4,12 @@
 // For query token i of a sequence of Lq queries and Lk keys and head h (key head h / G):
 //   p_j = softmax_j(scale q_i . k_j) over j < Lk (causal: j <= i + Lk - Lq),  o_i = sum_j p_j v_j.
 // One pass over the keys with a running reference maximum m and sum l (held in fp32, in the exp2
-// domain): o = (sum_j 2^(s_j - m) v_j) / l. m is raised only when a lane's 16 weights sum past a
-// cap (gw_packed.h), so P fits fp16 and no maximum is taken per tile otherwise; but for roundings the result does
-// not depend on which m was used. P is rounded to the inputs' 16-bit type for the second product (half a step,
-// 2^-8 or 2^-11 of a weight, with errors that average out over the keys; fp16 weights below 2^-24 of a row's
-// largest lose more, 2^-35 of that largest at most); sums add the fp32 weights.
+// domain): o = (sum_j 2^(s_j - m) v_j) / l. m is raised only when a lane's 16 weights sum past a cap
+// (gw_packed.h), so P fits fp16 and no maximum is taken per tile otherwise; but for roundings the result does not
+// depend on which m was used, and m depends on the row's own scores alone. P is rounded to the inputs'
+// 16-bit type for the second product (half a step, 2^-8 or 2^-11 of a weight, with errors that average out over
+// the keys; fp16 weights below 2^-24 of a row's largest lose more, 2^-35 of that largest at most); sums add the
+// fp32 weights.
 //
 // The rows of a key head are (token, head of the group), token-major, so a group's heads share the
 // K and V tiles. 4 waves per workgroup, each QPW blocks of 32 rows; tiles of 64 keys go from memory
@@ -167,12 +168,15 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedFwd
       };
       float ls = weights(-m[a]);
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= kPkSumCap<E>)) != 0ull, 0)) {
-        // A row's weights have grown past the cap (or these are its first keys): every row of the
-        // block moves its reference to (fp16: below) its largest score here if that is higher.
+        // A row's weights have grown past the cap (or these are its first keys): it moves its reference to (fp16:
+        // below) its largest score here if that is higher. The block's other rows keep theirs, so that a row's
+        // roundings depend on what it sees alone.
+        const bool up = pair_max(ls <= kPkSumCap<E> ? 0.f : 1.f) > 0.f;
         float mx = s[a][0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[a][r]);
-        const float mn = fmaxf(m[a], pair_max(mx) * sl2 - kPkBelow<E>);
+        mx = pair_max(mx);
+        const float mn = up ? fmaxf(m[a], mx * sl2 - kPkBelow<E>) : m[a];
         const float alpha = fexp2(m[a] - mn);
         m[a] = mn;
         l[a] *= alpha;

@@ -332,9 +332,11 @@ __global__ __launch_bounds__(256, 2) void rows_attn_kernel(const RowsParams p) {
     };
     float ls = weights(-m);
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= kPkSumCap<E>)) != 0ull, 0)) {
+      const bool up = rows_max(ls <= kPkSumCap<E> ? 0.f : 1.f) > 0.f;  // this row, not the tile's others
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      const float mn = fmaxf(m, rows_max(mx) * p.scale_log2 - kPkBelow<E>);
+      mx = rows_max(mx);
+      const float mn = up ? fmaxf(m, mx * p.scale_log2 - kPkBelow<E>) : m;
       const float alpha = fexp2(m - mn);
       m = mn;
       l *= alpha;
