@@ -28,6 +28,17 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
     if (!(cond)) return ::gw::set_error(GW_ERR_INVALID, __VA_ARGS__); \
   } while (0)
 
+// A launch takes fewer than 2^32 threads along a dimension of its grid.
+#define GW_CHECK_GRID(workgroups, threads)                                                                      \
+  do {                                                                                                          \
+    const int64_t wgs__ = (workgroups);                                                                         \
+    if (wgs__ >= (1ll << 32) / (threads))                                                                       \
+      return ::gw::set_error(GW_ERR_UNSUPPORTED,                                                                \
+                             "%lld workgroups of %d threads pass 2^32 threads: too many tokens, sequences or " \
+                             "heads for one call",                                                              \
+                             (long long)wgs__, (int)(threads));                                                 \
+  } while (0)
+
 #define GW_HIP_LAUNCH_CHECK(what)                                \
   do {                                                           \
     hipError_t e__ = hipGetLastError();                          \

@@ -49,6 +49,13 @@ inline int64_t rows_tiles(bool paged, int64_t n, int64_t Tq, int64_t G) {
 inline size_t rows_workspace(int64_t tiles, int64_t Hk, int64_t D) {
   return (size_t)2 * rows_want(Hk) * Hk * 16 * (D + 1) * sizeof(float) + (size_t)tiles * sizeof(int2);
 }
+// Workgroups of the attention launch. Packed: a sequence of at most kRowsMax rows has one or two tiles, and all have
+// no more than the rows in all allow.
+inline int64_t rows_grid(bool paged, int64_t n, int64_t Tq, int64_t G, int64_t Hk, bool split) {
+  int64_t tiles = rows_tiles(paged, n, Tq, G);
+  if (!paged && Tq * G / 16 + n + 2 < tiles) tiles = Tq * G / 16 + n + 2;
+  return (tiles + (split ? rows_want(Hk) : 0)) * Hk;
+}
 // Launches on checked arguments (dtype bf16 or fp16, D 64 or 128); p.split and p.want are set.
 int rows_attn(int dtype, int D, bool paged, RowsParams p, void* workspace, hipStream_t stream);
 

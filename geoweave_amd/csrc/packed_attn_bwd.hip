@@ -64,7 +64,9 @@ struct PackedBwdParams {
 constexpr int kBwdTile = 128;  // rows of a dQ workgroup, keys of a dK/dV workgroup
 
 // Workgroup slots per key head of the two passes.
-__host__ __device__ inline int dq_slots(const PackedBwdParams& p) { return (int)((int64_t)p.Tq * p.G / kBwdTile) + p.n + 2; }
+__host__ __device__ inline int dq_slots(const PackedBwdParams& p) {
+  return (int)((int64_t)p.Tq * p.G / kBwdTile) + p.n + 2;
+}
 __host__ __device__ inline int dkv_slots(const PackedBwdParams& p) { return p.Tk / kBwdTile + p.n + 2; }
 
 // Parts of a loop over `work` tiles of 64.
@@ -901,22 +903,31 @@ BwdPlan packed_bwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
 
 template <typename E, int D>
 int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
-  const int64_t qslots = dq_slots(p), kslots = dkv_slots(p);
-  GW_CHECK_ARG(qslots * p.Hk * p.split_dq < (1ll << 31) && kslots * p.Hk * p.split_dkv < (1ll << 31), "the grid is too large");
+  const int64_t qgrid = (int64_t)dq_slots(p) * p.Hk * p.split_dq, kgrid = (int64_t)dkv_slots(p) * p.Hk * p.split_dkv;
+  const int64_t rgrid = 2 + p.Tq / kStatTokens + (int64_t)p.n + 2;
+  const int64_t qjoin = ((int64_t)p.Tq * p.H * (D / 4) + 255) / 256, kjoin = ((int64_t)p.Tk * p.Hk * (D / 4) + 255) / 256;
+  // All launches fit, or none is made.
   if (p.Tq > 0) {
-    const int stat_q = p.Tq / kStatTokens + p.n + 2;
-    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D>), dim3(2u + stat_q), dim3(256), 0, stream, p);
+    GW_CHECK_GRID(rgrid, 256);
+    GW_CHECK_GRID(qgrid, 256);
+    if (p.split_dq > 1) GW_CHECK_GRID(qjoin, 256);
+  }
+  if (p.Tk > 0) {
+    GW_CHECK_GRID(kgrid, D == 64 ? 256 : 512);
+    if (p.split_dkv > 1) GW_CHECK_GRID(kjoin, 256);
+  }
+  if (p.Tq > 0) {
+    hipLaunchKernelGGL((packed_bwd_stats_kernel<E, D>), dim3((uint32_t)rgrid), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (rows)");
-    hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)(qslots * p.Hk * p.split_dq)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((packed_bwd_dq_kernel<E, D>), dim3((uint32_t)qgrid), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq)");
     if (p.split_dq > 1) {
-      const int64_t threads = (int64_t)p.Tq * p.H * (D / 4);
-      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D, false>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D, false>), dim3((uint32_t)qjoin), dim3(256), 0, stream, p);
       GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dq join)");
     }
   }
   if (p.Tk > 0) {
-    const dim3 tiles((uint32_t)(kslots * p.Hk * p.split_dkv));
+    const dim3 tiles((uint32_t)kgrid);
     if constexpr (D == 64) {
       hipLaunchKernelGGL(packed_bwd_dkv_kernel<E>, tiles, dim3(256), 0, stream, p);
     } else {
@@ -924,8 +935,7 @@ int packed_bwd_launch(const PackedBwdParams& p, hipStream_t stream) {
     }
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk, dv)");
     if (p.split_dkv > 1) {
-      const int64_t threads = (int64_t)p.Tk * p.Hk * (D / 4);
-      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D, true>), dim3((uint32_t)((threads + 255) / 256), 2), dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((packed_bwd_join_kernel<E, D, true>), dim3((uint32_t)kjoin, 2), dim3(256), 0, stream, p);
       GW_HIP_LAUNCH_CHECK("gw_packed_attn_bwd (dk, dv join)");
     }
   }

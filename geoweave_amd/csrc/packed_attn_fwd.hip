@@ -330,17 +330,18 @@ FwdPlan packed_fwd_plan(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
   return f;
 }
 
+inline int64_t fwd_grid(int64_t n, int64_t Tq, int64_t Hq, int64_t Hk, int qpw) {
+  return (Tq * (Hq / Hk) / (128 * qpw) + n + 2) * Hk;
+}
+inline int64_t fwd_join_grid(int64_t Tq, int64_t Hq, int64_t D) { return (Tq * Hq * (D / 4) + 255) / 256; }
+
 template <typename E, int D, int QPW>
 int packed_fwd_launch(const PackedFwdParams& p, hipStream_t stream) {
-  const int64_t slots = (int64_t)p.Tq * p.G / (128 * QPW) + p.n + 2;
-  GW_CHECK_ARG(slots * p.Hk < (1ll << 31), "grid of %lld workgroups is too large", (long long)(slots * p.Hk));
-  hipLaunchKernelGGL((packed_attn_fwd_kernel<E, D, QPW>), dim3((uint32_t)(slots * p.Hk), (uint32_t)p.split), dim3(256), 0,
-                     stream, p);
+  const dim3 grid((uint32_t)fwd_grid(p.n, p.Tq, p.H, p.Hk, QPW), (uint32_t)p.split);
+  hipLaunchKernelGGL((packed_attn_fwd_kernel<E, D, QPW>), grid, dim3(256), 0, stream, p);
   GW_HIP_LAUNCH_CHECK("gw_packed_attn_fwd");
   if (p.split > 1) {
-    constexpr int kRowsPerWg = 256 / (D / 4);
-    const int64_t wgs = ((int64_t)p.Tq * p.H + kRowsPerWg - 1) / kRowsPerWg;
-    hipLaunchKernelGGL((packed_join_kernel<E, D>), dim3((uint32_t)wgs), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((packed_join_kernel<E, D>), dim3((uint32_t)fwd_join_grid(p.Tq, p.H, D)), dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("gw_packed_attn_fwd (join)");
   }
   return GW_OK;
@@ -407,6 +408,13 @@ extern "C" int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_str
   GW_CHECK_ARG(f.rows_bytes + f.split_bytes == 0 ||
                    (workspace && aligned16(workspace) && workspace_bytes >= f.rows_bytes + f.split_bytes),
                "workspace of %zu bytes, %zu are needed", workspace_bytes, f.rows_bytes + f.split_bytes);
+  // All launches fit, or none is made.
+  if (f.rows) {
+    GW_CHECK_GRID(rows_grid(false, n, Tq, Hq / Hk, Hk, true), 256);
+    GW_CHECK_GRID(rows_tiles(false, n, Tq, Hq / Hk) * Hk, 256);
+  }
+  if (f.tiles) GW_CHECK_GRID(fwd_grid(n, Tq, Hq, Hk, f.qpw), 256);
+  if (f.tiles && f.split > 1) GW_CHECK_GRID(fwd_join_grid(Tq, Hq, D), 256);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (f.rows) {
     RowsParams r = {};

@@ -434,6 +434,7 @@ extern "C" int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strid
   // Few tokens a workgroup until the chip has four workgroups per CU, then up to 8.
   p.TT = kRotMaxTokens;
   while (p.TT > 1 && B * ((T + p.TT - 1) / p.TT) < 1024) p.TT >>= 1;
+  GW_CHECK_GRID((T + p.TT - 1) / p.TT, kRotThreads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case GW_DTYPE_BF16: return rot_launch<BF16>(p, V, staged, s);

@@ -540,18 +540,14 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
 
 template <typename E, int D, bool PAGED>
 int rows_launch(const RowsParams& p, hipStream_t stream) {
-  // Packed: a sequence of at most kRowsMax rows has one or two tiles, and all have no more than the rows
-  // in all allow.
-  const int64_t joins = rows_tiles(PAGED, p.n, p.Tq, p.G);
-  int64_t tiles = joins;
-  if (!PAGED && (int64_t)p.Tq * p.G / kRows + p.n + 2 < tiles) tiles = (int64_t)p.Tq * p.G / kRows + p.n + 2;
-  const int64_t grid = (tiles + (p.split ? p.want : 0)) * p.Hk;
-  GW_CHECK_ARG(grid < (1ll << 31), "grid of %lld workgroups is too large", (long long)grid);
+  const int64_t joins = rows_tiles(PAGED, p.n, p.Tq, p.G) * p.Hk, grid = rows_grid(PAGED, p.n, p.Tq, p.G, p.Hk, p.split);
+  GW_CHECK_GRID(grid, 256);
+  if (p.split) GW_CHECK_GRID(joins, 256);
   hipLaunchKernelGGL((rows_attn_kernel<E, D, PAGED>), dim3((uint32_t)grid), dim3(256), 0, stream, p);
   GW_HIP_LAUNCH_CHECK("rows attention");
   if (p.split) {
     const int64_t rows = (int64_t)p.Tq * p.G;
-    hipLaunchKernelGGL((rows_join_kernel<E, D, PAGED>), dim3((uint32_t)(joins * p.Hk), (uint32_t)(rows < kRows ? rows : kRows)),
+    hipLaunchKernelGGL((rows_join_kernel<E, D, PAGED>), dim3((uint32_t)joins, (uint32_t)(rows < kRows ? rows : kRows)),
                        dim3(256), 0, stream, p);
     GW_HIP_LAUNCH_CHECK("rows attention (join)");
   }

@@ -646,7 +646,7 @@ int gw_sparse_attn_bwd_dense(int dtype,
  * behind the other from dim 0; an even number of dims may remain behind them and is copied.
  * bases (host): positive. Dims i and i + d/2 of an axis's block of d turn by
  * pos * base^(-2 i / d), by the negative of it with inverse != 0 (the gradient).
- * dtype bf16, fp16 or fp32; D <= 256, up to 8 axes; B <= 65535. Angles are formed in 64 bits.
+ * dtype bf16, fp16 or fp32; D <= 256, up to 8 axes; B <= 65535, T < 2^27. Angles are formed in 64 bits.
  * ------------------------------------------------------------------------------------ */
 #define GW_POS_INT32 0
 #define GW_POS_INT64 1
@@ -668,10 +668,11 @@ int gw_rotary_axes(int dtype, const void* x0, const int64_t* x0_strides, void* y
  * [Tq, Hq], natural log. o_rest (nullable): [Tq, Hq, D] contiguous in o's type, what the rounding of o
  * left (the backward needs it). Bounds outside [0, Tq] or [0, Tk] are clamped.
  * D in {64, 128}, bf16 or fp16, softmax_scale > 0; 16-byte aligned rows, token strides in [0, 2^24)
- * elements; tokens x Hq below 2^31 - 2^12. workspace: gw_packed_attn_fwd_workspace_size(...) bytes,
- * 16-byte aligned (parts of the keys, where they are split over workgroups). Nothing is read from the
- * device by the host: a captured graph may be replayed with other bounds of the same n. Bounds out of
- * order give unspecified values, and no access outside the tensors and the workspace.
+ * elements; tokens x Hq below 2^31 - 2^12; Tq Hq / 128 + (n + 2) Hk below 2^24 (a launch takes 2^32
+ * threads). workspace: gw_packed_attn_fwd_workspace_size(...) bytes, 16-byte aligned (parts of the keys, where
+ * they are split over workgroups). Nothing is read from the device by the host: a captured graph may be replayed
+ * with other bounds of the same n. Bounds out of order give unspecified values, and no access outside the
+ * tensors and the workspace.
  * ------------------------------------------------------------------------------------ */
 size_t gw_packed_attn_fwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
 int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -684,7 +685,8 @@ int gw_packed_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const
  * Backward of gw_packed_attn_fwd: dq [Tq, Hq, D], dk and dv [Tk, Hk, D] (each element written once;
  * tokens of no sequence, and rows without keys, get zeros) from the forward's o, o_rest and lse and the
  * gradient dout of o. No float atomics: the same inputs give the same bits. Arguments and limits as
- * there. workspace: gw_packed_attn_bwd_workspace_size(...) bytes, 16-byte aligned.
+ * there, and Tk Hk / 128 + (n + 2) Hk below 2^24 (D = 128: 2^23), Tq / 16 + n + 4 below 2^24. workspace:
+ * gw_packed_attn_bwd_workspace_size(...) bytes, 16-byte aligned.
  * ------------------------------------------------------------------------------------ */
 size_t gw_packed_attn_bwd_workspace_size(int64_t n, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
 int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -707,8 +709,9 @@ int gw_packed_attn_bwd(int dtype, const void* q, const int64_t* q_strides, const
  * causal != 0: new token i of N sees the keys below lens - N + 1 + i, else all. A row with no key gets
  * o = 0, lse = -inf. lse (nullable): fp32 [B, N, Hq], natural log.
  * D in {64, 128}, bf16 or fp16, softmax_scale > 0, 16-byte aligned rows, table_width * page_size and
- * B * N * Hq below 2^31 - 2^12. workspace: gw_paged_attn_fwd_workspace_size(...) bytes, 16-byte
- * aligned. Nothing is read from the device by the host: a captured graph follows the table and lengths.
+ * B * N * Hq below 2^31 - 2^12, B * ceil(N Hq / (16 Hk)) * Hk below 2^24. workspace:
+ * gw_paged_attn_fwd_workspace_size(...) bytes, 16-byte aligned. Nothing is read from the device by the host: a
+ * captured graph follows the table and lengths.
  * ------------------------------------------------------------------------------------ */
 size_t gw_paged_attn_fwd_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D);
 int gw_paged_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
