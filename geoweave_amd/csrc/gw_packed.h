@@ -233,7 +233,8 @@ struct PkRows {
   int rows;
   int row;             // this lane's row in pass 0
   uint32_t stride;     // bytes
-  uint32_t off;        // this lane's offset in pass 0
+  uint32_t off;        // this lane's offset in pass 0,
+  uint32_t chunk;      // and within its row
   uint32_t seg;        // this wave's segment of the tile in pass 0
 
   __device__ __forceinline__ void init(const void* p, int64_t stride_elems, int n, int tid) {
@@ -244,7 +245,8 @@ struct PkRows {
     row = tid / kChunks;
     const int c = tid % kChunks;
     static_assert(kRowsPerPass % 16 == 0, "the swizzle repeats every 16 rows");
-    off = (uint32_t)row * stride + (uint32_t)((c ^ pk_swz<D>(row)) * 16);
+    chunk = (uint32_t)((c ^ pk_swz<D>(row)) * 16);
+    off = (uint32_t)row * stride + chunk;
     seg = (uint32_t)(tid >> 6) * 1024u;
   }
   // Rows [64 n, 64 n + 64) to lds.
@@ -252,7 +254,7 @@ struct PkRows {
   __device__ __forceinline__ void load(int n, uint8_t* lds) const {
     const int64_t at = (int64_t)n * 64 * stride;
     const __amdgpu_buffer_rsrc_t rs = pk_rsrc(base + at, bytes - at);
-    const uint32_t end = LAST ? off - (uint32_t)row * stride + (uint32_t)(rows - 1 - 64 * n) * stride : kPkNowhere;
+    const uint32_t end = LAST ? chunk + (uint32_t)(rows - 1 - 64 * n) * stride : kPkNowhere;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(

@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
   };
 
   const PkLane<D> at(lane);
-  bool unclean = false, unclean_q = false;  // dO, Q hold inf or NaN in tiles that see some keys only in part
+  bool unclean = false;  // dO or Q holds inf or NaN in tiles that see some keys only in part
   // A sub-tile of 32 queries. Entry x of this lane is query i0 + 8 (x / 4) + 4 half + x % 4.
   auto sub = [&](auto masked, const uint8_t* qt, const uint8_t* gt, const float* nl, const float* nd, int st, int i0)
                  __attribute__((always_inline)) {
@@ -515,8 +515,7 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
       const int ks = i / 2 / DB, db = i / 2 % DB;
       uint4 q[1] = {c[i % PRE]};
       if constexpr (decltype(masked)::value) {
-        const bool any = pk_clear_not_finite<E>(q);
-        (i % 2 == 0 ? unclean : unclean_q) |= any;
+        unclean |= pk_clear_not_finite<E>(q);
       }
       if (i % 2 == 0)
         av[db] = mma(E{}, q[0], pb[ks], av[db]);
@@ -557,13 +556,12 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
       tile(PkInt<1>{});
     }
     if (n < total) tile(PkInt<0>{});
-    if (__builtin_expect(unclean | unclean_q, 0)) {
+    if (__builtin_expect(unclean, 0)) {
       for (int x = t0; x < t0 + total; ++x) {
         const int h = x / per, i0 = 64 * (first + x % per);
         for (int i = i0; i < min(i0 + 64, min(64 * full, lq)); ++i) {
-          if (unclean) pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, av);
-          if (unclean_q)
-            pk_add_not_finite<E, true>(qbase + (int64_t)i * p.qst + (int64_t)h * p.qsh, half, key <= i + shift, ak);
+          pk_add_not_finite<E>(gbase + (int64_t)i * p.gst + (int64_t)h * p.gsh, half, key <= i + shift, av);
+          pk_add_not_finite<E, true>(qbase + (int64_t)i * p.qst + (int64_t)h * p.qsh, half, key <= i + shift, ak);
         }
       }
     }
