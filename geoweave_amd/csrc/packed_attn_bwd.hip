@@ -20,10 +20,11 @@
 // times the others' dO beside a key with 2^6 times the others' v left the dK of the keys behind it 5 times their bound
 // off.) The powers are exact and taken out of the fp32 sums again.
 //
-// Bound as the forward is, by the matrix cores and the vector unit: six sequences of 3,013 to 4,795 tokens,
-// 16 heads of 64 in bf16, dQ 552 us (1.01 PFLOP/s, matrix cores busy 60 % of the time), dK/dV 790 us (0.95, 54 %),
-// the statistics 28 us; the same with heads of 128 dQ 1,016 us (1.1 PFLOP/s), dK/dV 1,660 (0.90). 96 causal sequences of 17 to 697 tokens, 16 heads over 8: 27 + 54 + 79 us;
-// without the lists of tiles by falling work 24 + 61 + 103.
+// Bound as the forward is, by the matrix cores and the vector unit (smallest of four traced passes): six
+// sequences of 3,013 to 4,795 tokens, 16 heads of 64 in bf16, dQ 554 us (1.01 PFLOP/s, matrix cores busy 60 % of the
+// time), dK/dV 789 us (0.95, 52 %), the statistics 28 us; the same with heads of 128 dQ 1,028 us (1.1 PFLOP/s), dK/dV
+// 1,672 (0.90). Causal, fp16, 16 heads over 4 of 128: 55 + 568 + 940 us. 96 causal sequences of 17 to 697 tokens, 16
+// heads over 8 of 64: 26 + 55 + 81 us; the lists of tiles by falling work took 61 + 103 to 54 + 79.
 //
 // Rows behind a sequence's end add 0 to every gradient, and rows that see no key have P = 0.
 #include <math.h>
@@ -225,8 +226,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   if (kFp16) nlse += (float)kFitStart - kPScale<E>;
   // dP - delta: in bf16 at D = 128 delta is where the products start, in a register block of its own; at D = 64,
   // where three waves share a SIMD's registers, it is added afterwards (with the block 124 bytes of
-  // scratch a lane and 860 us for 563 on 6 scenes of 2 to 8 views), and so it is in fp16 (581 us with the block,
-  // 560 without).
+  // scratch a lane and half as much time again on 6 sequences of 3,013 to 4,795 tokens), and so it is in fp16 (4 % more
+  // with the block).
   constexpr bool kAddDelta = D == 64 || kFp16;
   const float ndelta = p.ndelta[srow];
   f32x16 dp0;
@@ -261,14 +262,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void packed_bwd_dq_kernel(con
   };
   // Three steps: the products S and dP while the column operands of K are read; dS; the product dQ while
   // `next` reads the next sub-tile's row operands. Kept in this order at D = 64, where that fits three
-  // waves per SIMD (6 scenes of 2 to 8 views: 544 us, 583 with two; left to the compiler 546 with two).
+  // waves per SIMD (with two the six sequences above took 7 % longer; left to the compiler, two waves as long as three).
   auto step = []() __attribute__((always_inline)) {
     if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
   };
   bool unclean = false;  // K holds inf or NaN in tiles that some rows see only in part
   auto sub = [&](auto masked, const uint8_t* kt, int st, int j0, Rows& r, auto&& next) __attribute__((always_inline)) {
     // fp16 at D = 128: read behind the fit, whose branch they would have to outlive (100 bytes of scratch a lane and
-    // 657 us for 548 on 6 causal sequences of 3,013 to 4,795 tokens, 16 heads over 4).
+    // 20 % more time).
     constexpr bool kLate = kFp16 && D == 128;
     uint4 kc[2 * DB];
     auto columns = [&]() __attribute__((always_inline)) {
@@ -466,8 +467,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
       dp[4 * g + 3] = y.w;
     }
     // Operands of the products in the order of their use, read PRE products ahead; the scheduling barriers
-    // keep the compiler from reading them all at once, for which there are no registers (759 us for 794
-    // on 6 scenes of 2 to 8 views).
+    // keep the compiler from reading them all at once, for which there are no registers (4 % less time on the
+    // six sequences above).
     constexpr int PRE = 2;
     auto row = [&](int i) __attribute__((always_inline)) { return i < KS ? at.row(qt, st, i) : at.row(gt, st, i - KS); };
     // Columns for each 16 queries and 32 dims: of dO, then of Q.
@@ -593,8 +594,8 @@ __global__ __launch_bounds__(256, 2) void packed_bwd_dkv_kernel(const PackedBwdP
 // w and w + 4 share 32 keys. The first holds K and dV: S, P and P^T dO. The second holds V and dK: dP, dS
 // and dS^T Q, with P from the first through LDS in fp32. A barrier in the middle of a tile hands P over; the
 // two meet on one SIMD, where the products of one run beside the weights of the other. Six sequences of 3,013 to
-// 4,795 tokens, 16 heads, bf16: 1,660 us, 2,062 with one wave per SIMD that holds all four, and longer still with dV
-// and dK in a pass each.
+// 4,795 tokens, 16 heads, bf16: 1,660 to 1,670 us, 2,062 with one wave per SIMD that holds all four, and longer still
+// with dV and dK in a pass each. 12 bytes of scratch a lane, outside the loop.
 template <typename E>
 __global__ __launch_bounds__(512, 2) void packed_bwd_dkv_pair_kernel(const PackedBwdParams p) {
   constexpr int D = 128, KS = D / 16, DB = D / 32, BN = kBwdTile;

@@ -19,8 +19,9 @@
 // transposing LDS reads. The next 32 keys' scores are issued before the current weights are formed.
 //
 // Bound by the matrix cores and the vector unit together (one exp2, half a pack and an add per score): 43,968
-// tokens x 16 heads of 64 in bf16 7.4 to 7.7 ms, 1.02 to 1.07 PFLOP/s with the matrix cores busy 55 % of the
-// time; 12 causal sequences of up to 8,844 tokens, 16 heads over 4 of 128 in fp16, 1.46 ms, 1.0 PFLOP/s (61 %).
+// tokens x 16 heads of 64 in bf16 7.6 to 7.8 ms, 1.01 to 1.04 PFLOP/s with the matrix cores busy 55 % of the
+// time; 12 causal sequences of up to 8,844 tokens, 16 heads over 4 of 128 in fp16, 1.50 ms, 0.98 PFLOP/s (57 %).
+// Heads of 128 keep 36 to 40 bytes of scratch a lane, written and read outside the loops.
 // Tiles by falling work, as in the backward, need a launch of their own here (7 to 14 us) and
 // saved 4 us of 57 on 96 short sequences, 20 of 428 on six long ones.
 //
@@ -301,7 +302,9 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackedFwdParams 
 
 // What a call launches, from the sizes that the host knows.
 // - Few-rows kernel (rows_attn_fwd.hip): where a sequence's rows are few on average and its keys many, the
-//   sequences of at most kRowsMax rows are split over all workgroups there; the tile kernel skips them.
+//   sequences of at most kRowsMax rows are split over all workgroups there; the tile kernel skips them. Up to 1,024
+//   sequences, since each of its workgroups scans them all: one query of 1,100 sequences of 600 keys, 8 heads of 64,
+//   took 539 us there and takes 273 in tiles of 128 rows; 4,000 sequences, 4 heads, 1,906 and 436.
 // - Tile kernel: rows in blocks of 128 (D = 64: or 256), and the keys of each tile cut into `split` parts
 //   where the tiles alone leave workgroup slots (two per CU) empty.
 struct FwdPlan {

@@ -14,10 +14,10 @@
 // Bound by memory: each element is read and written once. A workgroup takes TT tokens x all
 // heads of q and k; a thread keeps one pair group (V pairs: V elements of the first half and V of
 // the second) and walks over (token, head) rows, two rows' loads in flight, the first of them issued
-// before the angles are formed (the angles cost 1 to 2 us of a pass of 48 views). Eight tokens and two rows in flight: 65,952 tokens x 20 heads of 128 in bf16 139 us
-// (4.9 TB/s, what a large copy reaches), 16 tokens and four rows 161, four tokens and one row 135;
-// 9,973 tokens x 24 heads of 80 in fp32 53, 70 and 61 us. V is the widest of 8, 4, 2, 1 elements that
-// divides every half block and every stride.
+// before the angles are formed (the angles cost 1 to 2 us of a pass of 48 views). Eight tokens and two rows in
+// flight: 65,952 tokens x 20 heads of 128 in bf16 140 us (4.9 TB/s, what a large copy reaches), 16 tokens and
+// four rows 161, four tokens and one row 135; 9,973 tokens x 24 heads of 80 in fp32 53, 70 and 61 us. V is the
+// widest of 8, 4, 2, 1 elements that divides every half block and every stride.
 #include <math.h>
 #include <string.h>
 
@@ -192,8 +192,9 @@ __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(const RotParam
 // Blocks whose halves are not whole 16-byte (8-byte for the 16-bit types) groups: a wave reads whole
 // rows 16 bytes at a time, keeps them in its own LDS rows, and each thread fetches the partners of its
 // elements from there, wherever they lie. No barrier: a wave's LDS accesses are in order. 9,973 tokens x
-// 24 heads of 80 in fp32 by blocks of 18, 14, 20, 20 (four rows in flight): 70 us, with pairs of single
-// elements 78.
+// 24 heads of 80 in fp32 by blocks of 18, 14, 20, 20: 53 to 60 us (2.6 to 2.9 TB/s; 39 where the last-level cache
+// still holds the inputs), bound by the reads of single partners, pairs and angles from LDS; pairs of single elements
+// took 78 us where rows through LDS took 70 (both with four rows in flight).
 // ---------------------------------------------------------------------------------------
 template <typename E>
 __global__ __launch_bounds__(kRotThreads) void rotary_staged_kernel(const RotParams p) {

@@ -8,8 +8,9 @@
 // Bound by memory: each K and V row of a key head is read once, by one wave, for the up to 16 rows
 // (token, head of the group) that share it. No LDS tile: a wave takes 32 keys at a time straight into
 // the registers that the products read, the next 32 in flight meanwhile (16 KB per wave at D = 128).
-// One token of 64 sequences of up to 32,976 keys, 32 heads over 8 of 128, pages of 16, bf16: 557 us, 5.0
-// TB/s; five tokens of 8 sequences of up to 24,835 keys, 16 heads of 64: 95 us, 4.7 TB/s.
+// One token of 64 sequences of up to 32,976 keys, 32 heads over 8 of 128, pages of 16, bf16: 557 to 572 us, 5.0
+// TB/s; five tokens of 8 sequences of up to 24,835 keys, 16 heads of 64: 95 us, 4.7 TB/s. Many new tokens are right
+// but read all keys once per 16 rows.
 // S^T = K Q^T (16x16x32): lane (g, i) reads 16 bytes of rows i and 16 + i and then holds
 // the scores of keys 16 t + 4 g + r for row i. O^T += V^T P^T: the lane reads D / 16 dims of the 8
 // rows that its scores stand for; exchanging 16-bit halves between those registers gives the
@@ -573,7 +574,10 @@ int rows_attn(int dtype, int D, bool paged, RowsParams p, void* workspace, hipSt
 
 }  // namespace gw
 
-// Row tiles that reach sixteen workgroups per CU are not split.
+// Row tiles that reach sixteen workgroups per CU are not split: every workgroup of a split call scans the lengths, and
+// even batches lose by it (32 heads over 8 of 64, pages of 16, 512 sequences of 1,000 keys 224 us, 232 split; of 200
+// keys 44 and 74; 5,000 of 20 keys, one head, 32 and 221). One sequence of 60,000 keys among 511 of 1,000 is the
+// price: 702 us, 274 split.
 static bool paged_split(int64_t B, int64_t N, int64_t Hq, int64_t Hk) {
   return B * ((N * (Hq / Hk) + gw::kRows - 1) / gw::kRows) * Hk < 4096;
 }
