@@ -11,6 +11,7 @@
 // One token of 64 sequences of up to 32,976 keys, 32 heads over 8 of 128, pages of 16, bf16: 557 to 572 us, 5.0
 // TB/s; five tokens of 8 sequences of up to 24,835 keys, 16 heads of 64: 95 us, 4.7 TB/s. Many new tokens read all
 // keys once per 16 rows: 1,374 tokens x 16 heads of 64 over 20,000 keys 655 us.
+//
 // S^T = K Q^T (16x16x32): lane (g, i) reads 16 bytes of rows i and 16 + i and then holds
 // the scores of keys 16 t + 4 g + r for row i. O^T += V^T P^T: the lane reads D / 16 dims of the 8
 // rows that its scores stand for; exchanging 16-bit halves between those registers gives the
