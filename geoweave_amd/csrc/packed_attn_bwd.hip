@@ -3,7 +3,8 @@
 //
 // With P the softmax weights (formed again from the forward's lse) and delta_i = o_i . do_i, from o as it
 // was before its rounding (the forward keeps what the rounding left: where a row sees few keys, dP - delta
-// nearly cancels, and a delta from the rounded o would double the error of dQ and dK):
+// nearly cancels, and a delta from the rounded o would double the error of dQ and dK; what the rounding of the
+// forward's weights left in o, half a step of P|V| at most, stays in delta):
 //   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q.
 // Two passes, so that every gradient is summed by one workgroup in a fixed order: the dQ pass has the
 // forward's shape (rows of a key head in registers, K and V tiles through LDS: three products per
