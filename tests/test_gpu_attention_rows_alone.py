@@ -1,11 +1,11 @@
-"""A row's o and lse depend, bit by bit, on its query and on what it sees alone: not on later keys, nor on the
-queries of other tokens and other heads that share its tile."""
+"""A row's o, lse and dq depend, bit by bit, on its query and on what it sees alone: not on later keys, nor on the
+queries of other tokens and other heads that share its tile; a key's dk and dv on the queries that see it."""
 import pytest
 import torch
 
 from geoweave_amd.custom_flash_attn.packed_flash_attn import packed_flash_attn_inference_func
 from geoweave_amd.custom_flash_attn.paged_flash_attn import paged_flash_attn_inference_func
-from test_gpu_packed_attention import make
+from test_gpu_packed_attention import make, step
 from test_gpu_paged_attention import make as make_paged
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +71,25 @@ def test_new_tokens_over_a_cache(gpu_device, dtype, d, hq, hk):
     loud[:, 1::2] *= 9
     for a, b in zip(want, call(loud, k)):
         assert torch.equal(a[:, ::2], b[:, ::2]) and not torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hq,hk", HEADS)
+@pytest.mark.parametrize("lens_q,lens_k", [([700, 33], None), ([150], [6000]), ([5], [900])])
+def test_gradients(gpu_device, dtype, d, hq, hk, lens_q, lens_k):
+    args = make(lens_q, lens_k, hq, hk, d, dtype, 33)
+    n_q, n_k = args[4][1], args[5][1]
+    shift, cut = n_k - n_q, n_q // 2
+    _, dq, dk, dv = step(args, gpu_device, True)
+    q, k, v, do, cu_q, cu_k = (t.clone() if torch.is_tensor(t) else t for t in args)
+    k[cut + shift:n_k] *= 5
+    v[cut + shift:n_k] += 3
+    _, dq2, _, _ = step((q, k, v, do, cu_q, cu_k), gpu_device, True)
+    assert torch.equal(dq[:cut], dq2[:cut]) and torch.equal(dq[n_q:], dq2[n_q:]) and not torch.equal(dq, dq2)
+    q, k, v, do, cu_q, cu_k = (t.clone() if torch.is_tensor(t) else t for t in args)
+    q[:cut] *= 4
+    do[:cut] -= 2
+    _, _, dk2, dv2 = step((q, k, v, do, cu_q, cu_k), gpu_device, True)
+    first = cut + shift  # the first key that none of those queries sees
+    for a, b in ((dk, dk2), (dv, dv2)):
+        assert torch.equal(a[first:], b[first:]) and not torch.equal(a, b)
