@@ -13,8 +13,8 @@ struct RowsParams {
   uint16_t* o;
   uint16_t* rest;       // nullable (packed): [Tq][H][D], what the rounding of o left
   float* lse;           // nullable
-  float* part;          // parts of cut row tiles: [slot][Hk][16][D] normalised outputs,
-  float* part_lse;      // [slot][Hk][16] log2 sums
+  float* part;          // parts of cut row tiles: [slot][Hk][rows of a tile][D] normalised outputs,
+  float* part_lse;      // [slot][Hk][rows of a tile] log2 sums
   int2* cut;            // [tile] of a split call: where a row tile's parts are kept, and how many (paged: tile
                         // sequence * tiles of one + tile; packed: 2 sequence + tile)
   // Paged: table [B][table_width] page numbers (row stride table_stride), lens [B].
@@ -41,13 +41,13 @@ constexpr int kRowsMax = 32;
 // Parts per key head to aim at: about four workgroups per CU over all heads.
 inline int rows_want(int64_t Hk) { return (int)(1024 / Hk > 0 ? 1024 / Hk : 1); }
 // Row tiles of a call at most: the join's workgroups, and the entries of `cut`.
-inline int64_t rows_tiles(bool paged, int64_t n, int64_t Tq, int64_t G) {
-  return paged ? n * ((Tq * G + 15) / 16) : 2 * (n + 2);
+inline int64_t rows_tiles(bool paged, int64_t n, int64_t Tq, int64_t G, int64_t rows = 16) {
+  return paged ? n * ((Tq * G + rows - 1) / rows) : 2 * (n + 2);
 }
 // Workspace of a split call. A tile is cut where its keys exceed the part length, so it has fewer than
 // two parts per part length of keys, and all cut tiles fewer than 2 want.
-inline size_t rows_workspace(int64_t tiles, int64_t Hk, int64_t D) {
-  return (size_t)2 * rows_want(Hk) * Hk * 16 * (D + 1) * sizeof(float) + (size_t)tiles * sizeof(int2);
+inline size_t rows_workspace(int64_t tiles, int64_t Hk, int64_t D, int64_t rows = 16) {
+  return (size_t)2 * rows_want(Hk) * Hk * rows * (D + 1) * sizeof(float) + (size_t)tiles * sizeof(int2);
 }
 // Workgroups of the attention launch. Packed: a sequence of at most kRowsMax rows has one or two tiles, and all have
 // no more than the rows in all allow.
