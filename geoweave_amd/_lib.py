@@ -19,6 +19,8 @@ GW_OK = 0
 GW_DTYPE_BF16 = 0
 GW_DTYPE_FP16 = 1
 GW_DTYPE_FP32 = 2
+GW_CACHE_16BIT = 0
+GW_CACHE_FP4 = 1
 
 _i64 = ctypes.c_int64
 _p = ctypes.c_void_p
@@ -179,6 +181,23 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64, _p, _p, _i64p, _p, _i64, _i64, _i64, _i64, _i64,
          _i64, _i64, _i64, ctypes.c_int, ctypes.c_float, _p, _sz, _p],
+    ),
+    "gw_paged_kv_append": (
+        ctypes.c_int,
+        [ctypes.c_int, _p, _i64p, _p, _i64, _p, _i64p, _p, _i64p, _i64, _i64, ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p,
+         _p, _i64p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, _p, _i64p, ctypes.c_int,
+         ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_double), _p],
+    ),
+    "gw_paged_kv_read": (
+        ctypes.c_int,
+        [ctypes.c_int, ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _p, _p, _p],
+    ),
+    "gw_paged_attn_fp4_fwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "gw_paged_attn_fp4_fwd": (
+        ctypes.c_int,
+        [ctypes.c_int, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64, _p, _p, _i64p, _p, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_float, _p, _sz, _p],
     ),
 }
 

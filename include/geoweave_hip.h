@@ -720,6 +720,62 @@ int gw_paged_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const 
                       int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size, int64_t table_width,
                       int causal, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Paged key-value caches: the new tokens' k and v written into their slots, k and q rotated on the
+ * way, and sequences read back as packed rows.
+ *
+ * A cache is [pages, page_size, Hk] rows of D dims (64 or 128) through {stride_page, stride_slot, stride_h}:
+ * GW_CACHE_16BIT: rows in the tokens' type, strides in elements. GW_CACHE_FP4: rows of D / 2 bytes, e2m1 codes
+ * two to a byte (the even dim in the low half), strides in bytes, and k_scales / v_scales [pages,
+ * page_size, Hk] rows of D / 32 bytes through strides of their own: the biased exponent of the power of
+ * two that 32 dims share (255: not a number). Rows are 16-byte aligned, scale rows aligned to their size.
+ *
+ * Append: k and v [n, N, Hk, D] (cu_new NULL) through {stride_b, stride_t, stride_h}, or packed [N, Hk, D] (N
+ * tokens in all, stride_b unused) with cu_new int32 [n + 1]; q alike with Hq heads (Hq = 0: none), turned into
+ * q_out, contiguous (it may not overlap an input). Token i of a sequence's m new ones is key lens - m + i: slot j % page_size of page
+ * block_table[b][j / page_size] for key j (row stride table_stride, unit column stride). A key below 0, behind
+ * the table, or in a page outside [0, pages) is not written, nor is a token of no sequence; every token's q is
+ * turned. Two new tokens for one slot leave unspecified contents there. pos, axis_dims and bases as in
+ * gw_rotary_axes (n_axes = 0: nothing is turned); dims behind the axes are not turned. 4 bits: 32 dims with an inf or NaN are kept as not a number.
+ * Rows must not overlap the inputs.
+ *
+ * Read: sequence b's keys 0 .. cu[b + 1] - cu[b] - 1 to rows cu[b] .. of k_out and v_out [tokens, Hk, D],
+ * contiguous, in dtype (16 bits: the cache's own). Rows whose key has no slot, and rows of no sequence, are zeros.
+ *
+ * bf16 or fp16. Tokens x heads and table_width * page_size below 2^31 - 2^12, tokens below 2^27. Table, lengths and bounds are read
+ * on the device only; bounds out of order give unspecified values and no access outside the tensors.
+ * ------------------------------------------------------------------------------------ */
+#define GW_CACHE_16BIT 0
+#define GW_CACHE_FP4 1
+int gw_paged_kv_append(int dtype, const void* q, const int64_t* q_strides, void* q_out, int64_t Hq, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t Hk, int64_t D,
+                       int cache_format, void* k_cache, const int64_t* k_cache_strides, void* k_scales,
+                       const int64_t* k_scale_strides, void* v_cache, const int64_t* v_cache_strides, void* v_scales,
+                       const int64_t* v_scale_strides, const int32_t* block_table, int64_t table_stride,
+                       const int32_t* lens, const int32_t* cu_new, int64_t n, int64_t N, int64_t pages, int64_t page_size,
+                       int64_t table_width, int pos_type, const void* pos, const int64_t* pos_strides, int n_axes,
+                       const int32_t* axis_dims, const double* bases, void* stream);
+int gw_paged_kv_read(int dtype, int cache_format, const void* k_cache, const int64_t* k_cache_strides,
+                     const void* k_scales, const int64_t* k_scale_strides, const void* v_cache,
+                     const int64_t* v_cache_strides, const void* v_scales, const int64_t* v_scale_strides,
+                     const int32_t* block_table, int64_t table_stride, const int32_t* cu, int64_t n, int64_t tokens,
+                     int64_t Hk, int64_t D, int64_t pages, int64_t page_size, int64_t table_width, void* k_out,
+                     void* v_out, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * gw_paged_attn_fwd over a cache of GW_CACHE_FP4: the same formulas over the values that the codes stand for,
+ * with the same arguments, limits and rules; k and v are codes and scales as in gw_paged_kv_append, of at most 2^36 bytes of
+ * codes each. All values enter the products exactly, the weights as two bf16 terms.
+ * ------------------------------------------------------------------------------------ */
+size_t gw_paged_attn_fp4_fwd_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D);
+int gw_paged_attn_fp4_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const void* k_scales, const int64_t* k_scale_strides, const void* v, const int64_t* v_strides,
+                          const void* v_scales, const int64_t* v_scale_strides, const int32_t* block_table,
+                          int64_t table_stride, const int32_t* lens, void* o, const int64_t* o_strides, float* lse,
+                          int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size,
+                          int64_t table_width, int causal, float softmax_scale, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
