@@ -6,12 +6,13 @@
 // The rotation is that of rotary_axes.hip: angles in 64 bits, products and sums in fp32, each rounded once (no fused
 // multiply-add: so the 4-bit codes of k are those of the same steps taken one by one).
 //
-// Bound by memory: rows are read and written once, 16 bytes (eight dims) per thread. A workgroup takes TT tokens; its
-// waves first find the tokens' slots and form their cosines and sines in LDS, with the first rows' loads in
-// flight. A thread keeps its eight dims of a row and walks over (token, head) rows; the partners of its dims come from
-// the wave's own copy of its rows in LDS, W at a time (W: the widest of 8, 4, 2, 1 that divides every half block).
-// 4 bits: the 32 values of a power of two lie in four neighbouring lanes, which exchange their largest within the
-// vector unit.
+// Bound by memory: rows are read and written once, 16 bytes (eight dims) per thread. A workgroup takes TT tokens, a power
+// of two. A thread keeps one token and eight dims of a row and walks over the heads, so that its slot, its
+// cosines and sines (formed once for all heads, in LDS) and its addresses stay in registers; a wave's rows are
+// neighbouring tokens of one head, which lie one behind the other in a head-major cache (4 bits: 32 bytes a row). The partners of
+// its dims come from the wave's own copy of its rows in LDS, W at a time (W: the widest of 8, 4, 2, 1 that divides every half
+// block). 4 bits: the 32 values of a power of two lie in four neighbouring lanes, which exchange their largest
+// within the vector unit.
 #include <math.h>
 #include <string.h>
 
@@ -23,8 +24,9 @@ namespace gw {
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kKvMaxTokens = 8;  // tokens of a workgroup
-constexpr int kKvUnroll = 2;     // rows of a thread whose loads are in flight together
+constexpr int kKvLogTokens = 3;   // tokens of a workgroup: up to 8
+constexpr int kKvMaxTokens = 1 << kKvLogTokens;
+constexpr int kKvUnroll = 4;     // rows of a thread whose loads are in flight together
 constexpr int kKvMaxPairs = 64;
 
 struct KvCache {
@@ -56,17 +58,18 @@ struct KvAppendParams {
   const void* pos;
   int64_t pb, pt, pa;
   int pos_type;
-  int Hq, Hk, D, TT, pairs;
+  int Hq, Hk, D, pairs;
+  int TT;  // log2 of a workgroup's tokens
   double freq[kKvMaxPairs];
   uint8_t axis[kKvMaxPairs];
-  int8_t dim_pair[2 * kKvMaxPairs], dim_other[2 * kKvMaxPairs];  // a dim's pair (-1: not turned), distance to its partner
+  int8_t dim_pair[2 * kKvMaxPairs], dim_other[2 * kKvMaxPairs];  // a dim's pair, distance to its partner (0: not turned)
 };
 
 struct KvReadParams {
   KvCache cache[2];
   uint16_t* out[2];  // k, v: [T][Hk][D]
   KvTable t;
-  int Hk, D, TT;
+  int Hk, D, TT;  // TT: as above
 };
 
 // The sequence of packed token t: the last whose bound is not above t (64 bounds a step), by one wave.
@@ -91,17 +94,43 @@ __device__ __forceinline__ int2 kv_slot(const KvTable& t, int seq, int64_t key) 
   return make_int2((uint32_t)id < (uint32_t)t.pages ? id : -1, (int)key - pg * t.page);
 }
 
+// A token's rows in a cache.
+struct KvRows {
+  uint8_t* rows;
+  uint8_t* scales;
+};
 template <bool FP4>
-__device__ __forceinline__ uint8_t* kv_row(const KvCache& c, int2 at, int head) {
-  return c.rows + at.x * c.page + at.y * c.slot + head * c.head;
+__device__ __forceinline__ KvRows kv_rows(const KvCache& c, int2 at) {
+  return KvRows{c.rows + at.x * c.page + at.y * c.slot, FP4 ? c.scales + at.x * c.spage + at.y * c.sslot : nullptr};
 }
-__device__ __forceinline__ uint8_t* kv_scale(const KvCache& c, int2 at, int head) {
-  return c.scales + at.x * c.spage + at.y * c.sslot + head * c.shead;
+
+// W consecutive 16-bit values as floats.
+template <typename E, int W>
+__device__ __forceinline__ void kv_floats(const uint8_t* at, float* f) {
+  if constexpr (W == 8) {
+    unpack8<E>(*reinterpret_cast<const uint4*>(at), f);
+  } else if constexpr (W == 4) {
+    const uint2 x = *reinterpret_cast<const uint2*>(at);
+    unpack2(E{}, x.x, f[0], f[1]);
+    unpack2(E{}, x.y, f[2], f[3]);
+  } else if constexpr (W == 2) {
+    unpack2(E{}, *reinterpret_cast<const uint32_t*>(at), f[0], f[1]);
+  } else {
+    f[0] = ld_f32(E{}, at, 0);
+  }
 }
 
 __device__ __forceinline__ uint32_t kv_quad_max(uint32_t x) {
   x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor1, 0xF, 0xF, true));
   return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor2, 0xF, 0xF, true));
+}
+
+// First token of a workgroup. Workgroups go to the eight XCDs in turn; in 4 bits each XCD takes a run of neighbouring
+// tokens, so that lines which several workgroups write in part (the scales of 64 slots are one) are put together in one
+// L2 (six scenes of 16 heads of 64 into 4 bits and back: 134 -> 131 us; whole lines of 16 bits lose 1 % by it).
+template <bool FP4>
+__device__ __forceinline__ int kv_first_token(int TT) {
+  return (FP4 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x) << TT;
 }
 
 template <typename E, bool FP4, int W>
@@ -110,140 +139,145 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(const KvAppendPar
   __shared__ int2 where[kKvMaxTokens];
   __shared__ __align__(16) uint8_t rows_s[kKvThreads / 64][kKvUnroll * 64 * 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t0 = blockIdx.x * p.TT, nt = min(p.TT, p.t.T - t0);
+  const int t0 = kv_first_token<FP4>(p.TT), nt = min(1 << p.TT, p.t.T - t0);
+  if (nt <= 0) return;
   const int H0 = p.Hq, H1 = p.Hq + p.Hk, HT = p.Hq + 2 * p.Hk;
   const int C = p.D >> 3, shift = p.D == 64 ? 3 : 4;
-  const int r0 = threadIdx.x >> shift, c = threadIdx.x & (C - 1);
-  const int R = (kKvThreads >> shift) * gridDim.y;
-  const int rows = nt * HT;
-  const int step_t = R / HT, step_h = R - step_t * HT;
+  const int c = threadIdx.x & (C - 1), r0 = threadIdx.x >> shift;
+  const int tok = r0 & ((1 << p.TT) - 1);  // this thread's token
+  const int R = (kKvThreads >> shift) >> p.TT;  // heads of a round
+  const int step = R * gridDim.y;
+  int head = (r0 >> p.TT) + R * blockIdx.y;
+  if (tok >= nt) head = HT;  // nothing to do
 
-  int row = r0 + (kKvThreads >> shift) * blockIdx.y, tok = row / HT, head = row - tok * HT;
+  const int t = t0 + min(tok, nt - 1);
+  const int b = p.t.N ? t / p.t.N : 0, i_in_b = t - b * p.t.N;
+  // What differs between q, k and v is held in registers and selected: an index into the arguments would be a load.
+  auto row_of = [&](const KvIn& in) __attribute__((always_inline)) { return in.x + b * in.sb + i_in_b * in.st + c * 8; };
+  const uint16_t *const q_row = row_of(p.in[0]), *const k_row = row_of(p.in[1]), *const v_row = row_of(p.in[2]);
+  const uint64_t q_head = p.in[0].sh, k_head = p.in[1].sh, v_head = p.in[2].sh;
   uint4 x[kKvUnroll];
-  int at_tok[kKvUnroll], at_head[kKvUnroll];
-  auto load = [&](int u) __attribute__((always_inline)) {
-    at_tok[u] = row < rows ? tok : -1;
-    at_head[u] = head;
-    if (row < rows) {
-      const int s = head < H0 ? 0 : head < H1 ? 1 : 2;
-      const KvIn& in = p.in[s];
-      const int t = t0 + tok, b = p.t.cu ? 0 : t / p.t.N;
-      x[u] = *reinterpret_cast<const uint4*>(in.x + b * in.sb + (int64_t)(t - b * p.t.N) * in.st +
-                                             (int64_t)(head - (s == 0 ? 0 : s == 1 ? H0 : H1)) * in.sh + c * 8);
-    }
-    row += R;
-    tok += step_t;
-    head += step_h;
-    if (head >= HT) {
-      head -= HT;
-      ++tok;
+  auto load = [&](uint4(&to)[kKvUnroll], int first) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kKvUnroll; ++u) {
+      const int h = first + u * step;
+      const uint16_t* base = h < H0 ? q_row : h < H1 ? k_row : v_row;
+      const uint64_t sh = h < H0 ? q_head : h < H1 ? k_head : v_head;
+      if (h < HT) to[u] = *reinterpret_cast<const uint4*>(base + (uint32_t)(h - (h < H0 ? 0 : h < H1 ? H0 : H1)) * sh);
     }
   };
-#pragma unroll
-  for (int u = 0; u < kKvUnroll; ++u) load(u);
+  load(x, head);
 
   // Slots of the tokens, a wave each; angles by all threads.
   for (int i = wave; i < nt; i += kKvThreads / 64) {
-    const int t = t0 + i;
     int2 at = make_int2(-1, 0);
     if (p.t.n > 0) {
       int seq;
       int64_t first, count = p.t.N;
       if (p.t.cu) {
-        seq = kv_sequence(p.t.cu, p.t.n, t, lane);
+        seq = kv_sequence(p.t.cu, p.t.n, t0 + i, lane);
         first = p.t.cu[seq];
         count = p.t.cu[seq + 1] - first;
       } else {
-        seq = t / p.t.N;
+        seq = (t0 + i) / p.t.N;
         first = (int64_t)seq * p.t.N;
       }
-      const int64_t in = t - first;
+      const int64_t in = t0 + i - first;
       if (in >= 0 && in < count) at = kv_slot(p.t, seq, p.t.lens[seq] - count + in);
     }
     if (lane == 0) where[i] = at;
   }
   for (int i = threadIdx.x; i < nt * p.pairs; i += kKvThreads) {
     const int tk = i / p.pairs, pr = i - tk * p.pairs;
-    const int t = t0 + tk, b = p.t.cu ? 0 : t / p.t.N;
-    const double pos = rot_position(p.pos, p.pos_type, b * p.pb + (int64_t)(t - b * p.t.N) * p.pt + p.axis[pr] * p.pa);
+    const int tt = t0 + tk, bb = p.t.N ? tt / p.t.N : 0;
+    const double pos = rot_position(p.pos, p.pos_type, bb * p.pb + (int64_t)(tt - bb * p.t.N) * p.pt + p.axis[pr] * p.pa);
     cs[tk * p.pairs + pr] = rot_cos_sin(pos * p.freq[pr], 1.0);
-  }
-  // This thread's dims by W: their pairs, and where the partners lie.
-  int pair[8 / W], other[8 / W];
-#pragma unroll
-  for (int i = 0; i < 8 / W; ++i) {
-    pair[i] = p.dim_pair[c * 8 + i * W];
-    other[i] = p.dim_other[c * 8 + i * W];
   }
   __syncthreads();
 
+  const int2 at = where[tok < nt ? tok : 0];
+  const KvRows k_to = kv_rows<FP4>(p.cache[0], at), v_to = kv_rows<FP4>(p.cache[1], at);
+  const uint64_t k_step = p.cache[0].head, v_step = p.cache[1].head, ks_step = p.cache[0].shead, vs_step = p.cache[1].shead;
+  // This thread's dims by W: where the partners lie (0: not turned), cosines, and sines with the partner's sign.
+  int other[8 / W];
+  float co[8], si[8];
+#pragma unroll
+  for (int i = 0; i < 8 / W; ++i) {
+    other[i] = p.dim_other[c * 8 + i * W];
+    const int pair = p.dim_pair[c * 8 + i * W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float2 a = other[i] ? cs[(tok < nt ? tok : 0) * p.pairs + pair + j] : make_float2(1.f, 0.f);
+      co[i * W + j] = a.x;
+      si[i * W + j] = other[i] > 0 ? -a.y : a.y;
+    }
+  }
+
   uint8_t* const mine = rows_s[wave];
-  const int turns = (rows + R * kKvUnroll - 1) / (R * kKvUnroll);  // the same for every thread
+  const int turns = (HT + step * kKvUnroll - 1) / (step * kKvUnroll);  // the same for every thread
   for (int n = 0; n < turns; ++n) {
+    uint4 next[kKvUnroll];
+    load(next, head + step * kKvUnroll);
 #pragma unroll
     for (int u = 0; u < kKvUnroll; ++u) *reinterpret_cast<uint4*>(mine + (u * 64 + lane) * 16) = x[u];
     lds_fence();
 #pragma unroll
     for (int u = 0; u < kKvUnroll; ++u) {
-      if (at_tok[u] < 0) continue;
-      const int hd = at_head[u], tk = at_tok[u];
+      const int h = head + u * step;
+      if (h >= HT) continue;
       float y[8];
       unpack8<E>(x[u], y);
-      if (hd < H1) {
+      if (h < H1) {
 #pragma unroll
         for (int i = 0; i < 8 / W; ++i) {
-          if (pair[i] < 0) continue;
-          uint16_t o[W];
-          memcpy(o, __builtin_assume_aligned(mine + (u * 64 + lane) * 16 + (i * W + other[i]) * 2, 2 * W), 2 * W);
-          const float2* t = cs + tk * p.pairs + pair[i];
+          if (other[i] == 0) continue;
+          float o[W];
+          kv_floats<E, W>(mine + (u * 64 + lane) * 16 + (i * W + other[i]) * 2, o);
 #pragma unroll
           for (int j = 0; j < W; ++j) {
 #pragma clang fp contract(off)
-            const float a = y[i * W + j] * t[j].x, b = ld_f32(E{}, o, j) * t[j].y;
-            y[i * W + j] = other[i] > 0 ? a - b : a + b;
+            const float a = y[i * W + j] * co[i * W + j], d = o[j] * si[i * W + j];
+            y[i * W + j] = a + d;
           }
         }
       }
-      if (hd < H0) {
-        *reinterpret_cast<uint4*>(p.q_out + ((int64_t)(t0 + tk) * H0 + hd) * p.D + c * 8) = pack_quad<E>(y);
+      if (h < H0) {
+        *reinterpret_cast<uint4*>(p.q_out + ((int64_t)t * H0 + h) * p.D + c * 8) = pack_quad<E>(y);
         continue;
       }
-      const int2 at = where[tk];
       if (at.x < 0) continue;
-      const bool is_v = hd >= H1;
-      const KvCache& cache = p.cache[is_v];
-      const int h = hd - (is_v ? H1 : H0);
-      uint8_t* dst = kv_row<FP4>(cache, at, h);
+      const bool is_v = h >= H1;
+      const uint32_t hk = h - (is_v ? H1 : H0);
+      uint8_t* dst = (is_v ? v_to.rows : k_to.rows) + hk * (is_v ? v_step : k_step);
       if constexpr (FP4) {
         uint32_t top = 0u;
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
         const uint32_t scale = fp4_scale(kv_quad_max(top));
         reinterpret_cast<uint32_t*>(dst)[c] = scale == kFp4NaN ? 0u : fp4_pack8(y, scale);
-        if ((c & 3) == 0) kv_scale(cache, at, h)[c >> 2] = (uint8_t)scale;
+        if ((c & 3) == 0) ((is_v ? v_to.scales : k_to.scales) + hk * (is_v ? vs_step : ks_step))[c >> 2] = (uint8_t)scale;
       } else {
         reinterpret_cast<uint4*>(dst)[c] = is_v ? x[u] : pack_quad<E>(y);
       }
     }
     lds_fence();
-    if (n + 1 < turns) {
+    head += step * kKvUnroll;
 #pragma unroll
-      for (int u = 0; u < kKvUnroll; ++u) load(u);
-    }
+    for (int u = 0; u < kKvUnroll; ++u) x[u] = next[u];
   }
 }
 
 // Sequence b's keys 0 .. cu[b + 1] - cu[b] - 1 to rows cu[b] .. of k and v; rows without a slot are zeros.
 template <typename E, bool FP4>
 __global__ __launch_bounds__(kKvThreads) void kv_read_kernel(const KvReadParams p) {
-  constexpr int U = 4;
   __shared__ int2 where[kKvMaxTokens];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t0 = blockIdx.x * p.TT, nt = min(p.TT, p.t.T - t0);
+  const int t0 = kv_first_token<FP4>(p.TT), nt = min(1 << p.TT, p.t.T - t0);
+  if (nt <= 0) return;
   const int HT = 2 * p.Hk, shift = p.D == 64 ? 3 : 4;
-  const int r0 = threadIdx.x >> shift, c = threadIdx.x & ((p.D >> 3) - 1);
-  const int R = (kKvThreads >> shift) * gridDim.y;
-  const int rows = nt * HT;
+  const int c = threadIdx.x & ((p.D >> 3) - 1), r0 = threadIdx.x >> shift;
+  const int tok = r0 & ((1 << p.TT) - 1);
+  const int R = (kKvThreads >> shift) >> p.TT, step = R * gridDim.y;
   for (int i = wave; i < nt; i += kKvThreads / 64) {
     int2 at = make_int2(-1, 0);
     if (p.t.n > 0) {
@@ -254,46 +288,37 @@ __global__ __launch_bounds__(kKvThreads) void kv_read_kernel(const KvReadParams 
     if (lane == 0) where[i] = at;
   }
   __syncthreads();
-  const int step_t = R / HT, step_h = R - step_t * HT;
-  int row = r0 + (kKvThreads >> shift) * blockIdx.y, tok = row / HT, head = row - tok * HT;
-  while (row < rows) {
-    uint4 x[U];
-    uint32_t s[U];
-    int at_tok[U], at_head[U];
+  if (tok >= nt) return;
+  const int2 at = where[tok];
+  const KvRows k_from = kv_rows<FP4>(p.cache[0], at), v_from = kv_rows<FP4>(p.cache[1], at);
+  const uint64_t k_step = p.cache[0].head, v_step = p.cache[1].head, ks_step = p.cache[0].shead, vs_step = p.cache[1].shead;
+  uint16_t *const k_out = p.out[0], *const v_out = p.out[1];
+  const int64_t to = (int64_t)(t0 + tok) * p.Hk * p.D + c * 8;
+  for (int head = (r0 >> p.TT) + R * blockIdx.y; head < HT; head += step * kKvUnroll) {
+    uint4 x[kKvUnroll];
+    uint32_t s[kKvUnroll];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      at_tok[u] = row < rows ? tok : -1;
-      at_head[u] = head;
+    for (int u = 0; u < kKvUnroll; ++u) {
+      const int h = head + u * step;
+      const bool is_v = h >= p.Hk;
       x[u] = make_uint4(0u, 0u, 0u, 0u);
       s[u] = 0u;
-      if (row < rows) {
-        const int2 at = where[tok];
-        if (at.x >= 0) {
-          const bool is_v = head >= p.Hk;
-          const KvCache& cache = p.cache[is_v];
-          const int h = head - (is_v ? p.Hk : 0);
-          const uint8_t* src = kv_row<FP4>(cache, at, h);
-          if constexpr (FP4) {
-            x[u].x = reinterpret_cast<const uint32_t*>(src)[c];
-            s[u] = kv_scale(cache, at, h)[c >> 2];
-          } else {
-            x[u] = reinterpret_cast<const uint4*>(src)[c];
-          }
+      if (h < HT && at.x >= 0) {
+        const uint32_t hk = h - (is_v ? p.Hk : 0);
+        const uint8_t* src = (is_v ? v_from.rows : k_from.rows) + hk * (is_v ? v_step : k_step);
+        if constexpr (FP4) {
+          x[u].x = reinterpret_cast<const uint32_t*>(src)[c];
+          s[u] = ((is_v ? v_from.scales : k_from.scales) + hk * (is_v ? vs_step : ks_step))[c >> 2];
+        } else {
+          x[u] = reinterpret_cast<const uint4*>(src)[c];
         }
-      }
-      row += R;
-      tok += step_t;
-      head += step_h;
-      if (head >= HT) {
-        head -= HT;
-        ++tok;
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (at_tok[u] < 0) continue;
-      const bool is_v = at_head[u] >= p.Hk;
-      uint16_t* dst = p.out[is_v] + ((int64_t)(t0 + at_tok[u]) * p.Hk + at_head[u] - (is_v ? p.Hk : 0)) * p.D + c * 8;
+    for (int u = 0; u < kKvUnroll; ++u) {
+      const int h = head + u * step;
+      if (h >= HT) continue;
+      uint16_t* dst = (h >= p.Hk ? v_out + (h - p.Hk) * p.D : k_out + h * p.D) + to;
       *reinterpret_cast<uint4*>(dst) = FP4 ? fp4_unpack8<E>(x[u].x, s[u]) : x[u];
     }
   }
@@ -303,13 +328,13 @@ __global__ __launch_bounds__(kKvThreads) void kv_read_kernel(const KvReadParams 
 // Host side
 // ---------------------------------------------------------------------------------------
 
-// Workgroups along x and y: few tokens a workgroup until the chip has four workgroups per CU, and where the tokens are
-// too few for that, a token's rows over several (each forms the angles again).
-dim3 kv_grid(int64_t T, int64_t heads, int64_t D, int unroll, int* TT) {
-  *TT = kKvMaxTokens;
-  while (*TT > 1 && (T + *TT - 1) / *TT < 1024) *TT >>= 1;
-  const int64_t x = (T + *TT - 1) / *TT, per = kKvThreads / (D / 8) * unroll;
-  int64_t y = (*TT * heads + per - 1) / per;
+// Workgroups along x and y, and the logarithm of a workgroup's tokens: few tokens a workgroup until the chip has four
+// workgroups per CU, and where the tokens are too few for that, a token's heads over several (each forms the angles again).
+dim3 kv_grid(int64_t T, int64_t heads, int64_t D, int* TT) {
+  *TT = kKvLogTokens;
+  while (*TT > 0 && ((T - 1) >> *TT) + 1 < 1024) --*TT;
+  const int64_t x = ((((T - 1) >> *TT) >> 3) + 1) * 8, per = (kKvThreads / (D / 8) >> *TT) * kKvUnroll;  // a multiple of 8
+  int64_t y = (heads + per - 1) / per;
   if (y > 1024 / x) y = 1024 / x > 0 ? 1024 / x : 1;
   return dim3((uint32_t)x, (uint32_t)y);
 }
@@ -387,7 +412,6 @@ extern "C" int gw_paged_kv_append(int dtype, const void* q, const int64_t* q_str
                kRotMaxAxes, n_axes);
   KvAppendParams p = {};
   int turned = 0, W = 8;
-  for (int i = 0; i < (int)D; ++i) p.dim_pair[i] = -1;
   for (int a = 0; a < n_axes; ++a) {
     GW_CHECK_ARG(axis_dims[a] >= 0 && axis_dims[a] % 2 == 0, "axis %d has %d dims: an even number is needed", a, axis_dims[a]);
     GW_CHECK_ARG(bases[a] > 0 && isfinite(bases[a]), "axis %d: the base must be positive and finite", a);
@@ -434,7 +458,7 @@ extern "C" int gw_paged_kv_append(int dtype, const void* q, const int64_t* q_str
   p.Hk = (int)Hk;
   p.D = (int)D;
   p.pairs = turned / 2;
-  const dim3 grid = kv_grid(T, Hq + 2 * Hk, D, kKvUnroll, &p.TT);
+  const dim3 grid = kv_grid(T, Hq + 2 * Hk, D, &p.TT);
   GW_CHECK_GRID(grid.x, kKvThreads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool fp4 = cache_format == GW_CACHE_FP4;
@@ -468,7 +492,7 @@ extern "C" int gw_paged_kv_read(int dtype, int cache_format, const void* k_cache
   p.t = KvTable{block_table, nullptr, cu, table_stride, pages == 0 ? 0 : (int)table_width, (int)pages, (int)page_size, (int)n, 0, (int)tokens};
   p.Hk = (int)Hk;
   p.D = (int)D;
-  const dim3 grid = kv_grid(tokens, 2 * Hk, D, 4, &p.TT);
+  const dim3 grid = kv_grid(tokens, 2 * Hk, D, &p.TT);
   GW_CHECK_GRID(grid.x, kKvThreads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache_format != GW_CACHE_FP4) {
