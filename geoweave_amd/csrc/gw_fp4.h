@@ -44,10 +44,10 @@ template <int B>
 __device__ __forceinline__ uint32_t fp4_pair(FP16, uint32_t w, float unit) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, B));
 }
+// The eight values of a word.
 template <typename E>
-__device__ __forceinline__ uint4 fp4_unpack8(uint32_t w, uint32_t scale) {
-  const float u = fp4_unit(scale);
-  return make_uint4(fp4_pair<0>(E{}, w, u), fp4_pair<1>(E{}, w, u), fp4_pair<2>(E{}, w, u), fp4_pair<3>(E{}, w, u));
+__device__ __forceinline__ uint4 fp4_operand(uint32_t w, float unit) {
+  return make_uint4(fp4_pair<0>(E{}, w, unit), fp4_pair<1>(E{}, w, unit), fp4_pair<2>(E{}, w, unit), fp4_pair<3>(E{}, w, unit));
 }
 
 }  // namespace

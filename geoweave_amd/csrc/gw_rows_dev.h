@@ -161,7 +161,9 @@ __device__ __forceinline__ float rows_sum(float x) {
 // take the parts in turn, each part's row one 16-byte load per thread, and are summed in group order.
 constexpr int kJoinParts = 1024;  // weights kept in LDS at a time
 
-template <typename E, int D, bool PAGED, int ROWS = kRows>
+//
+// UNITS: a row tile's first part is in slot cut.x (odd), the i-th behind it in slot cut.x + 2 i - 1.
+template <typename E, int D, bool PAGED, int ROWS = kRows, bool UNITS = false>
 __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
   constexpr int LPR = D / 4, GROUPS = 256 / LPR;
   __shared__ float w[kJoinParts];
@@ -180,12 +182,13 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
   // One part, or (packed bounds out of order, which may name more rows than there are) a tile that no
   // workgroup took and whose entry may hold anything.
   if (parts <= 1 || parts > 2 * p.want || (uint32_t)where.x > (uint32_t)(2 * p.want - parts)) return;
+  auto slot = [](int i) { return UNITS ? 2 * i - (i > 0) : i; };
   const int64_t step = (int64_t)p.Hk * ROWS;
   const int64_t at = ((int64_t)where.x * p.Hk + hk) * ROWS + row;
   // The largest log2 sum (NaN if one is).
   float mx = -INFINITY;
   for (int i = tid; i < parts; i += 256) {
-    const float x = p.part_lse[at + i * step];
+    const float x = p.part_lse[at + slot(i) * step];
     mx = x > mx || x != x ? x : mx;
     if (mx != mx) break;
   }
@@ -202,14 +205,14 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
     const int np = min(kJoinParts, parts - p0);
     __syncthreads();
     for (int i = tid; i < np; i += 256) {
-      const float x = p.part_lse[at + (p0 + i) * step];
+      const float x = p.part_lse[at + slot(p0 + i) * step];
       w[i] = x == -INFINITY ? 0.f : fexp2(x - mx);  // a part of which nothing is seen
     }
     __syncthreads();
 #pragma unroll 4
     for (int i = grp; i < np; i += GROUPS) {
       const float f = w[i];
-      const float4 x = reinterpret_cast<const float4*>(p.part + (at + (p0 + i) * step) * D)[c];
+      const float4 x = reinterpret_cast<const float4*>(p.part + (at + slot(p0 + i) * step) * D)[c];
       lt += f;
       out.x = fmaf(x.x, f, out.x);
       out.y = fmaf(x.y, f, out.y);

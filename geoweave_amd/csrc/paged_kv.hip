@@ -319,7 +319,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_read_kernel(const KvReadParams 
       const int h = head + u * step;
       if (h >= HT) continue;
       uint16_t* dst = (h >= p.Hk ? v_out + (h - p.Hk) * p.D : k_out + h * p.D) + to;
-      *reinterpret_cast<uint4*>(dst) = FP4 ? fp4_unpack8<E>(x[u].x, s[u]) : x[u];
+      *reinterpret_cast<uint4*>(dst) = FP4 ? fp4_operand<E>(x[u].x, fp4_unit(s[u])) : x[u];
     }
   }
 }
