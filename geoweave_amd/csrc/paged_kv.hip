@@ -481,7 +481,7 @@ extern "C" int gw_paged_kv_read(int dtype, int cache_format, const void* k_cache
   if (tokens == 0) return GW_OK;
   GW_CHECK_ARG(k_out && v_out, "a tensor is missing");
   GW_CHECK_ARG(cu || n == 0, "the bounds are missing");
-  GW_CHECK_ARG(aligned16(k_out) && aligned16(v_out), "the rows need 16-byte alignment");
+  GW_CHECK_ARG(aligned16(k_out) && aligned16(v_out), "k and v need 16-byte aligned rows");
   KvReadParams p = {};
   rc = kv_check_cache("key", cache_format, D, k_cache, k_cache_strides, k_scales, k_scale_strides, pages, &p.cache[0]);
   if (rc == GW_OK)

@@ -59,7 +59,8 @@ def _check_lists(q, k_cache, block_table, cache_seqlens):
                          f"[{q.shape[0]}, W] and [{q.shape[0]}]")
     if block_table.shape[1] * k_cache.shape[1] > MAX_KEYS or q.numel() // q.shape[-1] > MAX_KEYS:
         raise ValueError(f"keys of a sequence, and new tokens x heads, must not exceed {MAX_KEYS}")
-    if not (q.is_cuda and all(t.device == q.device for t in (k_cache, block_table, cache_seqlens))):
+    device = q.device
+    if not (q.is_cuda and k_cache.device == block_table.device == cache_seqlens.device == device):
         raise ValueError("q, the caches, block_table and cache_seqlens must be tensors of one GPU")
 
 

@@ -22,6 +22,7 @@ graph follows them. These functions have no gradients; caches are written in pla
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
@@ -57,10 +58,18 @@ def fp4_paged_cache(pages: int, page_size: int, heads: int, head_dim: int, devic
                       for n in (2, 32)))
 
 
-def _rows_fit(x: torch.Tensor, align: int) -> bool:
-    """Unit last stride, and rows aligned to ``align`` bytes."""
-    n = align // x.element_size()
-    return x.numel() == 0 or (x.stride(-1) == 1 and not any(s % n for s in _lib.row_strides(x)) and x.data_ptr() % align == 0)
+def _layout(x: torch.Tensor, align: int):
+    """(address, strides of the first three dims) of x [.., .., .., row], None where its rows are not contiguous and aligned to
+    ``align`` bytes."""
+    s0, s1, s2, s3 = x.stride()
+    at, units = x.data_ptr(), align // x.element_size() - 1
+    if s3 != 1 or (s0 | s1 | s2) & units or at & (align - 1):
+        if x.numel() == 0:
+            return None, _lib.strides3(0, 0, 0)
+        s0, s1, s2 = _lib.row_strides(x)  # dims of one entry have any strides
+        if s3 != 1 and x.shape[3] != 1 or (s0 | s1 | s2) & units or at & (align - 1):
+            return None
+    return at, _lib.strides3(s0, s1, s2)
 
 
 def cache_args(k_cache: Cache, v_cache: Cache):
@@ -69,79 +78,84 @@ def cache_args(k_cache: Cache, v_cache: Cache):
     fp4 = isinstance(k_cache, FP4Cache)
     if fp4 != isinstance(v_cache, FP4Cache):
         raise TypeError("k_cache and v_cache must both be 16-bit tensors or both FP4Cache")
-    args = []
-    for c in (k_cache, v_cache):
-        rows = c[0] if fp4 else c
-        if rows.dim() != 4:
-            raise ValueError(f"caches must be [pages, page_size, Hk, D], got {tuple(rows.shape)}")
-        d = rows.shape[3] * (2 if fp4 else 1)
-        if d not in NATIVE_HEAD_DIMS:
-            raise ValueError(f"head dims {NATIVE_HEAD_DIMS} are supported over a paged cache, got {d}")
-        if rows.shape[1] < 1 or rows.shape[2] < 1:
-            raise ValueError("pages must have at least one slot, and slots a head")
-        # Copying a cache to align it would cost more than the call: the caller lays it out.
-        if not _rows_fit(rows, 16):
-            raise ValueError("caches need a unit last stride and 16-byte aligned rows")
-        if fp4:
-            scales = c[1]
-            if rows.dtype != torch.uint8 or scales.dtype != torch.uint8:
-                raise TypeError("codes and scales of an FP4Cache must be uint8")
-            if scales.shape != rows.shape[:3] + (d // 32,):
-                raise ValueError(f"scales {tuple(scales.shape)} of codes {tuple(rows.shape)} must have a byte for 32 dims")
-            if not _rows_fit(scales, d // 32):
-                raise ValueError(f"scales need a unit last stride and rows aligned to their {d // 32} bytes")
-            if scales.device != rows.device:
-                raise ValueError("codes and scales must be tensors of one GPU")
-            args += [rows.data_ptr(), _lib.strides3(*_lib.row_strides(rows)), scales.data_ptr(),
-                     _lib.strides3(*_lib.row_strides(scales))]
-        else:
-            if rows.dtype not in (torch.float16, torch.bfloat16):
-                raise TypeError("Only support fp16 and bf16")
-            args += [rows.data_ptr(), _lib.strides3(*_lib.row_strides(rows)), None, None]
     k, v = (k_cache[0], v_cache[0]) if fp4 else (k_cache, v_cache)
-    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
-        raise ValueError(f"k and v caches {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype} differ")
-    return _lib.GW_CACHE_FP4 if fp4 else _lib.GW_CACHE_16BIT, k, k.shape[2], d, args
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
+        raise ValueError(f"caches must be [pages, page_size, Hk, D], got {tuple(shape)} and {tuple(v.shape)}")
+    pages, page, hk, d = shape
+    if fp4:
+        d *= 2
+    if d not in NATIVE_HEAD_DIMS:
+        raise ValueError(f"head dims {NATIVE_HEAD_DIMS} are supported over a paged cache, got {d}")
+    if page < 1 or hk < 1:
+        raise ValueError("pages must have at least one slot, and slots a head")
+    # Copying a cache to align it would cost more than the call: the caller lays it out.
+    kl, vl = _layout(k, 16), _layout(v, 16)
+    if kl is None or vl is None:
+        raise ValueError("caches need a unit last stride and 16-byte aligned rows")
+    device = k.device
+    if not fp4:
+        if k.dtype != v.dtype:
+            raise TypeError("All tensors must have the same type")
+        if k.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError("Only support fp16 and bf16")
+        if v.device != device:
+            raise ValueError("k_cache and v_cache must be tensors of one GPU")
+        return _lib.GW_CACHE_16BIT, k, hk, d, (*kl, None, None, *vl, None, None)
+    ks, vs = k_cache[1], v_cache[1]
+    if any(t.dtype != torch.uint8 for t in (k, ks, v, vs)):
+        raise TypeError("codes and scales of an FP4Cache must be uint8")
+    if ks.shape != (pages, page, hk, d // 32) or vs.shape != ks.shape:
+        raise ValueError(f"scales {tuple(ks.shape)} and {tuple(vs.shape)} of codes {tuple(shape)} must have a byte for 32 dims")
+    ksl, vsl = _layout(ks, d // 32), _layout(vs, d // 32)
+    if ksl is None or vsl is None:
+        raise ValueError(f"scales need a unit last stride and rows aligned to their {d // 32} bytes")
+    if not device == ks.device == v.device == vs.device:
+        raise ValueError("codes and scales of k and v must be tensors of one GPU")
+    return _lib.GW_CACHE_FP4, k, hk, d, (*kl, *ksl, *vl, *vsl)
 
 
 def _check_table(rows, block_table, *more):
-    if any(t.dtype != torch.int32 for t in (block_table, *more)):
-        raise TypeError("block_table, lengths and bounds must be int32")
-    if block_table.dim() != 2:
-        raise ValueError(f"block_table must be [sequences, W], got {tuple(block_table.shape)}")
+    """block_table with unit column stride, checked together with the lists of lengths and bounds."""
+    device = rows.device
+    if not rows.is_cuda:
+        raise ValueError("the caches, block_table, lengths and bounds must be tensors of one GPU")
+    for t in (block_table, *more):
+        if t.dtype != torch.int32:
+            raise TypeError("block_table, lengths and bounds must be int32")
+        if t.device != device:
+            raise ValueError("the caches, block_table, lengths and bounds must be tensors of one GPU")
     if block_table.shape[1] * rows.shape[1] > MAX_KEYS:
         raise ValueError(f"keys of a sequence must not exceed {MAX_KEYS}")
-    if not (rows.is_cuda and all(t.device == rows.device for t in (block_table, *more))):
-        raise ValueError("the caches, block_table, lengths and bounds must be tensors of one GPU")
     return block_table if block_table.stride(1) == 1 or block_table.shape[1] == 1 else block_table.contiguous()
 
 
-def _token_rows(x: torch.Tensor):
+def _token_rows(x: torch.Tensor, packed: bool):
     """(x with 16-byte aligned rows, its {sequence, token, head} strides)."""
-    if not _rows_fit(x, 16):
-        x = x.clone(memory_format=torch.contiguous_format)
-    st = _lib.row_strides(x)
-    return x, _lib.strides3(*st) if x.dim() == 4 else _lib.strides3(0, *st)
+    st = x.stride()
+    if st[-1] != 1 or any(s & 7 for s in st[:-1]) or x.data_ptr() & 15:
+        st = _lib.row_strides(x)  # dims of one entry have any strides
+        if x.stride(-1) != 1 or any(s & 7 for s in st) or x.data_ptr() & 15:
+            x = x.clone(memory_format=torch.contiguous_format)
+            st = x.stride()
+    if x.dim() == 4:
+        return x, _lib.strides3(st[0], st[1], st[2])
+    return x, _lib.strides3(0, st[0], st[1]) if packed else _lib.strides3(st[0], 0, st[1])
 
 
-def _check_axes(positions, axis_dims, bases, lead, d, device):
-    axis_dims = tuple(int(n) for n in axis_dims)
+@functools.lru_cache(maxsize=256)
+def _axes(axis_dims: Tuple[int, ...], bases: Union[float, Tuple[float, ...]], d: int):
+    """The C entry's axes, checked."""
     if not 1 <= len(axis_dims) <= MAX_AXES:
         raise ValueError(f"1 to {MAX_AXES} axes, got {len(axis_dims)}")
-    if any(n < 0 or n % 2 for n in axis_dims) or sum(axis_dims) > d:
+    if any(int(n) != n or n < 0 or n % 2 for n in axis_dims) or sum(axis_dims) > d:
         raise ValueError(f"axis dims {axis_dims} must be even and fit the head dim {d}")
     if isinstance(bases, (int, float)):
-        bases = [bases] * len(axis_dims)
+        bases = (bases,) * len(axis_dims)
     bases = tuple(float(b) for b in bases)
     if len(bases) != len(axis_dims) or any(not (b > 0 and math.isfinite(b)) for b in bases):
         raise ValueError(f"one positive finite base per axis is needed, got {bases}")
-    if positions.dtype not in _POS_CODES:
-        raise TypeError(f"positions must be int32, int64 or float32, not {positions.dtype}")
-    if tuple(positions.shape) != lead + (len(axis_dims),):
-        raise ValueError(f"positions {tuple(positions.shape)} must be {lead + (len(axis_dims),)}")
-    if positions.device != device:
-        raise ValueError("positions must lie on the caches' GPU")
-    return axis_dims, bases
+    return _axis_args(tuple(int(n) for n in axis_dims), bases)
 
 
 def paged_kv_append_func(k: torch.Tensor, v: torch.Tensor, k_cache: Cache, v_cache: Cache, block_table: torch.Tensor,
@@ -166,65 +180,69 @@ def paged_kv_append_func(k: torch.Tensor, v: torch.Tensor, k_cache: Cache, v_cac
     sequences share) leave unspecified contents there. The caches must not overlap q, k or v."""
     fmt, rows, hk, d, args = cache_args(k_cache, v_cache)
     packed = cu_seqlens is not None
-    dims = (3,) if packed else (3, 4)
-    if k.dim() not in dims or k.shape != v.shape or k.shape[-2:] != (hk, d):
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be "
+    shape, dtype, dev = k.shape, k.dtype, rows.device
+    nd = len(shape)
+    if nd != 3 and (packed or nd != 4) or v.shape != shape or shape[-2] != hk or shape[-1] != d:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must be "
                          f"{'[T, Hk, D]' if packed else '[B, Hk, D] or [B, N, Hk, D]'} of the caches' Hk = {hk}, D = {d}")
-    if k.dtype not in (torch.float16, torch.bfloat16):
+    if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError("Only support fp16 and bf16")
-    lead = tuple(k.shape[:-2])
-    if q is not None and (q.dim() != k.dim() or tuple(q.shape[:-2]) != lead or q.shape[-1] != d):
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads")
-    xs = [k, v] if q is None else [k, v, q]
-    if any(x.dtype != k.dtype for x in xs) or (fmt == _lib.GW_CACHE_16BIT and rows.dtype != k.dtype):
+    if v.dtype != dtype or (q is not None and q.dtype != dtype) or (fmt == _lib.GW_CACHE_16BIT and rows.dtype != dtype):
         raise TypeError("All tensors must have the same type")
+    if q is not None and (q.dim() != nd or q.shape[:-2] != shape[:-2] or q.shape[-1] != d):
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(shape)} differ in more than their heads")
     if (positions is None) != (axis_dims is None):
         raise ValueError("positions and axis_dims go together")
-    if cache_seqlens.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != cache_seqlens.shape[0]:
+    n = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else -1
+    if block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError(f"block_table {tuple(block_table.shape)} and cache_seqlens {tuple(cache_seqlens.shape)} must be "
                          "[sequences, W] and [sequences]")
-    n = cache_seqlens.shape[0]
-    if (cu_seqlens.shape if packed else k.shape[:1]) != ((n + 1,) if packed else (n,)):
-        raise ValueError(f"{tuple(cu_seqlens.shape) if packed else lead} does not go with cache_seqlens of {n} sequences")
-    lists = [cache_seqlens, cu_seqlens] if packed else [cache_seqlens]
-    block_table = _check_table(rows, block_table, *lists)
-    dev = rows.device
-    if any(x.device != dev for x in xs):
+    if packed:
+        if cu_seqlens.shape != (n + 1,):
+            raise ValueError(f"cu_seqlens {tuple(cu_seqlens.shape)} does not go with cache_seqlens of {n} sequences")
+        block_table = _check_table(rows, block_table, cache_seqlens, cu_seqlens)
+        tokens, count = shape[0], shape[0]
+        cu_seqlens = cu_seqlens.contiguous()
+    else:
+        if shape[0] != n:
+            raise ValueError(f"k {tuple(shape)} does not go with cache_seqlens of {n} sequences")
+        block_table = _check_table(rows, block_table, cache_seqlens)
+        count = 1 if nd == 3 else shape[1]
+        tokens = n * count
+    if k.device != dev or v.device != dev or (q is not None and q.device != dev):
         raise ValueError("q, k, v and the caches must be tensors of one GPU")
     hq = 0 if q is None else q.shape[-2]
-    tokens = k.numel() // (hk * d)
     if tokens * (hq + 2 * hk) > MAX_KEYS:
         raise ValueError(f"tokens x heads must not exceed {MAX_KEYS}")
     axes, pos = (0, None, None), (0, None, None)
     if positions is not None:
-        axis_dims, bases = _check_axes(positions, axis_dims, bases, lead, d, dev)
-        axes = _axis_args(axis_dims, bases)
+        axes = _axes(tuple(axis_dims), bases if isinstance(bases, (int, float)) else tuple(bases), d)
+        if positions.dtype not in _POS_CODES:
+            raise TypeError(f"positions must be int32, int64 or float32, not {positions.dtype}")
+        if positions.shape != (*shape[:-2], axes[0]):
+            raise ValueError(f"positions {tuple(positions.shape)} must be {(*shape[:-2], axes[0])}")
+        if positions.device != dev:
+            raise ValueError("positions must lie on the caches' GPU")
         st = positions.stride()
-        pos = (_POS_CODES[positions.dtype], positions.data_ptr(), _lib.strides3(*st) if len(st) == 3 else
-               _lib.strides3(0, *st) if packed else _lib.strides3(st[0], 0, st[1]))
+        pos = (_POS_CODES[positions.dtype], positions.data_ptr(),
+               _lib.strides3(*st) if nd == 4 else _lib.strides3(0, *st) if packed else _lib.strides3(st[0], 0, st[1]))
     turned = None if q is None else _lib.empty_rows(q)
     if tokens == 0:
         return turned
-    (k, k_strides), (v, v_strides) = (_one(x, packed) for x in (k, v))
-    q, q_strides = (None, None) if q is None else _one(q, packed)
+    k, k_strides = _token_rows(k, packed)
+    v, v_strides = _token_rows(v, packed)
+    q_args = (None, None, None, 0)
+    if q is not None:
+        q, q_strides = _token_rows(q, packed)
+        q_args = (q.data_ptr(), q_strides, turned.data_ptr(), hq)
     cache_seqlens = cache_seqlens.contiguous()
-    cu = cu_seqlens.contiguous() if packed else None
     with _lib.on_device(dev):
         rc = _lib.load().gw_paged_kv_append(
-            _lib.dtype_code(k.dtype), _lib.ptr(q), q_strides, _lib.ptr(turned), hq, k.data_ptr(), k_strides, v.data_ptr(),
-            v_strides, hk, d, fmt, *args, block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), _lib.ptr(cu),
-            n, tokens if packed else tokens // n, rows.shape[0], rows.shape[1], block_table.shape[1], *pos, *axes,
-            _lib.stream_handle(dev))
+            _lib.dtype_code(dtype), *q_args, k.data_ptr(), k_strides, v.data_ptr(), v_strides, hk, d, fmt, *args,
+            block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), _lib.ptr(cu_seqlens), n, count, rows.shape[0],
+            rows.shape[1], block_table.shape[1], *pos, *axes, _lib.stream_handle(dev))
     _lib.check(rc, "gw_paged_kv_append")
     return turned
-
-
-def _one(x: torch.Tensor, packed: bool):
-    """:func:`_token_rows` with a token dim of one for ``[B, H, D]``."""
-    x, st = _token_rows(x)
-    if x.dim() == 3 and not packed:
-        st = _lib.strides3(st[1], 0, st[2])
-    return x, st
 
 
 def paged_kv_read_func(k_cache: Cache, v_cache: Cache, block_table: torch.Tensor, cu_seqlens: torch.Tensor, tokens: int,
