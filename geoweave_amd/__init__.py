@@ -10,7 +10,8 @@ Drop-in operator modules (same names and signatures as the reference):
 Operators beside them:
 
 * ``geoweave_amd.custom_flash_attn.packed_flash_attn``: attention over packed sequences of different
-  lengths, with backward; ``.paged_flash_attn``: new tokens over a paged key-value cache;
+  lengths, with backward; ``.paged_flash_attn``: new tokens over a paged key-value cache, in 16 or 4 bits;
+  ``.paged_kv_cache``: such caches written, with the rotation on the way, and read back;
 * ``geoweave_amd.rotary``: rotary positions with several axes, with backward.
 
 All compute runs in ``libgeoweave_hip.so`` (hand-written HIP for gfx950, C ABI in

@@ -35,6 +35,8 @@ import torch.nn.functional as F
 
 from . import dsa_layer, source_downsample
 from .custom_flash_attn.packed_flash_attn import packed_flash_attn_func, packed_flash_attn_inference_func
+from .custom_flash_attn.paged_flash_attn import paged_flash_attn_inference_func
+from .custom_flash_attn.paged_kv_cache import FP4Cache, paged_kv_append_func, paged_kv_read_func
 from .rotary import rotary_axes_qk_func
 
 __all__ = ["parse_indexer_layers", "parse_reuse_topk_groups", "slice_expand_and_flatten", "Aggregator",
@@ -150,7 +152,8 @@ class DenseAttention(nn.Module):
 
     With ``cu_seqlens`` (int32 ``[n + 1]`` on the GPU) x is a packed batch ``[1, T, dim]`` of n sequences
     of different lengths and each attends within itself (``packed_flash_attn``). ``forward_train`` is the
-    differentiable form on a packed batch, with any number of rotary axes."""
+    differentiable form on a packed batch, with any number of rotary axes; ``forward_cached`` the form for streams, whose
+    earlier tokens' keys and values are kept in a paged cache of 16 or 4 bits."""
 
     def __init__(self, dim: int, num_heads: int, qk_norm: bool, rope_base: Optional[float]):
         super().__init__()
@@ -199,6 +202,45 @@ class DenseAttention(nn.Module):
         o = packed_flash_attn_func(q, k, v, cu_seqlens, causal=causal)
         return self.proj(o.view(T, C))
 
+    # New tokens from which on attention takes the kept keys as packed rows read back, over 16 and over 4 bits: a pass over
+    # pages reads all keys once per 16 rows (4 bits: 32). 16 heads of 64 over 20,000 keys, pages and packed: 16 bits 72 and 82 us
+    # for 128 tokens, 126 and 76 for 256, 646 and 198 for 1,374; 4 bits 40 and 74, 64 and 68, 276 and 190. Four sequences
+    # of 4,122 keys, 16 heads over 4 of 128: 104 and 52, 158 and 67, 799 and 211; 59 and 49, 94 and 63, 363 and 204.
+    PACKED_FROM = (128, 256)
+
+    @torch.no_grad()
+    def forward_cached(self, x, k_cache, v_cache, block_table, cache_seqlens, pos=None, axis_dims=None, bases=None,
+                       causal=False, lengths: Optional[Sequence[int]] = None):
+        """x ``[B, N, dim]``: N new tokens of each of B sequences -> ``[B, N, dim]``. Their keys and values are written into the
+        caches (tensors, or ``FP4Cache``) and they attend to all that the sequences hold then. block_table int32 ``[B, W]``,
+        cache_seqlens int32 ``[B]`` (the new tokens counted) as in ``paged_kv_append_func``; pos ``[B, N, A]``, axis_dims and
+        bases as in :meth:`forward_train`. causal False: a new view's tokens see each other too. ``lengths``: what
+        cache_seqlens holds, where the host knows it: many new tokens then attend to the kept keys read back as packed rows."""
+        B, N, C = x.shape
+        if lengths is not None and len(lengths) != B:
+            raise ValueError(f"{len(lengths)} lengths of {B} sequences")
+        q, k, v = self.qkv(x).view(B, N, 3, self.num_heads, self.head_dim).unbind(2)
+        # one rounding to the activations' type behind the norm
+        q, k = self.q_norm(q).to(x.dtype), self.k_norm(k).to(x.dtype)
+        turn = {}
+        if pos is not None and (self.rope_base is not None or bases is not None):
+            axes = pos.shape[-1]
+            turn = {"positions": pos, "bases": self.rope_base if bases is None else bases,
+                    "axis_dims": axis_dims if axis_dims is not None else [self.head_dim // axes // 2 * 2] * axes}
+        turned = paged_kv_append_func(k, v, k_cache, v_cache, block_table, cache_seqlens, q=q if turn else None, **turn)
+        q = turned if turn else q
+        if lengths is None or N < self.PACKED_FROM[isinstance(k_cache, FP4Cache)]:
+            o, _ = paged_flash_attn_inference_func(q, k_cache, v_cache, block_table, cache_seqlens, causal)
+            return self.proj(o.view(B, N, C))
+        bounds = [0]
+        for n in lengths:
+            bounds.append(bounds[-1] + int(n))
+        cu_k = torch.tensor(bounds, dtype=torch.int32, device=x.device)
+        cu_q = torch.arange(0, (B + 1) * N, N, dtype=torch.int32, device=x.device)
+        k, v = paged_kv_read_func(k_cache, v_cache, block_table, cu_k, bounds[-1], dtype=x.dtype)
+        o, _ = packed_flash_attn_inference_func(q.reshape(B * N, self.num_heads, self.head_dim), k, v, cu_q, cu_k, causal)
+        return self.proj(o.view(B, N, C))
+
 
 class Block(nn.Module):
     """``x + ls1(attn(norm1(x))) -> + ls2(mlp(norm2(x)))`` (reference ``layers/block.py:28-99``);
@@ -241,6 +283,16 @@ class Block(nn.Module):
         x = x + self.ls1(a)
         x = x + self.ls2(self.mlp(self.norm2(x)))
         return x, idx
+
+    @torch.no_grad()
+    def forward_cached(self, x, k_cache, v_cache, block_table, cache_seqlens, pos=None, axis_dims=None, bases=None,
+                       causal=False, lengths: Optional[Sequence[int]] = None):
+        """The block on new tokens of streams, see :meth:`DenseAttention.forward_cached`."""
+        if self.sparse:
+            raise NotImplementedError("the sparse global attention selects from a whole scene, not from a cache")
+        x = x + self.ls1(self.attn.forward_cached(self.norm1(x), k_cache, v_cache, block_table, cache_seqlens, pos, axis_dims,
+                                                  bases, causal, lengths))
+        return x + self.ls2(self.mlp(self.norm2(x)))
 
 
 class PatchEmbedViT(nn.Module):
