@@ -215,7 +215,8 @@ class DenseAttention(nn.Module):
         caches (tensors, or ``FP4Cache``) and they attend to all that the sequences hold then. block_table int32 ``[B, W]``,
         cache_seqlens int32 ``[B]`` (the new tokens counted) as in ``paged_kv_append_func``; pos ``[B, N, A]``, axis_dims and
         bases as in :meth:`forward_train`. causal False: a new view's tokens see each other too. ``lengths``: what
-        cache_seqlens holds, where the host knows it: many new tokens then attend to the kept keys read back as packed rows."""
+        cache_seqlens holds, where the host knows it: many new tokens then attend to the kept keys read back as packed rows
+        (bounds made from a host value: not in a captured graph)."""
         B, N, C = x.shape
         if lengths is not None and len(lengths) != B:
             raise ValueError(f"{len(lengths)} lengths of {B} sequences")

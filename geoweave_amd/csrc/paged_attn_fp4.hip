@@ -681,8 +681,10 @@ extern "C" int gw_paged_attn_fp4_fwd(int dtype, const void* q, const int64_t* q_
   };
   GW_CHECK_ARG(scales_ok(k_scales, k_scale_strides) && scales_ok(v_scales, v_scale_strides),
                "scales need rows aligned to their %lld bytes", (long long)per);
+  for (const int64_t* s : {k_scale_strides, v_scale_strides})
+    GW_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[2] >= 0, "negative strides of a cache");
   for (const int64_t* s : {k_strides, v_strides}) {
-    GW_CHECK_ARG(s[0] >= 0 && s[1] >= 0, "negative strides of a cache");
+    GW_CHECK_ARG(s[0] >= 0 && s[1] >= 0 && s[2] >= 0, "negative strides of a cache");
     // Offsets of rows are 32 bits of 16 bytes.
     const unsigned __int128 span = (unsigned __int128)s[0] * (uint64_t)(pages > 0 ? pages - 1 : 0) +
                                    (unsigned __int128)s[1] * (uint64_t)(page_size - 1);

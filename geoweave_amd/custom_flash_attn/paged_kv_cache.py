@@ -79,6 +79,8 @@ def cache_args(k_cache: Cache, v_cache: Cache):
     if fp4 != isinstance(v_cache, FP4Cache):
         raise TypeError("k_cache and v_cache must both be 16-bit tensors or both FP4Cache")
     k, v = (k_cache[0], v_cache[0]) if fp4 else (k_cache, v_cache)
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise TypeError("a cache is a tensor or an FP4Cache")
     shape = k.shape
     if len(shape) != 4 or v.shape != shape:
         raise ValueError(f"caches must be [pages, page_size, Hk, D], got {tuple(shape)} and {tuple(v.shape)}")
@@ -177,7 +179,7 @@ def paged_kv_append_func(k: torch.Tensor, v: torch.Tensor, k_cache: Cache, v_cac
 
     A token whose key has no slot (below 0, behind the table, in a page outside the pool) and a token of no
     sequence is written nowhere; its q is turned all the same. Two new tokens that come to one slot (pages that
-    sequences share) leave unspecified contents there. The caches must not overlap q, k or v."""
+    sequences share) leave unspecified contents there. The caches must not overlap each other, q, k or v."""
     fmt, rows, hk, d, args = cache_args(k_cache, v_cache)
     packed = cu_seqlens is not None
     shape, dtype, dev = k.shape, k.dtype, rows.device

@@ -737,7 +737,7 @@ int gw_paged_attn_fwd(int dtype, const void* q, const int64_t* q_strides, const 
  * the table, or in a page outside [0, pages) is not written, nor is a token of no sequence; every token's q is
  * turned. Two new tokens for one slot leave unspecified contents there. pos, axis_dims and bases as in
  * gw_rotary_axes (n_axes = 0: nothing is turned); dims behind the axes are not turned. 4 bits: 32 dims with an inf or NaN are kept as not a number.
- * Rows must not overlap the inputs.
+ * The caches' rows must not overlap each other's or the inputs.
  *
  * Read: sequence b's keys 0 .. cu[b + 1] - cu[b] - 1 to rows cu[b] .. of k_out and v_out [tokens, Hk, D],
  * contiguous, in dtype (16 bits: the cache's own). Rows whose key has no slot, and rows of no sequence, are zeros.

@@ -104,6 +104,24 @@ def test_many_new_tokens(gpu_device, dtype, d, hq, hk, new, lens):
     check(o, lse, reference(args), args)
 
 
+@pytest.mark.parametrize("d,hq,hk,new", [(64, 16, 16, 1), (128, 24, 12, 2), (64, 32, 16, 40), (128, 16, 8, 17)])
+def test_units_of_many_blocks(gpu_device, d, hq, hk, new):
+    """Units of more than four blocks that end one row tile, take others whole and begin another."""
+    lens = [3000, 65, 64, 1, 0, 2500, 700, 128, 4100, 17, 17, 333]
+    args = make(lens, new, hq, hk, d, 16, BF, 50)
+    o, lse = run(args, gpu_device)
+    check(o, lse, reference(args), args)
+
+
+def test_more_key_heads_than_units(gpu_device):
+    """1,100 key heads: one unit takes all row tiles of a head."""
+    args = make([70, 0, 300, 64, 5], 3, 1100, 1100, 64, 16, HF, 51)
+    o, lse = run(args, gpu_device)
+    pick = [0, 1, 550, 1099]
+    some = (args[0][:, :, pick], *(tuple(t[:, :, pick] for t in c) for c in args[1:3]), *args[3:])
+    check(o[:, :, pick], lse[:, :, pick], reference(some), some)
+
+
 def test_many_sequences_without_a_split(gpu_device):
     lens = torch.randint(0, 90, (4200,), generator=torch.Generator().manual_seed(1)).tolist()
     args = make(lens, 1, 2, 1, 64, 32, BF)
@@ -152,18 +170,19 @@ def test_scales(gpu_device, scale):
     check(o, lse, reference(args, scale=scale), args)
 
 
-def test_unused_slots_and_pages_outside_the_pool(gpu_device):
+@pytest.mark.parametrize("page,d", [(24, 64), (32, 64), (32, 128)])
+def test_unused_slots_and_pages_outside_the_pool(gpu_device, page, d):
     """Scales that are not numbers wherever no key lies, page numbers outside the pool in the middle and at the end."""
-    args = make([300, 77, 500, 40], 4, 4, 2, 64, 24, BF, 3)
+    args = make([300, 77, 500, 40], 4, 4, 2, d, page, BF, 3)
     q, k, v, table, lens = args
     used = torch.zeros(k[0].shape[:2], dtype=torch.bool)
-    gone = [(0, 2), (0, 12), (2, 0), (2, 5), (3, 0), (3, 1)]
+    gone = [(0, 2), (0, 299 // page), (2, 0), (2, 5), (3, 0), (3, 1)]
     for (b, p), bad in zip(gone, (-1, 10 ** 6, k[0].shape[0], -2 ** 31, -5, 2 ** 31 - 1)):
         table[b, p] = bad
     for b, n in enumerate(lens.tolist()):
         for j in range(n):
-            if 0 <= table[b, j // 24] < k[0].shape[0]:
-                used[table[b, j // 24], j % 24] = True
+            if 0 <= table[b, j // page] < k[0].shape[0]:
+                used[table[b, j // page], j % page] = True
     assert not used.all()
     k[1][~used], v[1][~used] = 255, 255
     o, lse = run(args, gpu_device)

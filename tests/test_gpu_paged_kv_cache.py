@@ -165,6 +165,28 @@ def test_packed_bounds(gpu_device, fp4, cu, tokens):
     check_append(gpu_device, fp4, BF, 2, 2, 128, 24, [50, 20, 7, 64], (64, 64), None, cu=cu, tokens=tokens)
 
 
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("d,hq,hk", [(64, 1, 2), (128, 2, 1)])
+def test_many_tokens(gpu_device, fp4, d, hq, hk):
+    """Eight tokens to a workgroup, the last of them with fewer, sequences that end inside one."""
+    check_append(gpu_device, fp4, BF, hq, hk, d, 40, [5000, 3300, 90], (d,), None, cu=[0, 5000, 8197, 8261], tokens=8263)
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_heads(gpu_device, fp4, d):
+    """More heads than a workgroup takes of one token."""
+    check_append(gpu_device, fp4, HF, 300, 70, d, 8, [9, 20], (16, 24), None, count=3)
+    dev, g = gpu_device, torch.Generator().manual_seed(17)
+    table, pool = tables([9, 20], 8, g)
+    old, new = caches(fp4, pool, 8, 170, d, HF, g, dev)
+    k, v = paged_kv_read_func(*new, table.to(dev), torch.tensor([0, 9, 29], dtype=torch.int32, device=dev), 29, dtype=HF)
+    for was, got in zip(old, (k, v)):
+        rows = fp4_decode(*was).float().to(HF) if fp4 else was[0]
+        want = torch.stack([rows[s] for s in read_slots([0, 9, 29], table, 8, pool, 29)])
+        assert torch.equal(got.cpu(), want)
+
+
 @pytest.mark.parametrize("n", [1, 63, 64, 65, 200, 4200])
 def test_packed_many_sequences(gpu_device, n):
     g = torch.Generator().manual_seed(n)
@@ -307,7 +329,7 @@ def test_one_token_form_layouts_and_copies(gpu_device, fp4):
 @pytest.mark.parametrize("fp4", [False, True])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("d,hk", [(64, 1), (64, 5), (128, 2)])
-@pytest.mark.parametrize("cu,more", [([0, 1], 0), ([0, 100, 100, 133, 140], 5), ([3, 50, 51], 0)])
+@pytest.mark.parametrize("cu,more", [([0, 1], 0), ([0, 100, 100, 133, 140], 5), ([3, 50, 51], 0), ([0, 6000, 8205], 2)])
 def test_read(gpu_device, fp4, dtype, d, hk, cu, more):
     dev, g = gpu_device, torch.Generator().manual_seed(11)
     lens = [b - a for a, b in zip(cu[:-1], cu[1:])]

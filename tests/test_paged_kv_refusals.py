@@ -48,6 +48,7 @@ APPEND = [
     (dict(q=torch.zeros(2, 1, 2, 128, dtype=BF)), ValueError, "differ"),
     (dict(k_cache=cache4()), TypeError, "both"),
     (dict(v_cache=cache4()), TypeError, "both"),
+    (dict(k_cache=tuple(cache4()), v_cache=tuple(cache4())), TypeError, "a cache is"),
     (dict(v_cache=cache16(page=8)), ValueError, "caches must be"),
     (dict(k_cache=cache16()[0], v_cache=cache16()[0]), ValueError, "caches must be"),
     (dict(v_cache=cache16(dtype=HF)), TypeError, "same type"),
@@ -277,7 +278,7 @@ def attend(**over):
     (dict(ksc=None), 1, "cache"), (dict(kscs=None), 1, "missing"), (dict(table=None), 1, "table"), (dict(k=258), 1, "aligned"),
     (dict(ks=_lib.strides3(1024, 24, 64)), 1, "aligned"), (dict(qs=_lib.strides3(1024, 1024, 60)), 1, "aligned"),
     (dict(vsc=257), 1, "scales need"), (dict(vscs=_lib.strides3(64, 3, 2)), 1, "scales need"), (dict(pages=-1), 1, "negative"),
-    (dict(ks=_lib.strides3(-1024, 16, 64)), 1, "negative"), (dict(width=1 << 28), 2, "2^31"), (dict(b=1 << 30), 2, "2^31"),
+    (dict(ks=_lib.strides3(-1024, 16, 64)), 1, "negative"), (dict(vscs=_lib.strides3(64, 4, -2)), 1, "negative"), (dict(width=1 << 28), 2, "2^31"), (dict(b=1 << 30), 2, "2^31"),
     (dict(ks=_lib.strides3(1 << 36, 16, 64)), 2, "2^36"), (dict(), 1, "workspace"), (dict(ws=264, nbytes=1 << 30), 1, "workspace"),
     (dict(ws=256, nbytes=100), 1, "workspace"), (dict(b=1 << 23, ws=256, nbytes=1 << 60), 2, "2^32 threads"),
 ])
