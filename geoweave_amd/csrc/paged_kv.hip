@@ -13,6 +13,14 @@
 // its dims come from the wave's own copy of its rows in LDS, W at a time (W: the widest of 8, 4, 2, 1 that divides every half
 // block). 4 bits: the 32 values of a power of two lie in four neighbouring lanes, which exchange their largest
 // within the vector unit.
+//
+// Measured (kernels alone): 19,000 tokens of 24 scenes, q, k and v of 16 heads of 64, into 16 bits 30 us, 5.2 TB/s, what a
+// large copy reaches; 28,980 tokens, 16 + 4 + 4 heads of 128, four axes of odd halves (W = 1) 80 to 83 us, 4.4 TB/s; 50,160
+// tokens, 16 heads of 64, into 4 bits 74 to 80 us, 3.4 TB/s, the vector unit 75 % busy. The rows of all heads one
+// behind the other (token by token), with selects that the compiler made loads of: 159 us. Reading back: 41 us from 4 bits (5.8 TB/s, part
+// of it from the last-level cache), 88,036 tokens of 4 heads of 128 from 16 bits 61 to 65 us.
+// Moving addresses instead of one product per row: 128.5 for 131 us of the 4-bit pass with its reading, but 5.2 for 4.8 us of
+// 64 single tokens.
 #include <math.h>
 #include <string.h>
 
