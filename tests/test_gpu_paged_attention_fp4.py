@@ -139,7 +139,8 @@ def test_more_sequences_than_one_scan_round(gpu_device):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("gain,unit,spread", [(1e-3, 126, 2), (30.0, 122, 2), (1.5, 126, 12), (1e-30, 180, 3), (1e4, 113, 3)])
+@pytest.mark.parametrize("gain,unit,spread", [(1e-3, 126, 2), (30.0, 122, 2), (1.5, 126, 12), (1e-30, 180, 3), (1e4, 113, 3),
+                                              (2.0 ** -20, 137, 2)])
 def test_ranges(gpu_device, dtype, d, gain, unit, spread):
     """Small and large queries, kept rows whose powers of two differ widely."""
     if dtype == HF and gain == 1e-30:
@@ -313,6 +314,37 @@ def test_a_row_alone(gpu_device):
     loud[:, 1:] *= 40
     o2, lse2 = paged_flash_attn_inference_func(loud.to(dev), k, v, table, lens.to(dev), return_lse=True)
     assert torch.equal(o[:, 0], o2[:, 0]) and torch.equal(lse[:, 0], lse2[:, 0])
+
+
+def test_two_streams_and_two_graphs(gpu_device):
+    """Calls under way at once, and captured ones replayed in turn, have workspaces of their own."""
+    dev = gpu_device
+    calls = []
+    for seed, (lens, hq, hk, d) in enumerate([([9000, 4000, 31], 8, 2, 64), ([12000, 500], 4, 4, 128)]):
+        q, k, v, table, n = make(lens, 2, hq, hk, d, 16, BF, 60 + seed)
+        args = (q.to(dev), on_gpu(k, dev), on_gpu(v, dev), table.to(dev), n.to(dev))
+        calls.append(lambda args=args: paged_flash_attn_inference_func(*args)[0])
+    want = [call() for call in calls]
+    torch.cuda.synchronize(dev)
+    streams, got = [torch.cuda.Stream(dev) for _ in calls], [[], []]
+    for _ in range(5):
+        for i, (s, call) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(s):
+                got[i].append(call())
+    torch.cuda.synchronize(dev)
+    for outs, ref in zip(got, want):
+        assert all(torch.equal(o, ref) for o in outs)
+    graphs = []
+    for call in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    for _ in range(3):
+        for (graph, out), call, ref in zip(graphs, calls, want):
+            graph.replay()
+            torch.cuda.synchronize(dev)
+            assert torch.equal(out, ref) and torch.equal(call(), ref)
 
 
 @pytest.mark.parametrize("dtype,d,hq,hk", [(BF, 64, 4, 4), (HF, 128, 8, 2)])
