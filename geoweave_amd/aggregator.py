@@ -215,11 +215,17 @@ class DenseAttention(nn.Module):
         caches (tensors, or ``FP4Cache``) and they attend to all that the sequences hold then. block_table int32 ``[B, W]``,
         cache_seqlens int32 ``[B]`` (the new tokens counted) as in ``paged_kv_append_func``; pos ``[B, N, A]``, axis_dims and
         bases as in :meth:`forward_train`. causal False: a new view's tokens see each other too. ``lengths``: what
-        cache_seqlens holds, where the host knows it: many new tokens then attend to the kept keys read back as packed rows
+        cache_seqlens holds, where the host knows it and every key below has a slot (read back, a key of a page outside the pool
+        is a row of zeros that is seen): many new tokens then attend to the kept keys read back as packed rows
         (bounds made from a host value: not in a captured graph)."""
         B, N, C = x.shape
-        if lengths is not None and len(lengths) != B:
-            raise ValueError(f"{len(lengths)} lengths of {B} sequences")
+        if lengths is not None:
+            lengths = [int(n) for n in lengths]
+            if len(lengths) != B:
+                raise ValueError(f"{len(lengths)} lengths of {B} sequences")
+            slots = block_table.shape[1] * (k_cache.codes if isinstance(k_cache, FP4Cache) else k_cache).shape[1]
+            if any(not 0 <= n <= slots for n in lengths):
+                raise ValueError(f"lengths {lengths} must lie between 0 and the table's {slots} slots")
         q, k, v = self.qkv(x).view(B, N, 3, self.num_heads, self.head_dim).unbind(2)
         # one rounding to the activations' type behind the norm
         q, k = self.q_norm(q).to(x.dtype), self.k_norm(k).to(x.dtype)
@@ -235,7 +241,7 @@ class DenseAttention(nn.Module):
             return self.proj(o.view(B, N, C))
         bounds = [0]
         for n in lengths:
-            bounds.append(bounds[-1] + int(n))
+            bounds.append(bounds[-1] + n)
         cu_k = torch.tensor(bounds, dtype=torch.int32, device=x.device)
         cu_q = torch.arange(0, (B + 1) * N, N, dtype=torch.int32, device=x.device)
         k, v = paged_kv_read_func(k_cache, v_cache, block_table, cu_k, bounds[-1], dtype=x.dtype)

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from geoweave_amd import _lib
+from geoweave_amd import aggregator as agg
 from geoweave_amd.custom_flash_attn.paged_flash_attn import paged_flash_attn_inference_func
 from geoweave_amd.custom_flash_attn.paged_kv_cache import (FP4Cache, fp4_paged_cache, paged_kv_append_func,
                                                            paged_kv_read_func)
@@ -294,3 +295,13 @@ def test_workspaces_are_bounded_by_the_sizes():
         assert 0 < size(b, n, hq, hk, d) <= 1 << 26, (b, n, hq, hk, d)
     assert size(8192, 1, 32, 8, 128) == 0  # no split
     assert size(0, 1, 1, 1, 64) == 0 and size(1, 1 << 40, 1, 1, 64) == 0
+
+
+@pytest.mark.parametrize("lengths", [[20], [20, 20, 20], [20, -1], [33, 20]])
+@pytest.mark.parametrize("fp4", [False, True])
+def test_lengths_of_a_layer(fp4, lengths):
+    """What the host says of the lengths is checked against the table's slots before anything is written."""
+    m = agg.DenseAttention(128, 2, False, None).to(BF)
+    c = cache4() if fp4 else cache16()
+    with pytest.raises(ValueError, match="slots$|lengths of 2 sequences"):
+        m.forward_cached(torch.zeros(2, 1, 128, dtype=BF), c, c, torch.zeros(2, 2, dtype=torch.int32), INT2, lengths=lengths)
