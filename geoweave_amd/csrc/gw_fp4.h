@@ -15,6 +15,16 @@ namespace gw {
 namespace {
 
 constexpr uint32_t kFp4NaN = 255u;
+constexpr uint32_t kFp4Beyond = 253u;  // the least scale of values that 16 bits have no finite number for: 4 * 2^126 is 2^128
+
+// Of the eight codes of a word: all bits of those whose values, under a scale from kFp4Beyond on, are no finite number: magnitudes from
+// 4 on under 2^126, from 2 on under 2^127, all under NaN.
+__device__ __forceinline__ uint32_t fp4_beyond(uint32_t w, uint32_t scale) {
+  if (scale < kFp4Beyond) return 0u;
+  uint32_t hit = 0x11111111u;
+  if (scale != kFp4NaN) hit &= scale == kFp4Beyond ? (w >> 1) & (w >> 2) : w >> 2;
+  return hit * 15u;
+}
 
 // Byte of the power of two for 32 values, from the bits of the largest magnitude (inf and NaN have the largest bits).
 __device__ __forceinline__ uint32_t fp4_scale(uint32_t top) {

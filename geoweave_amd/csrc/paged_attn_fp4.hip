@@ -32,8 +32,9 @@
 // vector unit and the matrix cores alike: 72 us for 31 GFLOP; four row tiles to a wave (one wave per SIMD) took 87 for 82.
 //
 // Rows that are not keys (behind the length, in a page outside the pool) are masked, and their scales count as 2^-127:
-// what lies there cannot reach a result. Codes are always finite; a scale of 255 makes 32 values NaN: such values of V
-// count as 0 in the products and are added afterwards to the rows that see them.
+// what lies there cannot reach a result. A masked weight is 0, but 0 * inf is NaN, so values of V that are no finite number (gw_fp4.h:
+// NaN under a scale of 255, inf from 2^128 on, under 253 and 254) count as 0 in the products and are added afterwards to the
+// rows that see them.
 #include <math.h>
 #include <string.h>
 
@@ -390,10 +391,16 @@ __global__ __launch_bounds__(256, fp4_resident(D, RT)) void fp4_attn_kernel(cons
             top = max(top, __float_as_uint(unit[j]));
           }
         }
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(top == 0x7f800000u) != 0ull, 0)) {  // 255: seen to afterwards
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(top >= kFp4Beyond << 23) != 0ull, 0)) {  // seen to afterwards
           unclean = true;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) unit[j] = __float_as_uint(unit[j]) == 0x7f800000u ? 0.f : unit[j];
+          for (int j = 0; j < 8; ++j) {
+            uint32_t& x = b.v[D == 128 ? 8 * h + j : j];  // D = 64: this half's values are in its low or high 16 bits
+            const uint32_t half = D == 128 ? 0xFFFFFFFFu : h == 0 ? 0xFFFFu : 0xFFFF0000u;
+            const uint32_t scale = __float_as_uint(unit[j]) >> 23;
+            x &= ~(fp4_beyond(x, scale) & half);
+            if (scale == kFp4NaN) unit[j] = 0.f;
+          }
         }
         uint32_t hi[RT][4], lo[RT][4];
 #pragma unroll
@@ -499,22 +506,28 @@ __global__ __launch_bounds__(256, fp4_resident(D, RT)) void fp4_attn_kernel(cons
     // Dim of entry u of accumulator row r = 4 g + rr (its operand row, i16 above).
     auto dim_of = [](int r, int u) { return D == 128 ? 8 * r + u : 8 * (r & 7) + 4 * (r >> 3) + u; };
     if (__builtin_expect(unclean, 0)) {
-      // This wave's values that are not numbers go to the rows that see them.
+      // This wave's values that are no finite numbers go to the rows that see them.
       for (int j0 = j_first; j0 < ke; j0 += 256) {
         for (int i = 0; i < min(64, ke - j0); ++i) {
           const int pg = (j0 + i) / p.page, id = trow[pg];
           if ((uint32_t)id >= (uint32_t)p.pages) continue;
-          const uint8_t* src = vscales + id * p.vssp + (int64_t)(j0 + i - pg * p.page) * p.vsst;
-          for (int x = 0; x < D / 32; ++x) {
-            if (src[x] != kFp4NaN) continue;
+          const int at = j0 + i - pg * p.page;
+          // The lane's dims are of one power.
+          const uint32_t scale = (vscales + id * p.vssp + at * p.vsst)[D == 128 ? g : g & 1];
+          if (scale < kFp4Beyond) continue;
+          const uint8_t* codes = vcodes + ((uint64_t)((uint32_t)id * p.vup + (uint32_t)at * p.vut) << 4);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              if (j0 + i > lim[rt]) continue;
+          for (int rr = 0; rr < 4; ++rr) {
+            const uint8_t* word = codes + dim_of(4 * g + rr, 0) / 2;
+            const uint32_t w = D == 128 ? *reinterpret_cast<const uint32_t*>(word) : *reinterpret_cast<const uint16_t*>(word);
+            const uint32_t hit = fp4_beyond(w, scale);
 #pragma unroll
-              for (int u = 0; u < DV; ++u)
+            for (int u = 0; u < DV; ++u) {
+              if (!((hit >> (4 * u)) & 1u)) continue;
+              const float f = scale == kFp4NaN ? __uint_as_float(0x7fc00000u) : (w >> (4 * u)) & 8u ? -INFINITY : INFINITY;
 #pragma unroll
-                for (int rr = 0; rr < 4; ++rr)
-                  if (dim_of(4 * g + rr, u) >> 5 == x) acc[rt][u][rr] = __uint_as_float(0x7fc00000u);
+              for (int rt = 0; rt < RT; ++rt)
+                if (j0 + i <= lim[rt]) acc[rt][u][rr] += f;
             }
           }
         }
