@@ -6,8 +6,8 @@
 // Codes become 16-bit values by the conversion instruction, two of a row at a time with their power of two: exact, so that
 // the products are those of the values themselves.
 //   S^T = K Q^T (16x16x32): lane (g, i) reads the D / 4 dims from D / 4 g on of key i, which are its operands of the
-// D / 32 products one after the other, and holds q of row i in the same order. In fp16, where a unit is outside the normal
-// numbers (2^-13 to 2^13), K is bf16 and q two bf16 terms, exact.
+// D / 32 products one after the other, and holds q of row i in the same order. In fp16, the scores of a key with a unit
+// outside the normal numbers (2^-13 to 2^13) are those of K in bf16 and q in two bf16 terms, exact.
 // The block-scaled product (16x16x128, fp4 x fp8, q in e4m3 terms) would take K without a conversion, but sums
 // 2^-17 of the magnitudes off (measured; 3e-4 in a score of 13 whose magnitudes are 32), and is not faster here.
 //   O^T += V^T P^T (16x16x32): the scores of a lane stand for eight keys; exchanging halves between those keys'
@@ -347,31 +347,41 @@ __global__ __launch_bounds__(256, fp4_resident(D, RT)) void fp4_attn_kernel(cons
         const uint32_t ok = (uint32_t)(b.ok >> (32 * h));
         f32x4 sc[RT][2];
         const float ku[2] = {k_unit(b, h, 0), k_unit(b, h, 1)};
-        const bool split =
-            __is_same(E, FP16) && __builtin_amdgcn_ballot_w64(!fp4_fits_fp16(ku[0]) || !fp4_fits_fp16(ku[1])) != 0ull;
+        // Keys whose dims all lie in fp16's range take the products in fp16, whatever the other keys of the wave are: a
+        // row's scores keep their bits when a key that it does not see, or an unused slot, changes.
+        uint64_t fits[2] = {~0ull, ~0ull};
+        if constexpr (__is_same(E, FP16)) {
+          fits[0] = __builtin_amdgcn_ballot_w64(fp4_fits_fp16(ku[0]));
+          fits[1] = __builtin_amdgcn_ballot_w64(fp4_fits_fp16(ku[1]));
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) sc[rt][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-          if (__builtin_expect(!split, 1)) {
 #pragma unroll
-            for (int s = 0; s < D / 32; ++s) {
-              const uint4 x = fp4_operand<E>(reinterpret_cast<const uint32_t*>(&b.k[2 * h + t])[s], ku[t]);
+          for (int s = 0; s < D / 32; ++s) {
+            const uint4 x = fp4_operand<E>(reinterpret_cast<const uint32_t*>(&b.k[2 * h + t])[s], ku[t]);
 #pragma unroll
-              for (int rt = 0; rt < RT; ++rt) sc[rt][t] = mma16(E{}, x, q[rt][s], sc[rt][t]);
-            }
-          } else {
+            for (int rt = 0; rt < RT; ++rt) sc[rt][t] = mma16(E{}, x, q[rt][s], sc[rt][t]);
+          }
+          if (__builtin_expect(fits[t] != ~0ull, 0)) {
+            // Bit u: key 16 t + 4 g + u is of that kind (lanes i, i + 16, i + 32 and i + 48 hold parts of key i).
+            uint32_t mine = (uint32_t)fits[t] & (uint32_t)(fits[t] >> 32);
+            mine = (mine & mine >> 16) >> (4 * g);
 #pragma unroll
-            for (int s = 0; s < D / 32; ++s) {
-              const uint4 x = fp4_operand<BF16>(reinterpret_cast<const uint32_t*>(&b.k[2 * h + t])[s], ku[t]);
+            for (int rt = 0; rt < RT; ++rt) {
+              f32x4 wide = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int rt = 0; rt < RT; ++rt) {
+              for (int s = 0; s < D / 32; ++s) {
+                const uint4 x = fp4_operand<BF16>(reinterpret_cast<const uint32_t*>(&b.k[2 * h + t])[s], ku[t]);
                 uint4 high, low, x16 = q[rt][s];
                 asm volatile("" : "+v"(x16.x), "+v"(x16.y), "+v"(x16.z), "+v"(x16.w));  // here, not ahead of the loop
                 fp4_split_query(x16, high, low);
-                sc[rt][t] = mma16(BF16{}, x, high, sc[rt][t]);
-                sc[rt][t] = mma16(BF16{}, x, low, sc[rt][t]);
+                wide = mma16(BF16{}, x, high, wide);
+                wide = mma16(BF16{}, x, low, wide);
               }
+#pragma unroll
+              for (int u = 0; u < 4; ++u) sc[rt][t][u] = (mine >> u) & 1u ? sc[rt][t][u] : wide[u];
             }
           }
         }
