@@ -27,6 +27,7 @@ glue kernel as the sparse layers.
 """
 from __future__ import annotations
 
+import itertools
 from typing import Dict, List, Optional, Sequence, Set, Tuple
 
 import torch
@@ -202,11 +203,28 @@ class DenseAttention(nn.Module):
         o = packed_flash_attn_func(q, k, v, cu_seqlens, causal=causal)
         return self.proj(o.view(T, C))
 
-    # New tokens from which on attention takes the kept keys as packed rows read back, over 16 and over 4 bits: a pass over
-    # pages reads all keys once per 16 rows (4 bits: 32). 16 heads of 64 over 20,000 keys, pages and packed: 16 bits 72 and 82 us
-    # for 128 tokens, 126 and 76 for 256, 646 and 198 for 1,374; 4 bits 40 and 74, 64 and 68, 276 and 190. Four sequences
-    # of 4,122 keys, 16 heads over 4 of 128: 104 and 52, 158 and 67, 799 and 211; 59 and 49, 94 and 63, 363 and 204.
-    PACKED_FROM = (128, 256)
+    # (n, work) over a cache of 16 and of 4 bits: attention takes the kept keys as packed rows read back where (new tokens - n) x keys
+    # of all sequences x dim is above `work`. A pass over pages reads all keys once per 16 rows (4 bits: 32); reading back costs
+    # as much as n new tokens of that, and some 55 us of host time. Pages and read back, us, 16 heads of 64, 16 bits: 71 and 106 for 128
+    # new tokens over 20,000 keys, 126 and 100 for 256, 649 and 223 for 1,374; over 5,496 keys 52 and 66 for 256, 191 and 96 for 1,374;
+    # 1,096 and 894 for 128 of each of 16 sequences of 20,000. 4 bits: 67 and 94, 277 and 217 for 256 and 1,374; 108 and 97; 404 and 713.
+    # Over 112 shapes (16 and 4 heads of 64, 1 to 16 sequences of 1,374 to 100,000 keys, 64 to 1,374 new tokens) the rule takes 1.3 %
+    # (4 bits: 0.7 %) more time than the better of the two; the number of new tokens alone, from 128 and 256 on, took 29 % (18 %).
+    READ_BACK_FROM = ((80, 2.5e9), (300, 4e9))
+
+    def _reads_back(self, new: int, lengths: Sequence[int], k_cache) -> bool:
+        fp4 = isinstance(k_cache, FP4Cache)
+        least, work = self.READ_BACK_FROM[fp4]
+        return (new - least) * sum(lengths) * self.num_heads * self.head_dim > work
+
+    def _attend_read_back(self, q, k_cache, v_cache, block_table, causal, lengths):
+        """q ``[B, N, H, D]`` over the kept keys read back as packed rows."""
+        B, N, H, D = q.shape
+        bounds = [0, *itertools.accumulate(lengths)]
+        cu_k = torch.tensor(bounds, dtype=torch.int32, device=q.device)
+        cu_q = torch.arange(0, (B + 1) * N, N, dtype=torch.int32, device=q.device)
+        k, v = paged_kv_read_func(k_cache, v_cache, block_table, cu_k, bounds[-1], dtype=q.dtype)
+        return packed_flash_attn_inference_func(q.reshape(B * N, H, D), k, v, cu_q, cu_k, causal)[0]
 
     @torch.no_grad()
     def forward_cached(self, x, k_cache, v_cache, block_table, cache_seqlens, pos=None, axis_dims=None, bases=None,
@@ -216,8 +234,8 @@ class DenseAttention(nn.Module):
         cache_seqlens int32 ``[B]`` (the new tokens counted) as in ``paged_kv_append_func``; pos ``[B, N, A]``, axis_dims and
         bases as in :meth:`forward_train`. causal False: a new view's tokens see each other too. ``lengths``: what
         cache_seqlens holds, where the host knows it and every key below has a slot (read back, a key of a page outside the pool
-        is a row of zeros that is seen): many new tokens then attend to the kept keys read back as packed rows
-        (bounds made from a host value: not in a captured graph)."""
+        is a row of zeros that is seen): much work then takes the kept keys as packed rows read back (``READ_BACK_FROM``; bounds
+        made from a host value: not in a captured graph)."""
         B, N, C = x.shape
         if lengths is not None:
             lengths = [int(n) for n in lengths]
@@ -236,16 +254,10 @@ class DenseAttention(nn.Module):
                     "axis_dims": axis_dims if axis_dims is not None else [self.head_dim // axes // 2 * 2] * axes}
         turned = paged_kv_append_func(k, v, k_cache, v_cache, block_table, cache_seqlens, q=q if turn else None, **turn)
         q = turned if turn else q
-        if lengths is None or N < self.PACKED_FROM[isinstance(k_cache, FP4Cache)]:
+        if lengths is not None and self._reads_back(N, lengths, k_cache):
+            o = self._attend_read_back(q, k_cache, v_cache, block_table, causal, lengths)
+        else:
             o, _ = paged_flash_attn_inference_func(q, k_cache, v_cache, block_table, cache_seqlens, causal)
-            return self.proj(o.view(B, N, C))
-        bounds = [0]
-        for n in lengths:
-            bounds.append(bounds[-1] + n)
-        cu_k = torch.tensor(bounds, dtype=torch.int32, device=x.device)
-        cu_q = torch.arange(0, (B + 1) * N, N, dtype=torch.int32, device=x.device)
-        k, v = paged_kv_read_func(k_cache, v_cache, block_table, cu_k, bounds[-1], dtype=x.dtype)
-        o, _ = packed_flash_attn_inference_func(q.reshape(B * N, self.num_heads, self.head_dim), k, v, cu_q, cu_k, causal)
         return self.proj(o.view(B, N, C))
 
 
