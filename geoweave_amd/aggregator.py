@@ -212,8 +212,10 @@ class DenseAttention(nn.Module):
     # (4 bits: 0.7 %) more time than the better of the two; the number of new tokens alone, from 128 and 256 on, took 29 % (18 %).
     READ_BACK_FROM = ((80, 2.5e9), (300, 4e9))
 
-    def _reads_back(self, new: int, lengths: Sequence[int], k_cache) -> bool:
+    def _reads_back(self, new: int, lengths: Sequence[int], k_cache, dtype) -> bool:
         fp4 = isinstance(k_cache, FP4Cache)
+        if fp4 and dtype != torch.bfloat16:
+            return False  # 4 bits hold values that fp16 does not (65,504 is kept as 65,536)
         least, work = self.READ_BACK_FROM[fp4]
         return (new - least) * sum(lengths) * self.num_heads * self.head_dim > work
 
@@ -254,7 +256,7 @@ class DenseAttention(nn.Module):
                     "axis_dims": axis_dims if axis_dims is not None else [self.head_dim // axes // 2 * 2] * axes}
         turned = paged_kv_append_func(k, v, k_cache, v_cache, block_table, cache_seqlens, q=q if turn else None, **turn)
         q = turned if turn else q
-        if lengths is not None and self._reads_back(N, lengths, k_cache):
+        if lengths is not None and self._reads_back(N, lengths, k_cache, x.dtype):
             o = self._attend_read_back(q, k_cache, v_cache, block_table, causal, lengths)
         else:
             o, _ = paged_flash_attn_inference_func(q, k_cache, v_cache, block_table, cache_seqlens, causal)
