@@ -147,6 +147,18 @@ class Mlp(nn.Module):
         return self.fc2(self.act(self.fc1(x)))
 
 
+def _groups(lengths: Sequence[int], limit: int) -> List[Tuple[int, int]]:
+    """Neighbouring entries taken together, as (first, behind the last), as many as sum to ``limit``; a larger one is alone."""
+    out, total = [], 0
+    for i, n in enumerate(lengths):
+        if out and total + n <= limit:
+            out[-1], total = (out[-1][0], i + 1), total + n
+        else:
+            out.append((i, i + 1))
+            total = n
+    return out
+
+
 class DenseAttention(nn.Module):
     """Reference ``layers/attention.py:38-98`` (fused path): qkv, q/k LayerNorm, 2D RoPE,
     scaled-dot-product attention, proj. q/k LayerNorm + RoPE run in the HIP glue kernel.
@@ -211,6 +223,8 @@ class DenseAttention(nn.Module):
     # Over 112 shapes (16 and 4 heads of 64, 1 to 16 sequences of 1,374 to 100,000 keys, 64 to 1,374 new tokens) the rule takes 1.3 %
     # (4 bits: 0.7 %) more time than the better of the two; the number of new tokens alone, from 128 and 256 on, took 29 % (18 %).
     READ_BACK_FROM = ((80, 2.5e9), (300, 4e9))
+    # Keys and values read back at a time: sequences are taken together up to this size, and a longer one stays on its pages.
+    READ_BACK_BYTES = 1 << 30
 
     def _reads_back(self, new: int, lengths: Sequence[int], k_cache, dtype) -> bool:
         fp4 = isinstance(k_cache, FP4Cache)
@@ -219,14 +233,22 @@ class DenseAttention(nn.Module):
         least, work = self.READ_BACK_FROM[fp4]
         return (new - least) * sum(lengths) * self.num_heads * self.head_dim > work
 
-    def _attend_read_back(self, q, k_cache, v_cache, block_table, causal, lengths):
-        """q ``[B, N, H, D]`` over the kept keys read back as packed rows."""
-        B, N, H, D = q.shape
-        bounds = [0, *itertools.accumulate(lengths)]
-        cu_k = torch.tensor(bounds, dtype=torch.int32, device=q.device)
-        cu_q = torch.arange(0, (B + 1) * N, N, dtype=torch.int32, device=q.device)
-        k, v = paged_kv_read_func(k_cache, v_cache, block_table, cu_k, bounds[-1], dtype=q.dtype)
-        return packed_flash_attn_inference_func(q.reshape(B * N, H, D), k, v, cu_q, cu_k, causal)[0]
+    def _attend_read_back(self, q, k_cache, v_cache, block_table, cache_seqlens, causal, lengths):
+        """q ``[B, N, H, D]`` over the kept keys read back as packed rows, a group of sequences at a time."""
+        N, (H, D) = q.shape[1], q.shape[2:]
+        limit, out = self.READ_BACK_BYTES // (4 * H * D), []
+        for a, b in _groups(lengths, limit):
+            table, n = block_table[a:b], cache_seqlens[a:b]
+            bounds = [0, *itertools.accumulate(lengths[a:b])]
+            if bounds[-1] > limit:
+                o, _ = paged_flash_attn_inference_func(q[a:b], k_cache, v_cache, table, n, causal)
+            else:
+                cu_k = torch.tensor(bounds, dtype=torch.int32, device=q.device)
+                cu_q = torch.arange(0, (b - a + 1) * N, N, dtype=torch.int32, device=q.device)
+                k, v = paged_kv_read_func(k_cache, v_cache, table, cu_k, bounds[-1], dtype=q.dtype)
+                o, _ = packed_flash_attn_inference_func(q[a:b].reshape(-1, H, D), k, v, cu_q, cu_k, causal)
+            out.append(o.view(b - a, N, H, D))
+        return out[0] if len(out) == 1 else torch.cat(out)
 
     @torch.no_grad()
     def forward_cached(self, x, k_cache, v_cache, block_table, cache_seqlens, pos=None, axis_dims=None, bases=None,
@@ -257,7 +279,7 @@ class DenseAttention(nn.Module):
         turned = paged_kv_append_func(k, v, k_cache, v_cache, block_table, cache_seqlens, q=q if turn else None, **turn)
         q = turned if turn else q
         if lengths is not None and self._reads_back(N, lengths, k_cache, x.dtype):
-            o = self._attend_read_back(q, k_cache, v_cache, block_table, causal, lengths)
+            o = self._attend_read_back(q, k_cache, v_cache, block_table, cache_seqlens, causal, lengths)
         else:
             o, _ = paged_flash_attn_inference_func(q, k_cache, v_cache, block_table, cache_seqlens, causal)
         return self.proj(o.view(B, N, C))

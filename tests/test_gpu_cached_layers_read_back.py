@@ -31,6 +31,35 @@ def caches(fp4, pages, page, heads, d, dtype):
     return [torch.zeros(pages, page, heads, d, dtype=dtype, device="cuda") for _ in range(2)]
 
 
+def near(got, want, roundings):
+    """Two runs that round at different places: each of ``roundings`` steps by eps / 2 / sqrt(3) of the 2-norm of what it rounds,
+    independent in the two."""
+    assert torch.isfinite(got).all()
+    off = float((got.float() - want.float()).norm() / want.float().norm())
+    assert off <= (2 * roundings) ** 0.5 * torch.finfo(got.dtype).eps / 2 / 3 ** 0.5, off
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("limit,want", [(10 ** 9, [1700]), (700, [700, 640, 360]), (400, [300, 400, 360]), (350, [300, 350, 10])])
+def test_groups_of_sequences(gpu_device, reads, monkeypatch, fp4, limit, want):
+    """What is read back at a time is bounded; a sequence beyond the bound stays on its pages."""
+    g = torch.Generator().manual_seed(3)
+    m = layer(BF)
+    lengths, new, page, width = [300, 400, 640, 350, 10], 10, 16, 40
+    table = torch.randperm(5 * width, generator=g).to(torch.int32).view(5, width).cuda()
+    cache = caches(fp4, 5 * width, page, 4, 64, BF)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for b, length in enumerate(lengths):
+        x = torch.randn(1, length, 256, generator=g).to(BF).cuda()
+        m.forward_cached(x, *cache, table[b:b + 1], n[b:b + 1])
+    x = torch.randn(5, new, 256, generator=g).to(BF).cuda()
+    pages = m.forward_cached(x, *cache, table, n)
+    monkeypatch.setattr(agg.DenseAttention, "READ_BACK_BYTES", limit * 4 * 256)
+    got = m.forward_cached(x, *cache, table, n, lengths=lengths)
+    assert reads == want
+    near(got, pages, 3)
+
+
 def test_fp16_over_four_bits_stays_on_its_pages(gpu_device, reads):
     """Values near fp16's largest, kept as 65,536, of both signs: their mean is a number of fp16."""
     m = layer(HF, qk_norm=False)
