@@ -39,6 +39,64 @@ def near(got, want, roundings):
     assert off <= (2 * roundings) ** 0.5 * torch.finfo(got.dtype).eps / 2 / 3 ** 0.5, off
 
 
+@pytest.mark.parametrize("fp4,dtype", [(False, BF), (False, HF), (True, BF)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim,axes", [(256, (16, 24, 24)), (512, None)])
+@pytest.mark.parametrize("new,earlier", [(130, (900, 20)), (400, (1100, 0)), (1, (300, 64)), (257, (31, 1000))])
+def test_as_over_pages(gpu_device, reads, fp4, dtype, causal, dim, axes, new, earlier):
+    """New tokens behind earlier ones of sequences of different lengths. Roundings that differ: the weights', the output's, the
+    projection's."""
+    g = torch.Generator().manual_seed(1)
+    heads = dim // 64
+    m = layer(dtype, dim=dim, heads=heads)
+    page, width = 32, 50
+    table = torch.randperm(2 * width, generator=g).to(torch.int32).view(2, width).cuda()
+    cache = caches(fp4, 2 * width, page, heads, 64, dtype)
+    turn = lambda b, n: None if axes is None else torch.randint(0, 40, (b, n, 3), generator=g).to(torch.int32).cuda()  # noqa: E731
+    n = torch.tensor(earlier, dtype=torch.int32, device="cuda")
+    for b, length in enumerate(earlier):
+        if length:
+            x = torch.randn(1, length, dim, generator=g).to(dtype).cuda()
+            m.forward_cached(x, *cache, table[b:b + 1], n[b:b + 1], turn(1, length), axes)
+    n += new
+    lengths = [length + new for length in earlier]
+    x, pos = torch.randn(2, new, dim, generator=g).to(dtype).cuda(), turn(2, new)
+    pages = m.forward_cached(x, *cache, table, n, pos, axes, causal=causal)
+    assert not reads
+    got = m.forward_cached(x, *cache, table, n, pos, axes, causal=causal, lengths=lengths)
+    assert reads == [sum(lengths)]
+    near(got, pages, 3)
+    # every row, not the norm of all alone: a row that saw one key too many or too few would differ by far more
+    off = (got.float() - pages.float()).norm(dim=-1) / pages.float().norm(dim=-1)
+    assert off.max() <= 8 * torch.finfo(dtype).eps, float(off.max())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("qk_norm,axes", [(True, (16, 24, 24)), (False, None), (False, (32, 32))])
+def test_steps_are_the_whole_sequence(gpu_device, reads, dtype, qk_norm, axes):
+    """A causal layer on a sequence at once, and in blocks whose keys are read back. Roundings: projection, norm, rotation,
+    weights, o, output projection."""
+    g = torch.Generator().manual_seed(2)
+    m = layer(dtype, qk_norm)
+    total = 800
+    x = torch.randn(2, total, 256, generator=g).to(dtype).cuda()
+    pos = torch.randint(0, 40, (2, total, len(axes)), generator=g).to(torch.int32).cuda() if axes else None
+    page = 48
+    table = torch.randperm(34, generator=g).to(torch.int32).view(2, 17).cuda()
+    k, v = caches(False, 34, page, 4, 64, dtype)
+    lens, outs = torch.zeros(2, dtype=torch.int32, device="cuda"), []
+    blocks = ((0, 100), (100, 400), (400, 401), (401, 800))
+    for a, b in blocks:
+        lens.fill_(b)
+        outs.append(m.forward_cached(x[:, a:b], k, v, table, lens, None if pos is None else pos[:, a:b], axes, causal=True,
+                                     lengths=[b, b]))
+    assert reads == [2 * b for _, b in blocks]
+    got = torch.cat(outs, 1)
+    for i in range(2):
+        want = m.forward_train(x[i], None if pos is None else pos[i], None, axes, causal=True)
+        near(got[i], want.detach(), 6)
+
+
 @pytest.mark.parametrize("fp4", [False, True])
 @pytest.mark.parametrize("limit,want", [(10 ** 9, [1700]), (700, [700, 640, 360]), (400, [300, 400, 360]), (350, [300, 350, 10])])
 def test_groups_of_sequences(gpu_device, reads, monkeypatch, fp4, limit, want):
