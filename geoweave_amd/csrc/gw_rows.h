@@ -46,8 +46,8 @@ inline int64_t rows_tiles(bool paged, int64_t n, int64_t Tq, int64_t G, int64_t 
 }
 // Workspace of a split call. A tile is cut where its keys exceed the part length, so it has fewer than
 // two parts per part length of keys, and all cut tiles fewer than 2 want.
-inline size_t rows_workspace(int64_t tiles, int64_t Hk, int64_t D, int64_t rows = 16) {
-  return (size_t)2 * rows_want(Hk) * Hk * rows * (D + 1) * sizeof(float) + (size_t)tiles * sizeof(int2);
+inline size_t rows_workspace(int64_t tiles, int64_t Hk, int64_t D) {
+  return (size_t)2 * rows_want(Hk) * Hk * 16 * (D + 1) * sizeof(float) + (size_t)tiles * sizeof(int2);
 }
 // Workgroups of the attention launch. Packed: a sequence of at most kRowsMax rows has one or two tiles, and all have
 // no more than the rows in all allow.

@@ -1,5 +1,5 @@
-// Device pieces of the few-rows attention passes over 16-bit and 4-bit keys: which part of which sequence's keys a
-// workgroup takes, and the join of parts. Tiles are of ROWS rows (token, head of the group).
+// Device pieces of the few-rows attention passes: sequences, scans over a wave and the join of parts, for 16-bit and
+// 4-bit keys, and which part of which sequence's keys a workgroup takes, for 16-bit ones (4 bits: units, in their own pass).
 #pragma once
 
 #include "gw_packed.h"
@@ -10,7 +10,7 @@ namespace gw {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-constexpr int kRows = 16;  // rows of a tile; passes that keep more rows per key read name their own
+constexpr int kRows = 16;  // rows of a tile (token, head of the group); 4 bits: one or two tiles share a key read
 
 __device__ __forceinline__ f32x4 mma16(BF16, uint4 a, uint4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -88,36 +88,36 @@ struct RowsPart {
 };
 
 // Row tiles of a sequence: packed, those of the longer ones are another kernel's.
-template <bool PAGED, int ROWS = kRows>
+template <bool PAGED>
 __device__ __forceinline__ int rows_tiles_of(const RowsParams& p, const RowsSeq& s) {
   const int rows = s.lq * p.G;
-  return PAGED || rows <= kRowsMax ? (rows + ROWS - 1) / ROWS : 0;
+  return PAGED || rows <= kRowsMax ? (rows + kRows - 1) / kRows : 0;
 }
 
 // Keys of a part: about p.want parts over all row tiles.
-template <bool PAGED, int ROWS = kRows>
+template <bool PAGED>
 __device__ __forceinline__ int rows_part_len(const RowsParams& p, int lane) {
   const int nseq = rows_nseq<PAGED>(p);
   int64_t total = 0;
   for (int i = lane; i < nseq; i += 64) {
     const RowsSeq s = rows_seq<PAGED>(p, i);
-    total += (int64_t)rows_tiles_of<PAGED, ROWS>(p, s) * s.lk;
+    total += (int64_t)rows_tiles_of<PAGED>(p, s) * s.lk;
   }
   return rows_part_keys(wave_sum64(total), p.want);
 }
 
 // The part of slot `slot`.
-template <bool PAGED, int ROWS = kRows>
+template <bool PAGED>
 __device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, int lane) {
   RowsPart r = {-1, 0, 0, 1, 0, 0x7fffff00};
   if (!p.split) {  // paged only: as many row tiles in each sequence
-    const int rt = (p.Tq * p.G + ROWS - 1) / ROWS;
+    const int rt = (p.Tq * p.G + kRows - 1) / kRows;
     r.seq = slot / rt;
     r.tile = slot - r.seq * rt;
     if (r.seq >= p.n) r.seq = -1;
     return r;
   }
-  r.len = __builtin_amdgcn_readfirstlane(rows_part_len<PAGED, ROWS>(p, lane));
+  r.len = __builtin_amdgcn_readfirstlane(rows_part_len<PAGED>(p, lane));
   const int nseq = rows_nseq<PAGED>(p);
   int before = 0, cut_before = 0;
   for (int i0 = 0; i0 < nseq; i0 += 64) {
@@ -125,7 +125,7 @@ __device__ __forceinline__ RowsPart rows_find(const RowsParams& p, int slot, int
     int tiles = 0, parts = 1;
     if (i < nseq) {
       const RowsSeq s = rows_seq<PAGED>(p, i);
-      tiles = rows_tiles_of<PAGED, ROWS>(p, s);
+      tiles = rows_tiles_of<PAGED>(p, s);
       parts = rows_parts(s.lk, r.len);
     }
     const int mine = tiles * parts, cut = parts > 1 ? mine : 0;
@@ -157,11 +157,10 @@ __device__ __forceinline__ float rows_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// Joins the parts of one row of a cut row tile. D / 4 threads hold four dims each; the groups of them
-// take the parts in turn, each part's row one 16-byte load per thread, and are summed in group order.
 constexpr int kJoinParts = 1024;  // weights kept in LDS at a time
 
-//
+// Joins the parts of one row of a cut row tile of ROWS rows. D / 4 threads hold four dims each; the groups of them
+// take the parts in turn, each part's row one 16-byte load per thread, and are summed in group order.
 // UNITS: a row tile's first part is in slot cut.x (odd), the i-th behind it in slot cut.x + 2 i - 1.
 template <typename E, int D, bool PAGED, int ROWS = kRows, bool UNITS = false>
 __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p) {
