@@ -134,3 +134,23 @@ def test_fp16_over_four_bits_stays_on_its_pages(gpu_device, reads):
     assert not reads
     # 64 more of one sign, of 320: -65,536 / 5, rounded once to fp16
     assert torch.equal(got, torch.full_like(got, -65536.0 / 5))
+
+
+@pytest.mark.parametrize("limit", [10 ** 9, 400, 0])
+def test_sequences_of_no_keys(gpu_device, reads, monkeypatch, limit):
+    """Beside others, in a group of their own, and behind one that stays on its pages."""
+    g = torch.Generator().manual_seed(4)
+    m = layer(BF)
+    lengths = [0, 640, 0, 0, 30]
+    table = torch.randperm(200, generator=g).to(torch.int32).view(5, 40).cuda()
+    cache = caches(False, 200, 16, 4, 64, BF)
+    for c in cache:
+        c.copy_(torch.randn(c.shape, generator=g))
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    x = torch.randn(5, 10, 256, generator=g).to(BF).cuda()
+    pages = m.forward_cached(x, *cache, table, n)
+    monkeypatch.setattr(agg.DenseAttention, "READ_BACK_BYTES", limit * 4 * 256)
+    got = m.forward_cached(x, *cache, table, n, lengths=lengths)
+    assert sum(reads) == {10 ** 9: 670, 400: 30, 0: 0}[limit]
+    near(got, pages, 3)
+    assert torch.equal(got[[0, 2, 3]], m.proj.bias.detach().expand(3, 10, 256))
