@@ -1,7 +1,6 @@
 // The 4-bit format of a paged cache: e2m1 values (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign; two to a byte, the first in the
 // low half) with one power of two for each 32 of a row (a biased exponent in a byte, 255: not a number). It is
-// the matrix cores' own block format, so keys enter a product as they lie in memory and values take one conversion
-// for two.
+// the matrix cores' own block format: two values become 16-bit ones by one instruction.
 //
 // The power of two is the one that brings the largest of the 32 to (3.5, 7]: then no value is off by more than one
 // unit, half the widest step (4 to 6; a largest of up to 7 becomes 6). Over normal rows the rms error is 0.112 of

@@ -28,8 +28,9 @@
 // lanes that need them (the 32 streams in pages of 100: 469 to 495 us).
 //
 // Bound by memory where rows are few: those 32 streams 414 us of the kernel alone, 5.2 TB/s; one token of 64 sequences to
-// 32,976 keys, 32 heads over 8 of 128, pages of 16: 113 to 117 us, 5.0 TB/s. With 64 rows over a key (8 tokens x 8 heads) by the
-// vector unit and the matrix cores alike: 72 us for 31 GFLOP; four row tiles to a wave (one wave per SIMD) took 87 for 82.
+// 32,976 keys, 32 heads over 8 of 128, pages of 16: 113 to 117 us, 5.0 TB/s. With 64 rows over a key (8 tokens x 8 heads) no
+// unit is full (vector unit 49 % busy, matrix cores 26 %; two waves per SIMD wait for data and for each other; a key is
+// converted twice): 73 us for 31 GFLOP; four row tiles to a wave (one wave per SIMD) took 87 for 82.
 //
 // Rows that are not keys (behind the length, in a page outside the pool) are masked, and their scales count as 2^-127:
 // what lies there cannot reach a result. A masked weight is 0, but 0 * inf is NaN, so values of V that are no finite number (gw_fp4.h:

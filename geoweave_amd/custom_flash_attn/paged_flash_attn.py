@@ -20,7 +20,7 @@ Table and lengths are read by the kernels only.
 
 The caches may also be a pair of ``paged_kv_cache.FP4Cache``: the same attention over the values that 4 bits hold, at a
 quarter of the bytes. They enter the products exactly, and the weights keep 16 bits. 32 values kept as not a number
-are NaN in the rows that see them.
+are NaN, and values of 2^128 and above inf, in the rows that see them.
 """
 from __future__ import annotations
 

@@ -175,7 +175,7 @@ def paged_kv_append_func(k: torch.Tensor, v: torch.Tensor, k_cache: Cache, v_cac
 
     ``positions`` (``k.shape[:-2] + (A,)``, int32, int64 or float32) and ``axis_dims`` (of A axes) turn k and q as
     ``rotary_axes_func`` does, with ``bases``; without them nothing is turned. The result is rounded once,
-    to the tokens' type or to 4 bits; 32 dims with an inf or NaN are kept as NaN in 4 bits.
+    to the tokens' type or to 4 bits; 32 dims with an inf or NaN are kept as NaN in 4 bits, bf16 values above 3.5 * 2^126 as inf.
 
     A token whose key has no slot (below 0, behind the table, in a page outside the pool) and a token of no
     sequence is written nowhere; its q is turned all the same. Two new tokens that come to one slot (pages that

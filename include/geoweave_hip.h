@@ -765,7 +765,8 @@ int gw_paged_kv_read(int dtype, int cache_format, const void* k_cache, const int
 /* ------------------------------------------------------------------------------------
  * gw_paged_attn_fwd over a cache of GW_CACHE_FP4: the same formulas over the values that the codes stand for,
  * with the same arguments, limits and rules; k and v are codes and scales as in gw_paged_kv_append, of at most 2^36 bytes of
- * codes each. All values enter the products exactly, the weights as two bf16 terms.
+ * codes each. All values enter the products exactly, the weights as two bf16 terms. Values of 2^128 and above are inf; values of v
+ * that are no finite number reach only the rows that see their key.
  * ------------------------------------------------------------------------------------ */
 size_t gw_paged_attn_fp4_fwd_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D);
 int gw_paged_attn_fp4_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
